@@ -334,6 +334,68 @@ int nats_b200_decode_step(const void* d_q, const void* d_k_new, const void* d_v_
                           int max_len_bound, int B, int Hq, int Hkv, int D, int C, int SW, float sm_scale,
                           void* d_workspace, size_t workspace_bytes, void* stream);
 
+/* ------------------------------------------------------------------------------------------------
+ * The paged cache: K and V of every (slot, kv-head) in pages of one chunk each, out of one pool.  Nothing like it in the reference, whose
+ * cache pads every head to the longest one and moves rows when it evicts; here eviction gives pages back and a fork shares them.
+ *
+ *   d_pages_k, d_pages_v  bf16 [num_pages, page_size, head_dim]
+ *   d_refs                int32 [num_pages]: rows that hold a page (0: free)
+ *   d_free_bits           uint32 [ceil(num_pages / 32)]: bit p is set where page p is free (bits behind the last page: 0)
+ *   d_entries             int32 [slots, n_kv_heads, max_entries, 4], the first d_n_pages of a row in use, in the order of positions:
+ *                         page, position of its first token, last query position that may see it, 0
+ *                         (limit 2^31 - 1: for good; 2^31 - 2: a local chunk that no completed global chunk has closed yet)
+ *   d_n_pages             int32 [slots, n_kv_heads]
+ *   d_length              int32 [slots]: tokens so far.  Where it is no multiple of the page size, the last page of each of the slot's
+ *                         rows is the unfinished chunk: it has no limit and no other holder.
+ * page_size 16, 32, 64 or 128; head_dim 64 or 128; slots * n_kv_heads <= 65535; num_pages <= 2^24.  Page numbers are checked where they are
+ * read: a bad one counts as a page that is not there.  The status word (see prefill) takes 64: no free page left, 65: no entry left,
+ * 66: a slot number out of range; the tables then hold what could be done, and are to be thrown away.
+ * Workspaces must be zero in front of their first use and belong to one stream at a time.
+ */
+typedef struct NatsPagedKV {
+    void* d_pages_k; void* d_pages_v;
+    int32_t* d_refs; uint32_t* d_free_bits;
+    int32_t* d_entries; int32_t* d_n_pages; int32_t* d_length;
+    int num_pages, page_size, head_dim, slots, n_kv_heads, max_entries;
+} NatsPagedKV;
+
+/* New tokens into pages: every slot's first d_n_new[slot] (NULL: N) of the N tokens of d_k, d_v (bf16, or fp32 with f32 != 0, which are
+ * rounded; element (slot, head, token, d) at slot * slot_stride + head * head_stride + token * token_stride + d, strides keeping 16-byte
+ * alignment).  d_roles uint8 [slots, n_kv_heads, n_roles] describes the chunks from a slot's unfinished one on; chunks behind them, and a chunk
+ * that stays unfinished, count as global.  A completed chunk gets its limit: none if global, c * page_size + SW + page_size - 1 if sliding
+ * (c: its number), the end of the next completed global chunk if local, which closes local chunks of earlier calls too.
+ * Free pages are taken from the lowest on in the order (slot, kv-head, chunk).  skip_hidden != 0: whole chunks that no query behind this call
+ * sees are not stored (a prompt whose attention does not read the pages).
+ */
+size_t nats_b200_paged_append_workspace_bytes(int slots, int n_kv_heads, int N, int page_size);
+int nats_b200_paged_append(const NatsPagedKV* kv, const void* d_k, const void* d_v, long long k_slot_stride, long long k_head_stride,
+                           long long k_token_stride, long long v_slot_stride, long long v_head_stride, long long v_token_stride,
+                           int f32, const uint8_t* d_roles, int n_roles, const int32_t* d_n_new, int N, int SW, int skip_hidden,
+                           void* d_workspace, size_t workspace_bytes, int32_t* d_status, void* stream);
+
+/* Attention of the last d_n_new[slot] (NULL: N) tokens of every slot, whose K and V are in the pages.  q bf16 and o (bf16, or fp32 with
+ * o_f32 != 0) are [slots, n_heads, N, head_dim] with the strides given, the last axis dense.  Row i of a slot is the token at position
+ * length - n_new + i; rows behind the slot's new tokens, and rows that see no key, are written as zero.  max_pages: a bound of d_n_pages (work is
+ * split by it; where it is too low the result stays right).  A value that is not finite in a V row reaches the rows of the call that
+ * share a 128-key tile with it from its own position on or not at all only where its page is hidden from all of them.
+ */
+size_t nats_b200_paged_attention_workspace_bytes(int slots, int n_heads, int n_kv_heads, int N, int head_dim, int page_size, int max_pages);
+int nats_b200_paged_attention(const NatsPagedKV* kv, const void* d_q, long long q_slot_stride, long long q_head_stride, long long q_token_stride,
+                              void* d_o, long long o_slot_stride, long long o_head_stride, long long o_token_stride, int o_f32,
+                              const int32_t* d_n_new, int n_heads, int N, int max_pages, float sm_scale, void* d_workspace,
+                              size_t workspace_bytes, int32_t* d_status, void* stream);
+
+/* Pages that the next query position (d_length) cannot see leave the rows; a page that loses its last holder is free again. */
+int nats_b200_paged_evict(const NatsPagedKV* kv, void* stream);
+
+/* Every slot s becomes a copy of what slot d_src[s] (int32 [slots]) was; -1: an empty one.  Whole pages are shared; the unfinished page
+ * stays with its own slot if that keeps its sequence, else with the first slot that takes it, and is copied for the others, into the lowest
+ * free pages in the order (slot, kv-head), those that the call gives back among them.
+ */
+size_t nats_b200_paged_reorder_workspace_bytes(int slots, int n_kv_heads, int max_entries);
+int nats_b200_paged_reorder(const NatsPagedKV* kv, const int32_t* d_src, void* d_workspace, size_t workspace_bytes, int32_t* d_status,
+                            void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -12,6 +12,14 @@ LIB_PATH = os.environ.get('NATS_B200_LIB') or os.path.join(_HERE, 'libnats_b200.
 _c = ctypes
 _P, _I, _F, _SZ = _c.c_void_p, _c.c_int, _c.c_float, _c.c_size_t
 
+_LL = _c.c_longlong
+
+
+class NatsPagedKV(_c.Structure):
+    _fields_ = [(n, _P) for n in ('d_pages_k', 'd_pages_v', 'd_refs', 'd_free_bits', 'd_entries', 'd_n_pages', 'd_length')] + \
+               [(n, _I) for n in ('num_pages', 'page_size', 'head_dim', 'slots', 'n_kv_heads', 'max_entries')]
+
+
 # name -> (restype, argtypes); mirrors include/nats_b200.h
 SIGNATURES = {
     'nats_b200_last_error': (_c.c_char_p, []),
@@ -46,6 +54,13 @@ SIGNATURES = {
     'nats_b200_decode_step_fwd': (_I, [_P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _SZ, _P]),
     'nats_b200_decode_step_place': (_I, [_P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     'nats_b200_decode_step': (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _SZ, _P]),
+    'nats_b200_paged_append_workspace_bytes': (_SZ, [_I, _I, _I, _I]),
+    'nats_b200_paged_append': (_I, [_P, _P, _P, _LL, _LL, _LL, _LL, _LL, _LL, _I, _P, _I, _P, _I, _I, _I, _P, _SZ, _P, _P]),
+    'nats_b200_paged_attention_workspace_bytes': (_SZ, [_I, _I, _I, _I, _I, _I, _I]),
+    'nats_b200_paged_attention': (_I, [_P, _P, _LL, _LL, _LL, _P, _LL, _LL, _LL, _I, _P, _I, _I, _I, _F, _P, _SZ, _P, _P]),
+    'nats_b200_paged_evict': (_I, [_P, _P]),
+    'nats_b200_paged_reorder_workspace_bytes': (_SZ, [_I, _I, _I]),
+    'nats_b200_paged_reorder': (_I, [_P, _P, _P, _SZ, _P, _P]),
     'nats_b200_decode_place': (_I, [_P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
 }
 

@@ -1,0 +1,32 @@
+// What the operators of the paged cache share.
+//
+// K and V lie in pages of P consecutive tokens of one (sequence, kv-head); a page is one chunk of the role rule.  A slot (a sequence) has a
+// row of entries per kv-head: int4 (page, position of its first token, last query position that may see it, 0) in the order of positions.
+// Only the last page of a row may be part filled, and nobody else holds that page.  refs counts the rows that hold a page; a page that
+// nobody holds has its bit set in free_bits.
+#pragma once
+#include "common.cuh"
+
+namespace nats {
+
+constexpr int32_t kOpenLocal = kNoLimit - 1;     // limit of a local chunk that no completed global chunk has closed yet
+
+// codes of the status word
+constexpr int kErrNoPage = 64, kErrNoEntry = 65, kErrSlot = 66;
+
+struct PagedKv {
+    uint8_t* k; uint8_t* v;                      // [num_pages, P, D] bf16
+    int32_t* refs;                               // [num_pages]
+    uint32_t* free_bits;                         // [ceil(num_pages / 32)]
+    int4* entries;                               // [S, H, M]
+    int32_t* n_pages;                            // [S, H]
+    int32_t* length;                             // [S]
+    int num_pages, P, D, S, H, M;
+};
+
+// checks what every entry point is given and fills the above
+int paged_kv(const NatsPagedKV* d, PagedKv& kv);
+
+__device__ __forceinline__ void paged_status(int32_t* status, int code) { atomicCAS(status, 0, code); }
+
+}  // namespace nats

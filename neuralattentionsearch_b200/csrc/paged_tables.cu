@@ -1,0 +1,521 @@
+// Page tables of the paged cache: new tokens into pages, pages given back, sequences forked, moved and dropped.
+//
+// A page is never moved: eviction shortens a row of entries, a fork copies the row and counts the pages once more.  What has to be copied is
+// the unfinished page, which its holder goes on writing.
+//
+// Free pages are handed out from the lowest one on in the order (slot, kv-head, chunk), whatever order the blocks run in: every block knows the
+// ranks of its pages from the lengths (or the counts) of the rows in front and picks the set bits of those ranks; the block that ends last
+// clears them.  All these kernels are bound by latency, but for the copy of many tokens, which HBM bounds.
+#include "paged.cuh"
+
+namespace nats {
+
+constexpr int kTabThreads = 256;
+constexpr int kTabWarps = kTabThreads / 32;
+constexpr int kCopyTokens = 64;                  // tokens per block of the copy kernel
+constexpr int kMaxSlots = 4096;
+
+// Exclusive prefix sum over the block and the sum; every thread calls it.  `s_part` is free again behind the caller's next barrier.
+__device__ __forceinline__ int block_scan(int v, int& total, int (&s_part)[kTabWarps]) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int incl = warp_incl_scan(v, lane);
+    if (lane == 31) s_part[warp] = incl;
+    __syncthreads();
+    int before = 0;
+    total = 0;
+#pragma unroll
+    for (int w = 0; w < kTabWarps; ++w) {
+        if (w < warp) before += s_part[w];
+        total += s_part[w];
+    }
+    __syncthreads();
+    return before + incl - v;
+}
+
+// Sums of two values over the block
+__device__ __forceinline__ void block_sum2(int& a, int& b, int (&s_a)[kTabWarps], int (&s_b)[kTabWarps]) {
+    a = __reduce_add_sync(0xffffffffu, a);
+    b = __reduce_add_sync(0xffffffffu, b);
+    if ((threadIdx.x & 31) == 0) { s_a[threadIdx.x >> 5] = a; s_b[threadIdx.x >> 5] = b; }
+    __syncthreads();
+    a = b = 0;
+#pragma unroll
+    for (int w = 0; w < kTabWarps; ++w) { a += s_a[w]; b += s_b[w]; }
+    __syncthreads();
+}
+
+// Walks the free pages of rank [r0, r1), the lowest free page having rank 0: f(rank, page).  Returns min(r1, free pages) - r0 (or less than 0).
+template <class F>
+__device__ __forceinline__ int for_free(const PagedKv& kv, int r0, int r1, int (&s_part)[kTabWarps], F f) {
+    const int words = (kv.num_pages + 31) / 32;
+    int base = 0;
+    for (int w0 = 0; w0 < words && base < r1; w0 += 4 * kTabThreads) {
+        uint32_t word[4];
+        int n = 0;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int w = w0 + 4 * threadIdx.x + j;
+            word[j] = w < words ? kv.free_bits[w] : 0u;
+            if (w == words - 1 && (kv.num_pages & 31)) word[j] &= (1u << (kv.num_pages & 31)) - 1u;
+            n += __popc(word[j]);
+        }
+        int total;
+        int rank = base + block_scan(n, total, s_part);
+        if (rank + n > r0 && rank < r1) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                for (uint32_t m = word[j]; m != 0u; m &= m - 1u, ++rank)
+                    if (rank >= r0 && rank < r1) f(rank, (w0 + 4 * (int)threadIdx.x + j) * 32 + __ffs(m) - 1);
+        }
+        base += total;
+    }
+    return min(base, r1) - r0;
+}
+
+// The block that ends last takes the lowest `total` free pages out of the free ones (all others have picked theirs).
+__device__ __forceinline__ bool last_block(int32_t* ticket, int n_blocks) {
+    __shared__ int s_last;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        __threadfence();
+        s_last = atomicAdd(ticket, 1) == n_blocks - 1;
+        if (s_last) *ticket = 0;
+        __threadfence();
+    }
+    __syncthreads();
+    return s_last != 0;
+}
+__device__ __forceinline__ void take_lowest(const PagedKv& kv, int total, int (&s_part)[kTabWarps]) {
+    if (total > 0) for_free(kv, 0, total, s_part, [&](int, int page) { atomicAnd(&kv.free_bits[page >> 5], ~(1u << (page & 31))); });
+}
+
+__device__ __forceinline__ void give_back(const PagedKv& kv, int page) {
+    if ((unsigned)page < (unsigned)kv.num_pages && atomicSub(&kv.refs[page], 1) == 1) atomicOr(&kv.free_bits[page >> 5], 1u << (page & 31));
+}
+
+// =================================================================================================
+// append
+// =================================================================================================
+struct AppendParams {
+    PagedKv kv;
+    const uint8_t* k; const uint8_t* v;
+    long long k_slot, k_head, k_token, v_slot, v_head, v_token;      // strides in elements
+    int f32;
+    const uint8_t* roles;                        // [S, H, n_roles]: of the chunks from the unfinished one on
+    int n_roles;
+    const int32_t* n_new;                        // [S] or nullptr: N everywhere
+    int N, SW, n_chunks;                         // n_chunks: the most chunks that N tokens touch
+    int copy_here;                               // the blocks of the table kernel copy the tokens as well
+    int32_t* ticket;
+    int32_t* counts;                             // [S * H]           new pages of a row (only where hidden chunks are skipped)
+    int32_t* ids;                                // [S * H, n_chunks] pages that a row takes
+    int32_t* map;                                // [S * H, n_chunks] page of every chunk of the call, -1: not stored
+    int32_t* status;
+};
+
+struct AppendRow { int s, h, old, n, fill, chunks; };
+__device__ __forceinline__ int new_tokens(const AppendParams& p, int s) { return p.n_new == nullptr ? p.N : min(max(p.n_new[s], 0), p.N); }
+__device__ __forceinline__ AppendRow append_row(const AppendParams& p, int row) {
+    AppendRow r;
+    r.s = row / p.kv.H; r.h = row - r.s * p.kv.H;
+    r.old = p.kv.length[r.s]; r.n = new_tokens(p, r.s);
+    r.fill = r.old % p.kv.P;
+    r.chunks = r.n > 0 ? (r.fill + r.n + p.kv.P - 1) / p.kv.P : 0;
+    return r;
+}
+// pages that a row takes if every new chunk gets one: the same for all heads of a slot
+__device__ __forceinline__ int pages_taken(const AppendParams& p, int s) {
+    const int n = new_tokens(p, s), fill = p.kv.length[s] % p.kv.P;
+    return n > 0 ? (fill + n + p.kv.P - 1) / p.kv.P - (fill > 0) : 0;
+}
+
+// Goes over the chunks of a call, tile by tile from the last one: f(i, chunk is there, last query position that may see it).
+// Returns the first completed global chunk of the call (-1: none).  limit of a chunk c: none if it is global or unfinished,
+// c P + SW + P - 1 if sliding, the end of the next completed global chunk if local.
+template <class F>
+__device__ __forceinline__ int for_chunks(const AppendParams& p, const AppendRow& r, F f) {
+    __shared__ unsigned s_global[kTabWarps];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, P = p.kv.P, c0 = r.old / P;
+    const uint8_t* roles = p.roles + ((size_t)r.s * p.kv.H + r.h) * p.n_roles;
+    int after = -1;                              // first completed global chunk behind the tile
+    for (int t0 = (r.chunks - 1) / kTabThreads * kTabThreads; t0 >= 0 && r.chunks > 0; t0 -= kTabThreads) {
+        const int i = t0 + threadIdx.x, c = c0 + i;
+        const bool there = i < r.chunks;
+        const int role = there && i < p.n_roles ? roles[i] : NATS_ROLE_GLOBAL;
+        const bool done = there && (long long)(c + 1) * P <= (long long)r.old + r.n;
+        const unsigned own = __ballot_sync(0xffffffffu, done && role == NATS_ROLE_GLOBAL);
+        if (lane == 0) s_global[warp] = own;
+        __syncthreads();
+        int next = -1, first = after;
+        if (own >> lane) next = c + __ffs(own >> lane) - 1;
+#pragma unroll
+        for (int w = kTabWarps - 1; w >= 0; --w) {
+            const unsigned g = s_global[w];
+            if (g != 0u) first = c0 + t0 + 32 * w + __ffs(g) - 1;
+            if (w == warp + 1 && next < 0) next = first;
+        }
+        if (warp == kTabWarps - 1 && next < 0) next = after;
+        long long limit = kNoLimit;
+        if (done && role != NATS_ROLE_GLOBAL) {
+            limit = role == NATS_ROLE_SLIDING ? (long long)c * P + p.SW + P - 1 : next >= 0 ? (long long)(next + 1) * P - 1 : kOpenLocal;
+            if (limit > kOpenLocal) limit = kOpenLocal;
+        }
+        f(i, there, (int)limit);
+        after = first;
+        __syncthreads();
+    }
+    return after;
+}
+
+// Pages that a row takes if chunks that no later query sees are not stored
+__global__ void __launch_bounds__(kTabThreads) paged_count_kernel(const AppendParams p) {
+    __shared__ int s_a[kTabWarps], s_b[kTabWarps];
+    const AppendRow r = append_row(p, blockIdx.x);
+    int n = 0, none = 0;
+    for_chunks(p, r, [&](int i, bool there, int limit) { n += there && !(i == 0 && r.fill > 0) && limit >= r.old + r.n; });
+    block_sum2(n, none, s_a, s_b);
+    if (threadIdx.x == 0) p.counts[blockIdx.x] = n;
+}
+
+// Token rows [t0, t1) of a row into their pages.  Four vectors of K and of V are on their way before the first is stored.
+__device__ __forceinline__ uint4 load_row8(const uint8_t* base, long long at, int f32) {
+    if (!f32) return ld16_stream(base + 2 * at);
+    return round8(ld16_stream(base + 4 * at), ld16_stream(base + 4 * at + 16));
+}
+__device__ __forceinline__ void copy_tokens(const AppendParams& p, const AppendRow& r, int row, int t0, int t1) {
+    const int vecs = p.kv.D / 8, P = p.kv.P, c0 = r.old / P;
+    const int32_t* map = p.map + (size_t)row * p.n_chunks;
+    const long long kb = r.s * p.k_slot + r.h * p.k_head, vb = r.s * p.v_slot + r.h * p.v_head;
+    const int n = (t1 - t0) * vecs;
+    for (int i0 = threadIdx.x; i0 < n; i0 += 4 * kTabThreads) {
+        uint4 a[4], b[4];
+        size_t to[4];
+        bool ok[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int i = i0 + j * kTabThreads, t = t0 + i / vecs, c = i % vecs;
+            ok[j] = i < n;
+            if (!ok[j]) continue;
+            const int pos = r.old + t, page = map[pos / P - c0];
+            ok[j] = page >= 0;
+            to[j] = (((size_t)page * P + pos % P) * p.kv.D + c * 8) * 2;
+            if (!ok[j]) continue;
+            a[j] = load_row8(p.k, kb + t * p.k_token + c * 8, p.f32);
+            b[j] = load_row8(p.v, vb + t * p.v_token + c * 8, p.f32);
+        }
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+            if (ok[j]) { st16(p.kv.k + to[j], a[j]); st16(p.kv.v + to[j], b[j]); }
+    }
+}
+
+// One block per (slot, kv-head): takes pages, writes the entries of the call's chunks, closes the open local ones, copies few tokens.
+template <bool SKIP>
+__global__ void __launch_bounds__(kTabThreads) paged_append_kernel(const AppendParams p) {
+    __shared__ int s_a[kTabWarps], s_b[kTabWarps];
+    const PagedKv& kv = p.kv;
+    const int row = blockIdx.x, tid = threadIdx.x, rows = kv.S * kv.H;
+    const AppendRow r = append_row(p, row);
+    // ranks of this row's pages among all that the call takes
+    int base = 0, total = 0;
+    if (SKIP) {
+        for (int i = tid; i < rows; i += kTabThreads) { const int n = p.counts[i]; total += n; if (i < row) base += n; }
+    } else {
+        for (int s = tid; s < kv.S; s += kTabThreads) { const int n = pages_taken(p, s) * kv.H; total += n; if (s < r.s) base += n; }
+    }
+    block_sum2(base, total, s_a, s_b);
+    const int take = SKIP ? p.counts[row] : pages_taken(p, r.s);
+    if (!SKIP) base += r.h * take;
+    int32_t* ids = p.ids + (size_t)row * p.n_chunks;
+    int room = 0;
+    if (take > 0) {
+        const int found = for_free(kv, base, base + take, s_a, [&](int rank, int page) { ids[rank - base] = page; });
+        room = min(max(found, 0), take);
+        __syncthreads();
+    }
+    int4* entries = kv.entries + (size_t)row * kv.M;
+    const int n0 = min(max(kv.n_pages[row], 0), kv.M);
+    if (tid == 0 && room < take) paged_status(p.status, kErrNoPage);
+    if (room > kv.M - n0) {
+        if (tid == 0) paged_status(p.status, kErrNoEntry);
+        room = kv.M - n0;
+    }
+    const bool tail = r.fill > 0 && n0 > 0 && entries[n0 - 1].y == r.old - r.fill;
+    int32_t* map = p.map + (size_t)row * p.n_chunks;
+    int behind = 0;                              // SKIP: stored chunks behind the tile
+    const int closing = for_chunks(p, r, [&](int i, bool there, int limit) {
+        const bool fresh = there && !(i == 0 && r.fill > 0);
+        int k = i - (r.fill > 0);
+        bool stored = fresh;
+        if (SKIP) {
+            stored = fresh && limit >= r.old + r.n;
+            int in_tile;
+            const int in_front = block_scan(stored ? 1 : 0, in_tile, s_a);
+            k = take - behind - in_tile + in_front;
+            behind += in_tile;
+        }
+        int page = -1;
+        if (stored && k < room) {
+            page = ids[k];
+            entries[n0 + k] = make_int4(page, (r.old / kv.P + i) * kv.P, limit, 0);
+            kv.refs[page] = 1;
+        } else if (there && !fresh && tail) {
+            page = entries[n0 - 1].x;
+            entries[n0 - 1].z = limit;
+            if ((unsigned)page >= (unsigned)kv.num_pages) page = -1;
+        }
+        if (there) map[i] = page;
+    });
+    if (closing >= 0)
+        for (int e = tid; e < n0; e += kTabThreads)
+            if (entries[e].z == kOpenLocal) entries[e].z = (int)min((long long)(closing + 1) * kv.P - 1, (long long)kOpenLocal - 1);
+    if (tid == 0) kv.n_pages[row] = n0 + room;
+    if (p.copy_here) {
+        __syncthreads();
+        copy_tokens(p, r, row, 0, r.n);
+    }
+    if (!last_block(p.ticket, rows)) return;
+    take_lowest(kv, total, s_a);
+    for (int s = tid; s < kv.S; s += kTabThreads) kv.length[s] += new_tokens(p, s);
+}
+
+__global__ void __launch_bounds__(kTabThreads) paged_copy_kernel(const AppendParams p) {
+    AppendRow r = append_row(p, blockIdx.y);
+    r.old -= r.n;                                // the table kernel has moved the lengths on
+    const int t0 = blockIdx.x * kCopyTokens;
+    if (t0 < r.n) copy_tokens(p, r, blockIdx.y, t0, min(t0 + kCopyTokens, r.n));
+}
+
+// =================================================================================================
+// evict
+// =================================================================================================
+// One block per (slot, kv-head): entries that the next query position (the length) cannot see leave the row, their pages are given back.
+__global__ void __launch_bounds__(kTabThreads) paged_evict_kernel(const PagedKv kv) {
+    __shared__ int s_part[kTabWarps];
+    const int row = blockIdx.x, s = row / kv.H;
+    int4* entries = kv.entries + (size_t)row * kv.M;
+    const int next = kv.length[s], n = min(max(kv.n_pages[row], 0), kv.M);
+    int out = 0;
+    for (int t0 = 0; t0 < n; t0 += kTabThreads) {
+        const int i = t0 + threadIdx.x;
+        const int4 e = i < n ? entries[i] : make_int4(0, 0, 0, 0);
+        const bool keep = i < n && e.z >= next;
+        int kept;
+        const int at = out + block_scan(keep ? 1 : 0, kept, s_part);       // its barriers: the tile has been read before any of it is written
+        if (keep && at != i) entries[at] = e;
+        if (i < n && !keep) give_back(kv, e.x);
+        out += kept;
+    }
+    if (threadIdx.x == 0 && out != n) kv.n_pages[row] = out;
+}
+
+// =================================================================================================
+// reorder
+// =================================================================================================
+// Slot s becomes a copy of what slot src[s] was (-1: empty).  Two kernels: the first counts the pages for their new holders, gives back
+// those that lose all of theirs and saves the rows that move; the second writes the moved rows and copies unfinished pages.  An unfinished
+// page stays with its own slot if that keeps its sequence, else with the first slot that takes it; the others get a page of their own.
+struct ReorderParams {
+    PagedKv kv;
+    const int32_t* src;                          // [S]
+    int32_t* ticket;
+    int4* entries;                               // [S, H, M]: rows that move
+    int32_t* n_pages;                            // [S, H]: as they were
+    int32_t* length;                             // [S]
+    int32_t* status;
+};
+
+__global__ void __launch_bounds__(kTabThreads) paged_release_kernel(const ReorderParams p) {
+    __shared__ int s_a[kTabWarps], s_b[kTabWarps];
+    const PagedKv& kv = p.kv;
+    const int row = blockIdx.x, s = row / kv.H, tid = threadIdx.x;
+    int uses = 0, bad = 0;
+    for (int i = tid; i < kv.S; i += kTabThreads) {
+        const int o = p.src[i];
+        uses += o == s;
+        bad |= o < -1 || o >= kv.S;
+    }
+    block_sum2(uses, bad, s_a, s_b);
+    if (bad && tid == 0) paged_status(p.status, kErrSlot);
+    const int n = min(max(kv.n_pages[row], 0), kv.M), length = kv.length[s];
+    const bool moves = uses > (p.src[s] == s ? 1 : 0);
+    if (tid == 0) {
+        p.n_pages[row] = n;
+        if (row == s * kv.H) p.length[s] = length;
+    }
+    if (!moves && uses == 1) return;
+    const int4* from = kv.entries + (size_t)row * kv.M;
+    int4* to = p.entries + (size_t)row * kv.M;
+    for (int i = tid; i < n; i += kTabThreads) {
+        const int4 e = from[i];
+        if (moves) to[i] = e;
+        if ((unsigned)e.x >= (unsigned)kv.num_pages) continue;
+        if (uses == 0) give_back(kv, e.x);
+        else if (uses > 1 && !(i == n - 1 && length % kv.P != 0)) atomicAdd(&kv.refs[e.x], uses - 1);
+    }
+}
+
+__global__ void __launch_bounds__(kTabThreads) paged_move_kernel(const ReorderParams p) {
+    __shared__ int s_a[kTabWarps], s_b[kTabWarps];
+    __shared__ int s_page;
+    extern __shared__ int s_first[];             // [S]: the slot that an unfinished page stays with
+    const PagedKv& kv = p.kv;
+    const int row = blockIdx.x, s = row / kv.H, h = row - s * kv.H, tid = threadIdx.x;
+    for (int o = tid; o < kv.S; o += kTabThreads) s_first[o] = p.src[o] == o ? -1 : kv.S;
+    if (tid == 0) s_page = -1;
+    __syncthreads();
+    for (int i = tid; i < kv.S; i += kTabThreads) {
+        const int o = p.src[i];
+        if (o >= 0 && o < kv.S && o != i) atomicMin(&s_first[o], i);
+    }
+    __syncthreads();
+    auto copies = [&](int i) {                   // slot i needs an unfinished page of its own in every head
+        const int o = p.src[i];
+        return o >= 0 && o < kv.S && o != i && s_first[o] != i && p.length[o] % kv.P != 0 ? 1 : 0;
+    };
+    int base = 0, total = 0;
+    for (int i = tid; i < kv.S; i += kTabThreads) { const int c = copies(i) * kv.H; total += c; if (i < s) base += c; }
+    block_sum2(base, total, s_a, s_b);
+    const int o = p.src[s];
+    if (o != s) {
+        const bool empty = o < 0 || o >= kv.S;
+        const int n = empty ? 0 : p.n_pages[(size_t)o * kv.H + h], length = empty ? 0 : p.length[o];
+        const bool copy = copies(s) != 0 && n > 0;
+        if (copy) {
+            const int rank = base + h;
+            for_free(kv, rank, rank + 1, s_a, [&](int, int page) { s_page = page; });
+            __syncthreads();
+        }
+        const int4* from = empty ? nullptr : p.entries + ((size_t)o * kv.H + h) * kv.M;
+        int4* to = kv.entries + (size_t)row * kv.M;
+        for (int i = tid; i < n - (copy ? 1 : 0); i += kTabThreads) to[i] = from[i];
+        int out = n;
+        if (copy) {
+            int4 e = from[n - 1];
+            const int old_page = e.x, page = s_page;
+            if (page < 0 || (unsigned)old_page >= (unsigned)kv.num_pages) {
+                out = n - 1;
+                if (tid == 0) paged_status(p.status, kErrNoPage);
+            } else {
+                e.x = page;
+                if (tid == 0) { to[n - 1] = e; kv.refs[page] = 1; }
+                const int vecs = length % kv.P * (kv.D / 8);
+                const size_t page_bytes = (size_t)kv.P * kv.D * 2;
+                for (int i = tid; i < vecs; i += kTabThreads) {
+                    const uint4 a = ld16(kv.k + old_page * page_bytes + i * 16), b = ld16(kv.v + old_page * page_bytes + i * 16);
+                    st16(kv.k + page * page_bytes + i * 16, a);
+                    st16(kv.v + page * page_bytes + i * 16, b);
+                }
+            }
+        }
+        if (tid == 0) {
+            kv.n_pages[row] = out;
+            if (h == 0) kv.length[s] = length;
+        }
+    }
+    if (last_block(p.ticket, kv.S * kv.H)) take_lowest(kv, total, s_a);
+}
+
+// ---- host side ------------------------------------------------------------------------------------
+int paged_kv(const NatsPagedKV* d, PagedKv& kv) {
+    NATS_CHECK_ARG(d != nullptr && d->d_pages_k && d->d_pages_v && d->d_refs && d->d_free_bits && d->d_entries && d->d_n_pages && d->d_length,
+                   "null pointer");
+    NATS_CHECK_ARG(((uintptr_t)d->d_pages_k | (uintptr_t)d->d_pages_v | (uintptr_t)d->d_entries) % 16 == 0, "pages and entries must be 16-byte aligned");
+    NATS_CHECK_ARG(d->num_pages > 0 && d->num_pages <= (1 << 24), "the number of pages must lie in [1, %d], got %d", 1 << 24, d->num_pages);
+    NATS_CHECK_ARG(d->page_size == 16 || d->page_size == 32 || d->page_size == 64 || d->page_size == 128, "page size %d: 16, 32, 64 or 128", d->page_size);
+    NATS_CHECK_ARG(d->slots > 0 && d->slots <= kMaxSlots && d->n_kv_heads > 0 && d->max_entries > 0 && (long long)d->slots * d->n_kv_heads <= 65535,
+                   "bad table [%d, %d, %d]: up to %d slots and 65535 rows", d->slots, d->n_kv_heads, d->max_entries, kMaxSlots);
+    if (d->head_dim != 64 && d->head_dim != 128) return fail(NATS_ERR_UNSUPPORTED, "the paged cache supports head_dim {64,128}, got %d", d->head_dim);
+    kv.k = (uint8_t*)d->d_pages_k; kv.v = (uint8_t*)d->d_pages_v; kv.refs = d->d_refs; kv.free_bits = d->d_free_bits;
+    kv.entries = (int4*)d->d_entries; kv.n_pages = d->d_n_pages; kv.length = d->d_length;
+    kv.num_pages = d->num_pages; kv.P = d->page_size; kv.D = d->head_dim; kv.S = d->slots; kv.H = d->n_kv_heads; kv.M = d->max_entries;
+    return NATS_OK;
+}
+
+static int append_chunks(int N, int P) { return (N + 2 * P - 2) / P; }
+
+}  // namespace nats
+
+using namespace nats;
+
+#define NATS_EXPORT extern "C" __attribute__((visibility("default")))
+
+NATS_EXPORT size_t nats_b200_paged_append_workspace_bytes(int slots, int n_kv_heads, int N, int page_size) {
+    if (slots <= 0 || n_kv_heads <= 0 || N <= 0 || page_size <= 0) return 0;
+    const size_t rows = (size_t)slots * n_kv_heads;
+    return 256 + align_up(rows * 4, 256) + 2 * align_up(rows * append_chunks(N, page_size) * 4, 256);
+}
+
+NATS_EXPORT int nats_b200_paged_append(const NatsPagedKV* kv, const void* d_k, const void* d_v, long long k_slot_stride, long long k_head_stride,
+                                       long long k_token_stride, long long v_slot_stride, long long v_head_stride, long long v_token_stride,
+                                       int f32, const uint8_t* d_roles, int n_roles, const int32_t* d_n_new, int N, int SW, int skip_hidden,
+                                       void* d_workspace, size_t workspace_bytes, int32_t* d_status, void* stream) {
+    AppendParams p;
+    if (const int e = paged_kv(kv, p.kv)) return e;
+    NATS_CHECK_ARG(d_k && d_v && d_workspace && d_status && (d_roles || n_roles == 0), "null pointer");
+    NATS_CHECK_ARG(N > 0 && N <= (1 << 24) && n_roles >= 0, "bad sizes N=%d n_roles=%d", N, n_roles);
+    NATS_CHECK_ARG(SW > 0 && SW % p.kv.P == 0, "sliding window %d must be a positive multiple of the page size %d", SW, p.kv.P);
+    NATS_CHECK_ARG(((uintptr_t)d_k | (uintptr_t)d_v) % 16 == 0, "K and V must be 16-byte aligned");
+    const int step = f32 ? 4 : 8;                // elements of 16 bytes
+    NATS_CHECK_ARG((k_slot_stride | k_head_stride | k_token_stride | v_slot_stride | v_head_stride | v_token_stride) % step == 0,
+                   "strides of K and V must keep 16-byte alignment");
+    const size_t need = nats_b200_paged_append_workspace_bytes(p.kv.S, p.kv.H, N, p.kv.P), rows = (size_t)p.kv.S * p.kv.H;
+    if (workspace_bytes < need) return fail(NATS_ERR_WORKSPACE, "paged append workspace: %zu bytes given, %zu needed", workspace_bytes, need);
+    p.k = (const uint8_t*)d_k; p.v = (const uint8_t*)d_v; p.f32 = f32;
+    p.k_slot = k_slot_stride; p.k_head = k_head_stride; p.k_token = k_token_stride;
+    p.v_slot = v_slot_stride; p.v_head = v_head_stride; p.v_token = v_token_stride;
+    p.roles = d_roles; p.n_roles = n_roles; p.n_new = d_n_new; p.N = N; p.SW = SW; p.n_chunks = append_chunks(N, p.kv.P);
+    p.copy_here = N <= kCopyTokens;
+    uint8_t* ws = (uint8_t*)d_workspace;
+    p.ticket = (int32_t*)ws;
+    p.counts = (int32_t*)(ws + 256);
+    p.ids = (int32_t*)(ws + 256 + align_up(rows * 4, 256));
+    p.map = p.ids + align_up(rows * p.n_chunks * 4, 256) / 4;
+    p.status = d_status;
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (skip_hidden) {
+        paged_count_kernel<<<(unsigned)rows, kTabThreads, 0, st>>>(p);
+        paged_append_kernel<true><<<(unsigned)rows, kTabThreads, 0, st>>>(p);
+    } else {
+        paged_append_kernel<false><<<(unsigned)rows, kTabThreads, 0, st>>>(p);
+    }
+    if (!p.copy_here) paged_copy_kernel<<<dim3(cdiv(N, kCopyTokens), (unsigned)rows), kTabThreads, 0, st>>>(p);
+    NATS_CHECK_CUDA(cudaGetLastError());
+    return NATS_OK;
+}
+
+NATS_EXPORT int nats_b200_paged_evict(const NatsPagedKV* d, void* stream) {
+    PagedKv kv;
+    if (const int e = paged_kv(d, kv)) return e;
+    paged_evict_kernel<<<kv.S * kv.H, kTabThreads, 0, (cudaStream_t)stream>>>(kv);
+    NATS_CHECK_CUDA(cudaGetLastError());
+    return NATS_OK;
+}
+
+NATS_EXPORT size_t nats_b200_paged_reorder_workspace_bytes(int slots, int n_kv_heads, int max_entries) {
+    if (slots <= 0 || n_kv_heads <= 0 || max_entries <= 0) return 0;
+    const size_t rows = (size_t)slots * n_kv_heads;
+    return 256 + align_up((size_t)slots * 4, 256) + align_up(rows * 4, 256) + rows * max_entries * 16;
+}
+
+NATS_EXPORT int nats_b200_paged_reorder(const NatsPagedKV* kv, const int32_t* d_src, void* d_workspace, size_t workspace_bytes, int32_t* d_status,
+                                        void* stream) {
+    ReorderParams p;
+    if (const int e = paged_kv(kv, p.kv)) return e;
+    NATS_CHECK_ARG(d_src && d_workspace && d_status, "null pointer");
+    NATS_CHECK_ARG((uintptr_t)d_workspace % 16 == 0, "the workspace must be 16-byte aligned");
+    const size_t need = nats_b200_paged_reorder_workspace_bytes(p.kv.S, p.kv.H, p.kv.M), rows = (size_t)p.kv.S * p.kv.H;
+    if (workspace_bytes < need) return fail(NATS_ERR_WORKSPACE, "paged reorder workspace: %zu bytes given, %zu needed", workspace_bytes, need);
+    uint8_t* ws = (uint8_t*)d_workspace;
+    p.src = d_src;
+    p.ticket = (int32_t*)ws;
+    p.length = (int32_t*)(ws + 256);
+    p.n_pages = (int32_t*)(ws + 256 + align_up((size_t)p.kv.S * 4, 256));
+    p.entries = (int4*)(ws + 256 + align_up((size_t)p.kv.S * 4, 256) + align_up(rows * 4, 256));
+    p.status = d_status;
+    const cudaStream_t st = (cudaStream_t)stream;
+    paged_release_kernel<<<(unsigned)rows, kTabThreads, 0, st>>>(p);
+    paged_move_kernel<<<(unsigned)rows, kTabThreads, p.kv.S * 4, st>>>(p);
+    NATS_CHECK_CUDA(cudaGetLastError());
+    return NATS_OK;
+}

@@ -14,6 +14,7 @@ with PyTorch ops: if the CUDA library is missing the import of ``_lib`` raises.
 """
 from __future__ import annotations
 
+import ctypes
 import math
 
 import torch
@@ -75,8 +76,14 @@ def status_word(device: torch.device) -> torch.Tensor:
     return _status[idx]
 
 
+PAGED_STATUS = {64: 'a paged cache has run out of pages', 65: 'a row of a paged cache has run out of entries',
+                66: 'paged_reorder was given a slot number out of range'}
+
+
 def _raise_status(device: torch.device, code: int) -> None:
     status_word(device).zero_()
+    if code in PAGED_STATUS:
+        raise _lib.NatsB200Error(f'{PAGED_STATUS[code]} (code {code}); its contents are invalid')
     raise _lib.NatsB200Error(f'the prefill kernel gave up a bounded wait (code {code}); its output is invalid')
 
 
@@ -633,3 +640,143 @@ def decode_place(roles: torch.Tensor, cache_k: torch.Tensor, cache_v: torch.Tens
     B, H, _, D = cache_k.shape
     _call(cache_k.device, 'nats_b200_decode_place', _p(roles), _p(cache_k), _p(cache_v), _p(valid), cache_k.shape[2], _p(size_global),
               _p(size_local), _p(state), tail, B, H, D, chunk_size, sliding_window, _stream(cache_k.device))
+
+
+# ------------------------------------------------------------------------------------------------
+# the paged cache
+# ------------------------------------------------------------------------------------------------
+PAGE_SIZES = (16, 32, 64, 128)
+PAGED_HEAD_DIMS = (64, 128)
+NO_LIMIT, OPEN_LOCAL = 2 ** 31 - 1, 2 ** 31 - 2       # limits of an entry: for good / a local chunk not closed yet
+
+
+class PagedKV:
+    """The tensors of a paged cache: K and V of every (slot, kv-head) in pages of one chunk each, out of one pool.
+
+    ``pages_k`` / ``pages_v`` bf16 [n,P,D]; ``refs`` int32 [n]: rows that hold a page; ``free_bits`` int32 [ceil(n/32)]: bit p % 32 of word
+    p // 32 is set where page p is free; ``entries`` int32 [S,Hkv,M,4]: (page, position of its first token, last query position that
+    may see it, 0), the first ``n_pages`` int32 [S,Hkv] of a row in use, in the order of positions; ``length`` int32 [S]: tokens so far.
+    All contiguous.  ``paged_append``, ``paged_attention``, ``paged_evict`` and ``paged_reorder`` work on it; nothing is copied."""
+
+    def __init__(self, pages_k: torch.Tensor, pages_v: torch.Tensor, refs: torch.Tensor, free_bits: torch.Tensor, entries: torch.Tensor,
+                 n_pages: torch.Tensor, length: torch.Tensor):
+        tensors = (pages_k, pages_v, refs, free_bits, entries, n_pages, length)
+        self.device = _need_cuda(*tensors)
+        n, P, D = pages_k.shape
+        S, H, M, four = entries.shape
+        if pages_k.dtype != torch.bfloat16 or pages_v.dtype != torch.bfloat16 or pages_v.shape != pages_k.shape:
+            raise ValueError('pages_k and pages_v must be bf16 [pages, page_size, head_dim]')
+        for t, shape, name in ((refs, (n,), 'refs'), (free_bits, (-(-n // 32),), 'free_bits'), (entries, (S, H, M, 4), 'entries'),
+                               (n_pages, (S, H), 'n_pages'), (length, (S,), 'length')):
+            if t.dtype != torch.int32 or t.shape != shape:
+                raise ValueError(f'{name} must be int32 {list(shape)}, got {t.dtype} {list(t.shape)}')
+        if not all(t.is_contiguous() for t in tensors):
+            raise ValueError('the tensors of a paged cache must be contiguous')
+        if P not in PAGE_SIZES:
+            raise ValueError(f'page size {P}: {PAGE_SIZES} are supported')
+        if D not in PAGED_HEAD_DIMS:
+            raise NotImplementedError(f'head_dim {D}: the paged cache is built for {PAGED_HEAD_DIMS}')
+        self.pages_k, self.pages_v, self.refs, self.free_bits, self.entries, self.n_pages, self.length = tensors
+        self.num_pages, self.page_size, self.head_dim, self.slots, self.n_kv_heads, self.max_entries = n, P, D, S, H, M
+        self._c = _lib.NatsPagedKV(*(t.data_ptr() for t in tensors), n, P, D, S, H, M)
+        self._ref = ctypes.byref(self._c)
+
+
+def _paged_workspace(kind: str, device: torch.device, nbytes: int) -> torch.Tensor:
+    """Zeroed scratch of the current stream.  While a graph is recorded it is the graph's own, so that two recorded graphs never share it."""
+    if torch.cuda.is_current_stream_capturing():
+        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
+    return _workspace(kind, device, nbytes, zero=True)
+
+
+def _strided_ok(t: torch.Tensor) -> bool:
+    """Rows dense, everything 16-byte aligned: what the kernels read without a copy."""
+    step = 16 // t.element_size()
+    a, b, c, d = t.stride()
+    return d == 1 and t.data_ptr() % 16 == 0 and a % step == 0 and b % step == 0 and c % step == 0
+
+
+def _check_n_new(kv: PagedKV, n_new: torch.Tensor | None) -> int | None:
+    if n_new is None:
+        return None
+    if n_new.dtype != torch.int32 or n_new.shape != (kv.slots,) or n_new.device != kv.device or not n_new.is_contiguous():
+        raise ValueError(f'n_new must be int32 [{kv.slots}] on {kv.device}')
+    return n_new.data_ptr()
+
+
+def paged_append(kv: PagedKV, k_new: torch.Tensor, v_new: torch.Tensor, roles: torch.Tensor | None, sliding_window: int,
+                 n_new: torch.Tensor | None = None, skip_hidden: bool = False) -> None:
+    """Writes new tokens into pages and moves ``length`` on.  k_new / v_new [S,Hkv,N,D] (bf16, or fp32 that is rounded on the way; any strides
+    that keep rows dense and 16-byte aligned), of which slot s has the first ``n_new[s]`` (int32 [S]; None: N).  ``roles`` uint8 [S,Hkv,R]
+    describes the chunks from a slot's unfinished one on; chunks behind them (None: all) and a chunk that stays unfinished count as
+    global.  A chunk that a call completes gets its limit from its role; a completed global one closes the local ones in front.
+    ``skip_hidden``: whole chunks that no query behind this call sees are not stored -- for a prompt whose attention does not
+    read the pages.  Running out of pages or of entries raises the device's status word (``check_status``)."""
+    dev = _need_cuda(kv.pages_k, k_new, v_new)
+    S, H, N, D = k_new.shape
+    if (S, H, D) != (kv.slots, kv.n_kv_heads, kv.head_dim) or v_new.shape != k_new.shape:
+        raise ValueError(f'k_new / v_new must be [{kv.slots},{kv.n_kv_heads},N,{kv.head_dim}], got {tuple(k_new.shape)} / {tuple(v_new.shape)}')
+    if roles is not None and (roles.dtype != torch.uint8 or roles.dim() != 3 or roles.shape[:2] != (S, H) or roles.device != dev):
+        raise ValueError(f'roles must be uint8 [{S},{H},chunks] on {dev}')
+    lens = _check_n_new(kv, n_new)
+    if N == 0:
+        return
+    if k_new.dtype != v_new.dtype or k_new.dtype not in (torch.bfloat16, torch.float32):
+        k_new, v_new = k_new.to(torch.bfloat16), v_new.to(torch.bfloat16)
+    if not _strided_ok(k_new):
+        k_new = k_new.contiguous()
+    if not _strided_ok(v_new):
+        v_new = v_new.contiguous()
+    if roles is not None and not roles.is_contiguous():
+        roles = roles.contiguous()
+    ws = _paged_workspace('paged_append', dev, _lib.lib().nats_b200_paged_append_workspace_bytes(S, H, N, kv.page_size))
+    _call(dev, 'nats_b200_paged_append', kv._ref, k_new.data_ptr(), v_new.data_ptr(), *k_new.stride()[:3], *v_new.stride()[:3],
+          int(k_new.dtype == torch.float32), _p(roles), 0 if roles is None else roles.shape[2], lens, N, sliding_window, int(skip_hidden),
+          ws.data_ptr(), ws.numel(), status_word(dev).data_ptr(), _stream(dev))
+
+
+def paged_attention(kv: PagedKV, q: torch.Tensor, sm_scale: float | None = None, n_new: torch.Tensor | None = None,
+                    max_pages: int | None = None, token_major: bool = False) -> torch.Tensor:
+    """Attention of the newest tokens of every slot over its pages, which hold their K and V already.  q [S,Hq,N,D] (cast to bf16 if needed;
+    any strides that keep rows dense and 16-byte aligned); row i of slot s is the token at position ``length[s] - n_new[s] + i``
+    (``n_new`` int32 [S]; None: N everywhere).  A key is seen from its own position on up to the limit of its page.  Rows behind a slot's
+    new tokens and rows that see nothing are zero.  ``max_pages``: a bound of ``n_pages`` the host knows (the work is split by it; the
+    result does not depend on its being right).  Returns o [S,Hq,N,D] in q's dtype; ``token_major``: a view of a [S,N,Hq,D] tensor."""
+    dev = _need_cuda(kv.pages_k, q)
+    S, Hq, N, D = q.shape
+    if S != kv.slots or D != kv.head_dim or Hq == 0 or Hq % kv.n_kv_heads:
+        raise ValueError(f'q must be [{kv.slots},multiple of {kv.n_kv_heads},N,{kv.head_dim}], got {tuple(q.shape)}')
+    lens = _check_n_new(kv, n_new)
+    scale = D ** -0.5 if sm_scale is None else float(sm_scale)
+    if not scale > 0.0:
+        raise ValueError('sm_scale must be positive')
+    dtype = torch.float32 if q.dtype == torch.float32 else torch.bfloat16      # fp32 callers: the kernel writes fp32 itself
+    o = torch.empty((S, N, Hq, D) if token_major else (S, Hq, N, D), dtype=dtype, device=dev)
+    if token_major:
+        o = o.transpose(1, 2)
+    if N > 0:
+        qb = q if q.dtype == torch.bfloat16 else q.to(torch.bfloat16)
+        if not _strided_ok(qb):
+            qb = qb.contiguous()
+        bound = kv.max_entries if max_pages is None else max(0, min(int(max_pages), kv.max_entries))
+        ws = _paged_workspace('paged_attention', dev, _lib.lib().nats_b200_paged_attention_workspace_bytes(S, Hq, kv.n_kv_heads, N, D, kv.page_size, bound))
+        _call(dev, 'nats_b200_paged_attention', kv._ref, qb.data_ptr(), *qb.stride()[:3], o.data_ptr(), *o.stride()[:3],
+              int(dtype == torch.float32), lens, Hq, N, bound, scale, ws.data_ptr(), ws.numel(), status_word(dev).data_ptr(), _stream(dev))
+    return o if o.dtype == q.dtype else o.to(q.dtype)
+
+
+def paged_evict(kv: PagedKV) -> None:
+    """Pages that the next query position (``length``) cannot see leave the rows; those that lose their last holder are free again."""
+    _call(kv.device, 'nats_b200_paged_evict', kv._ref, _stream(kv.device))
+
+
+def paged_reorder(kv: PagedKV, src: torch.Tensor) -> None:
+    """Every slot s becomes a copy of what slot ``src[s]`` (int32 [S], on the device) was, -1: an empty one -- replies forked off a prompt, the
+    survivors of a beam step, sequences dropped.  Whole pages are shared; the unfinished page stays with its own slot if that keeps its
+    sequence, else with the first one that takes it, and is copied for the others.  A number out of range raises the device's status
+    word (``check_status``) and leaves the slot empty."""
+    if src.dtype != torch.int32 or src.shape != (kv.slots,) or src.device != kv.device or not src.is_contiguous():
+        raise ValueError(f'src must be int32 [{kv.slots}] on {kv.device}')
+    dev = kv.device
+    ws = _paged_workspace('paged_reorder', dev, _lib.lib().nats_b200_paged_reorder_workspace_bytes(kv.slots, kv.n_kv_heads, kv.max_entries))
+    _call(dev, 'nats_b200_paged_reorder', kv._ref, src.data_ptr(), ws.data_ptr(), ws.numel(), status_word(dev).data_ptr(), _stream(dev))
