@@ -1,0 +1,429 @@
+"""The operators of the paged cache against a plain model of it in 64 bits.
+
+Pages hold NaN until a token is written to them, so that a row that nobody may see shows wherever it is read.
+Tolerance of attention, from its roundings: weights are rounded to bf16 (2^-8 of each, so 2^-8 softmax . |v|), a bf16 output once more (2^-8 |o|);
+scores are 128-term sums in fp32, off by at most 128 2^-24 sum |q k| scale < 1e-4 for unit normal inputs, and their exponentials by as much."""
+import numpy as np
+import pytest
+import torch
+
+from tests.paged_model import GLOBAL, LOCAL, SLIDING, PagedModel
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda'
+
+
+def bf16(x):
+    return x.to(torch.bfloat16)
+
+
+class Pair:
+    """The kernels and the model on the same inputs"""
+
+    def __init__(self, S, Hkv, G, P, D, SW, num_pages, M, seed=0):
+        from neuralattentionsearch_b200 import functional as F
+        self.F, self.G = F, G
+        self.gen = torch.Generator(device=DEV).manual_seed(seed)
+        self.rng = np.random.default_rng(seed)
+        nan = float('nan')
+        free = np.zeros(-(-num_pages // 32) * 32, dtype=np.int64)
+        free[:num_pages] = 1
+        bits = (free.reshape(-1, 32) << np.arange(32)).sum(1).astype(np.uint32).view(np.int32)
+        i32 = dict(dtype=torch.int32, device=DEV)
+        self.kv = F.PagedKV(torch.full((num_pages, P, D), nan, dtype=torch.bfloat16, device=DEV),
+                            torch.full((num_pages, P, D), nan, dtype=torch.bfloat16, device=DEV), torch.zeros(num_pages, **i32),
+                            torch.from_numpy(bits.copy()).to(DEV), torch.full((S, Hkv, M, 4), -7, **i32), torch.zeros(S, Hkv, **i32),
+                            torch.zeros(S, **i32))
+        self.model = PagedModel(S, Hkv, P, D, num_pages, SW)
+        self.S, self.H, self.P, self.D, self.SW = S, Hkv, P, D, SW
+
+    def randn(self, *shape, dtype=torch.bfloat16):
+        return torch.randn(*shape, generator=self.gen, device=DEV, dtype=torch.float32).to(dtype)
+
+    def roles(self, n, mix=(0.3, 0.3, 0.4)):
+        return self.rng.choice([GLOBAL, LOCAL, SLIDING], size=(self.S, self.H, n), p=mix).astype(np.uint8)
+
+    def append(self, N, n_new=None, roles='draw', dtype=torch.bfloat16, skip_hidden=False, token_major=False, mix=(0.3, 0.3, 0.4)):
+        shape = (self.S, N, self.H, self.D) if token_major else (self.S, self.H, N, self.D)
+        k, v = self.randn(*shape, dtype=dtype), self.randn(*shape, dtype=dtype)
+        if token_major:
+            k, v = k.transpose(1, 2), v.transpose(1, 2)
+        if isinstance(roles, str):
+            roles = self.roles((N + 2 * self.P - 2) // self.P, mix)
+        dev_roles = None if roles is None else torch.from_numpy(roles).to(DEV)
+        dev_n = None if n_new is None else torch.tensor(n_new, dtype=torch.int32, device=DEV)
+        self.F.paged_append(self.kv, k, v, dev_roles, self.SW, n_new=dev_n, skip_hidden=skip_hidden)
+        self.model.append(bf16(k).double().cpu().numpy(), bf16(v).double().cpu().numpy(), roles, n_new or [N] * self.S, skip_hidden)
+        self.compare()
+
+    def attend(self, N, n_new=None, dtype=torch.bfloat16, q=None, **more):
+        q = self.randn(self.S, self.H * self.G, N, self.D, dtype=dtype) if q is None else q
+        dev_n = None if n_new is None else torch.tensor(n_new, dtype=torch.int32, device=DEV)
+        o = self.F.paged_attention(self.kv, q, n_new=dev_n, **more)
+        self.F.check_status()
+        assert o.dtype == q.dtype and o.shape == q.shape
+        want, mag = self.model.attention(bf16(q).double().cpu().numpy(), n_new or [N] * self.S, more.get('sm_scale') or self.D ** -0.5)
+        got = o.double().cpu().numpy()
+        tol = (2.0 ** -8 + 2e-4) * mag + (2.0 ** -8 * np.abs(want) if dtype == torch.bfloat16 else 0)
+        assert np.isfinite(got).all()
+        worst = np.max(np.abs(got - want) - tol) if got.size else -1
+        assert worst <= 1e-30, worst
+        return o
+
+    def evict(self):
+        self.F.paged_evict(self.kv)
+        self.model.evict()
+        self.compare()
+
+    def reorder(self, src):
+        self.F.paged_reorder(self.kv, torch.tensor(src, dtype=torch.int32, device=DEV))
+        self.model.reorder(src)
+        self.compare()
+
+    def compare(self):
+        self.F.check_status()
+        kv, m = self.kv, self.model
+        assert kv.length.tolist() == m.length
+        assert kv.n_pages.tolist() == [[len(r) for r in rows] for rows in m.rows]
+        entries = kv.entries.cpu().numpy()
+        for s in range(self.S):
+            for h in range(self.H):
+                want = [[*e, 0] for e in m.rows[s][h]]
+                assert entries[s, h, :len(want)].tolist() == want, (s, h)
+        assert kv.refs.tolist() == m.refs
+        bits = kv.free_bits.cpu().numpy().view(np.uint32)
+        free = ((bits[:, None] >> np.arange(32, dtype=np.uint32)) & 1).reshape(-1)
+        assert free.tolist() == [int(r == 0) for r in m.refs] + [0] * (-len(m.refs) % 32)
+        used = [p for p, r in enumerate(m.refs) if r]
+        for dev, host in ((kv.pages_k, m.k), (kv.pages_v, m.v)):
+            got = dev[torch.tensor(used, dtype=torch.long, device=DEV)].double().cpu().numpy()
+            there = ~np.isnan(host[used])
+            assert np.array_equal(got[there], host[used][there])
+
+
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('P', [16, 32, 64, 128])
+def test_prompt_then_tokens(D, P):
+    t = Pair(S=2, Hkv=2, G=4, P=P, D=D, SW=2 * P, num_pages=200, M=40)
+    t.append(5 * P + 3)
+    t.attend(5 * P + 3)
+    t.evict()
+    for _ in range(P + 2):
+        t.append(1)
+    t.attend(1)
+    t.evict()
+    t.attend(1)
+
+
+@pytest.mark.parametrize('G', [1, 2, 3, 4, 5, 8, 16, 20])
+@pytest.mark.parametrize('N', [1, 2, 7, 33, 129])
+def test_group_sizes_and_lengths(G, N):
+    t = Pair(S=2, Hkv=2, G=G, P=16, D=64, SW=64, num_pages=400, M=80, seed=G * 1000 + N)
+    t.append(150)
+    t.evict()
+    t.append(N)
+    t.attend(N)
+    t.attend(N, token_major=True)
+
+
+@pytest.mark.parametrize('mix', [(1, 0, 0), (0, 1, 0), (0, 0, 1), (0.05, 0.15, 0.8)])
+def test_roles_of_one_kind(mix):
+    t = Pair(S=1, Hkv=2, G=2, P=32, D=128, SW=64, num_pages=120, M=50)
+    for n in (100, 1, 300, 27, 64, 200):
+        t.append(n, mix=mix)
+        t.attend(n)
+        t.evict()
+
+
+def test_ragged_batches_with_empty_slots():
+    t = Pair(S=5, Hkv=2, G=4, P=32, D=64, SW=96, num_pages=300, M=40, seed=3)
+    for n_new in ([70, 0, 1, 33, 200], [0, 0, 0, 0, 0], [1, 0, 31, 64, 9], [1, 1, 1, 1, 1], [200, 5, 0, 0, 17]):
+        N = max(max(n_new), 1)
+        t.append(N, n_new=n_new)
+        t.attend(N, n_new=n_new)
+        t.evict()
+
+
+def test_padded_rows_are_zero_and_lengths_out_of_range_are_clamped():
+    t = Pair(S=2, Hkv=1, G=4, P=16, D=64, SW=32, num_pages=60, M=20)
+    t.append(40, n_new=[40, 3])
+    o = t.attend(200, n_new=[40, 3])
+    assert not o[0, :, 40:].any() and not o[1, :, 3:].any()
+    q = t.randn(2, 4, 3, 64)
+    a = t.F.paged_attention(t.kv, q, n_new=torch.tensor([99, -5], dtype=torch.int32, device=DEV))
+    b = t.F.paged_attention(t.kv, q, n_new=torch.tensor([3, 0], dtype=torch.int32, device=DEV))
+    assert torch.equal(a, b) and not a[1].any()
+
+
+def test_an_empty_cache_gives_zeros():
+    t = Pair(S=2, Hkv=2, G=2, P=64, D=128, SW=64, num_pages=10, M=4)
+    for n in (1, 50):
+        q = t.randn(2, 4, n, 128)
+        assert not t.F.paged_attention(t.kv, q).any()
+    t.evict()
+    t.reorder([1, 0])
+    t.append(0)
+    assert t.F.paged_attention(t.kv, t.randn(2, 4, 0, 128)).shape == (2, 4, 0, 128)
+
+
+def test_rows_whose_pages_are_all_hidden():
+    t = Pair(S=1, Hkv=1, G=2, P=16, D=64, SW=16, num_pages=30, M=20)
+    t.append(48, roles=np.full((1, 1, 3), SLIDING, np.uint8))
+    # limits 31, 47, 63: the next query (position 48) sees the last chunk only; with that one hidden too, nothing
+    t.kv.entries[0, 0, :3, 2] = torch.tensor([31, 40, 40], dtype=torch.int32, device=DEV)
+    for e, lim in zip(t.model.rows[0][0], (31, 40, 40)):
+        e[2] = lim
+    o = t.attend(10)                                # positions 38 .. 47: 41 .. 47 see nothing
+    assert o[:, :, :3].abs().amax() > 0 and not o[:, :, 3:].any()
+
+
+@pytest.mark.parametrize('skip', [False, True])
+def test_a_prompt_without_its_hidden_chunks(skip):
+    a = Pair(S=3, Hkv=2, G=2, P=16, D=64, SW=48, num_pages=700, M=100, seed=5)
+    n_new = [16 * 30, 16 * 60 + 5, 7]
+    a.append(1000, n_new=n_new, skip_hidden=skip, mix=(0.1, 0.3, 0.6))
+    a.evict()
+    a.append(1)
+    a.attend(1)
+    if skip:
+        assert max(a.kv.n_pages.flatten().tolist()) < 45
+
+
+def test_many_chunks_per_call():
+    t = Pair(S=1, Hkv=2, G=1, P=16, D=64, SW=64, num_pages=2000, M=900, seed=8)
+    roles = t.roles(700, (0.02, 0.5, 0.48))
+    roles[:, :, 260:600] = LOCAL                    # no global chunk for more than a block's width
+    t.append(16 * 690 + 3, roles=roles)
+    t.attend(3)
+    t.evict()
+    t.append(30, skip_hidden=True)
+    t.attend(30)
+
+
+def test_roles_that_are_not_given_count_as_global():
+    t = Pair(S=1, Hkv=2, G=2, P=16, D=64, SW=32, num_pages=40, M=20)
+    t.append(100, roles=t.roles(2))
+    t.append(60, roles=None)
+    t.attend(60)
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+def test_types_and_strides(dtype):
+    t = Pair(S=2, Hkv=3, G=2, P=32, D=64, SW=64, num_pages=100, M=30)
+    t.append(77, dtype=dtype, token_major=True)
+    q = t.randn(2, 77, 6, 64, dtype=dtype).transpose(1, 2)
+    t.attend(77, dtype=dtype, q=q)
+    t.attend(77, dtype=dtype, q=q, sm_scale=0.3)
+    wide = t.randn(2, 6, 77, 72, dtype=dtype)
+    t.attend(77, dtype=dtype, q=wide[..., 4:68])     # rows that are not 16-byte aligned
+    one = t.randn(1, 1, 77, 64, dtype=dtype).expand(2, 6, 77, 64)
+    t.attend(77, dtype=dtype, q=one)
+
+
+def test_fork_beams_and_drop():
+    t = Pair(S=6, Hkv=2, G=2, P=32, D=64, SW=64, num_pages=300, M=30, seed=2)
+    t.append(150, n_new=[150, 0, 0, 0, 0, 0])
+    t.evict()
+    t.reorder([0, 0, 0, 0, -1, 0])
+    for step in range(3):
+        t.append(9, n_new=[9, 9, 3, 9, 0, 1])
+        t.attend(9, n_new=[9, 9, 3, 9, 0, 1])
+        t.evict()
+        t.reorder([[1, 0, 3, 3, 5, 5], [2, 2, 2, -1, 0, 4], [5, 4, 3, 2, 1, 0]][step])
+    t.append(40)
+    t.attend(40)
+    t.reorder([-1] * 6)
+    assert sum(t.model.refs) == 0 and t.kv.refs.sum().item() == 0
+
+
+def test_reorder_refuses_slots_out_of_range():
+    from neuralattentionsearch_b200 import _lib
+    t = Pair(S=3, Hkv=1, G=1, P=16, D=64, SW=16, num_pages=20, M=8)
+    t.append(20)
+    t.F.paged_reorder(t.kv, torch.tensor([0, 3, -2], dtype=torch.int32, device=DEV))
+    with pytest.raises(_lib.NatsB200Error, match='slot number'):
+        t.F.check_status()
+    assert t.kv.length.tolist() == [20, 0, 0]
+
+
+def test_out_of_pages_and_out_of_entries():
+    from neuralattentionsearch_b200 import _lib
+    for pages, M, text in ((5, 10, 'out of pages'), (50, 3, 'out of entries')):
+        t = Pair(S=2, Hkv=2, G=1, P=16, D=64, SW=16, num_pages=pages, M=M)
+        t.F.paged_append(t.kv, t.randn(2, 2, 100, 64), t.randn(2, 2, 100, 64), None, 16)
+        with pytest.raises(_lib.NatsB200Error, match=text):
+            t.F.check_status()
+        assert torch.isfinite(t.F.paged_attention(t.kv, t.randn(2, 2, 4, 64))).all()
+        t.F.paged_append(t.kv, t.randn(2, 2, 1, 64), t.randn(2, 2, 1, 64), None, 16)
+        t.F.paged_reorder(t.kv, torch.tensor([1, 1], dtype=torch.int32, device=DEV))
+        torch.cuda.synchronize()
+        t.F.status_word(torch.device(DEV, 0)).zero_()
+
+
+def test_bad_page_numbers_are_pages_that_are_not_there():
+    t = Pair(S=1, Hkv=1, G=2, P=16, D=64, SW=64, num_pages=40, M=12)
+    t.append(160, roles=None)
+    keep = t.kv.entries.clone()
+    for n in (2, 100):
+        t.kv.entries.copy_(keep)
+        t.kv.entries[0, 0, 3, 0] = 1 << 20
+        t.kv.entries[0, 0, 5, 0] = -4
+        q = t.randn(1, 2, n, 64)
+        got = t.F.paged_attention(t.kv, q)
+        t.kv.entries.copy_(keep)
+        t.kv.entries[0, 0, [3, 5], 2] = -1          # hidden from everybody instead
+        assert torch.equal(got, t.F.paged_attention(t.kv, q))
+
+
+def test_any_bound_of_the_pages_gives_the_same():
+    t = Pair(S=2, Hkv=2, G=4, P=16, D=64, SW=64, num_pages=1200, M=260, seed=4)
+    t.append(4000, roles=None)
+    for n in (1, 40, 300):
+        for bound in (None, 250, 260, 1, 0, 100):
+            t.attend(n, n_new=None, max_pages=bound)
+
+
+def test_other_streams_and_a_recorded_step():
+    t = Pair(S=2, Hkv=2, G=4, P=16, D=128, SW=32, num_pages=300, M=40, seed=6)
+    t.append(90)
+    t.evict()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        t.append(5)
+        t.attend(5)
+        t.evict()
+    torch.cuda.current_stream().wait_stream(side)
+    # one token per slot, every step replayed from one of two graphs, the lengths on the device
+    k, v, q = t.randn(2, 2, 1, 128), t.randn(2, 2, 1, 128), t.randn(2, 8, 1, 128)
+    roles = torch.zeros(2, 2, 1, dtype=torch.uint8, device=DEV)
+    src = torch.arange(2, dtype=torch.int32, device=DEV)
+
+    def step():
+        t.F.paged_append(t.kv, k, v, roles, 32)
+        o = t.F.paged_attention(t.kv, q)
+        t.F.paged_evict(t.kv)
+        t.F.paged_reorder(t.kv, src)
+        return o
+    graphs = []
+    for _ in range(2):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            o = step()
+        graphs.append((g, o))
+    for i in range(40):
+        k.copy_(t.randn(2, 2, 1, 128)); v.copy_(t.randn(2, 2, 1, 128)); q.copy_(t.randn(2, 8, 1, 128))
+        r = t.roles(1)
+        roles.copy_(torch.from_numpy(r))
+        src.copy_(torch.tensor([1, 0] if i % 7 == 3 else [1, 1] if i == 20 else [0, 1]))
+        g, o = graphs[i % 2]
+        g.replay()
+        t.model.append(k.double().cpu().numpy(), v.double().cpu().numpy(), r, [1, 1])
+        want, mag = t.model.attention(q.double().cpu().numpy(), [1, 1], 128 ** -0.5)
+        assert (np.abs(o.double().cpu().numpy() - want) <= (2.0 ** -8 + 2e-4) * mag + 2.0 ** -8 * np.abs(want)).all()
+        t.model.evict()
+        t.model.reorder(src.tolist())
+        t.compare()
+
+
+def test_pages_behind_32_bits():
+    """Page numbers whose byte and element offsets need more than 32 bits"""
+    from neuralattentionsearch_b200 import functional as F
+    n, P, D = 140000, 128, 128
+    g = torch.Generator(device=DEV).manual_seed(0)
+    i32 = dict(dtype=torch.int32, device=DEV)
+    kv = F.PagedKV(torch.zeros(n, P, D, dtype=torch.bfloat16, device=DEV), torch.zeros(n, P, D, dtype=torch.bfloat16, device=DEV),
+                   torch.ones(n, **i32), torch.zeros(-(-n // 32), **i32), torch.zeros(1, 1, 8, 4, **i32), torch.zeros(1, 1, **i32), torch.zeros(1, **i32))
+    kv.refs[n - 7:] = 0
+    for p in range(n - 7, n):
+        kv.free_bits[p // 32] |= 1 << (p % 32) if p % 32 < 31 else -(1 << 31)
+    k, v = (torch.randn(1, 1, 700, D, generator=g, device=DEV).bfloat16() for _ in range(2))
+    F.paged_append(kv, k, v, None, 128)
+    assert kv.entries[0, 0, :6, 0].tolist() == list(range(n - 7, n - 1))
+    assert torch.equal(kv.pages_k[n - 7:n - 2].reshape(1, 1, -1, D), k[:, :, :640])
+    for N in (2, 300):
+        q = torch.randn(1, 4, N, D, generator=g, device=DEV).bfloat16()
+        x = (q.double() @ k.double().transpose(-1, -2)) * D ** -0.5
+        x.masked_fill_(torch.arange(700, device=DEV) > torch.arange(700 - N, 700, device=DEV)[:, None], -float('inf'))
+        w = x.softmax(-1)
+        want, mag = w @ v.double(), w @ v.double().abs()
+        assert ((F.paged_attention(kv, q).double() - want).abs() <= (2.0 ** -8 + 2e-4) * mag + 2.0 ** -8 * want.abs()).all()
+    F.paged_reorder(kv, torch.tensor([-1], **i32))
+    assert kv.refs[n - 7:].sum().item() == 0
+
+
+def test_long_rows_against_dense_attention():
+    """Sizes of real use: several row tiles, splits and ragged tables, against attention over gathered pages in 64 bits"""
+    from neuralattentionsearch_b200 import functional as F
+    for S, Hkv, G, D, P, M, N, seed in ((1, 2, 4, 128, 128, 90, 700, 0), (3, 2, 3, 64, 16, 500, 40, 1), (2, 4, 8, 128, 64, 70, 1, 2), (1, 1, 1, 64, 32, 300, 260, 3)):
+        g = torch.Generator(device=DEV).manual_seed(seed)
+        n_pool = S * Hkv * M
+        i32 = dict(dtype=torch.int32, device=DEV)
+        n_pages = torch.randint(M // 2, M + 1, (S, Hkv), generator=g, device=DEV).int()
+        length = n_pages.amax(1) * P - 5
+        entries = torch.zeros(S, Hkv, M, 4, **i32)
+        entries[..., 0] = torch.randperm(n_pool, generator=g, device=DEV).view(S, Hkv, M).int()
+        # the last pages of every row are the newest chunks; some pages end inside the queries
+        order = torch.arange(M, device=DEV).int()
+        entries[..., 1] = (order + (length[:, None, None] + P - 1) // P - n_pages[..., None]) * P
+        limit = length[:, None, None] - 1 - torch.randint(-N // 2, N, (S, Hkv, M), generator=g, device=DEV)
+        limit = torch.where(torch.rand(S, Hkv, M, generator=g, device=DEV) < 0.5, limit, 2 ** 31 - 1)
+        entries[..., 2] = torch.where(order >= n_pages[..., None] - 2, 2 ** 31 - 1, limit).int()
+        pages = [torch.randn(n_pool, P, D, generator=g, device=DEV).bfloat16() for _ in range(2)]
+        kv = F.PagedKV(*pages, torch.zeros(n_pool, **i32), torch.zeros(-(-n_pool // 32), **i32), entries, n_pages, length.int())
+        q = torch.randn(S, Hkv * G, N, D, generator=g, device=DEV).bfloat16()
+        o = F.paged_attention(kv, q).double()
+        F.check_status()
+        for s in range(S):
+            for h in range(Hkv):
+                row = entries[s, h, :n_pages[s, h]].long()
+                K, V = (x[row[:, 0]].reshape(-1, D).double() for x in pages)
+                pos = (row[:, 1:2] + torch.arange(P, device=DEV)).flatten()
+                qp = torch.arange(N, device=DEV) + length[s] - N
+                x = (q[s, h * G:(h + 1) * G].double() @ K.T) * D ** -0.5
+                x.masked_fill_(~((pos <= qp[:, None]) & (qp[:, None] <= row[:, 2].repeat_interleave(P))), -float('inf'))
+                w = x.softmax(-1)
+                want, mag = w @ V, w @ V.abs()
+                tol = (2.0 ** -8 + 2e-4) * mag + 2.0 ** -8 * want.abs()
+                assert ((o[s, h * G:(h + 1) * G] - want).abs() <= tol).all()
+
+
+def test_two_runs_give_the_same_bits():
+    outs = []
+    for _ in range(2):
+        t = Pair(S=3, Hkv=2, G=4, P=16, D=64, SW=64, num_pages=700, M=200, seed=9)
+        t.append(1500, roles=None)
+        outs.append([t.attend(n) for n in (1, 5, 300)])
+    for a, b in zip(*outs):
+        assert torch.equal(a, b)
+
+
+def test_refusals_of_the_python_entry_points():
+    t = Pair(S=2, Hkv=2, G=2, P=16, D=64, SW=32, num_pages=20, M=4)
+    F, kv = t.F, t.kv
+    parts = [kv.pages_k, kv.pages_v, kv.refs, kv.free_bits, kv.entries, kv.n_pages, kv.length]
+
+    def with_(i, x):
+        return parts[:i] + [x] + parts[i + 1:]
+    for bad in (with_(0, kv.pages_k.float()), with_(1, kv.pages_v[:5]), with_(2, kv.refs[:-1]), with_(3, kv.free_bits.long()), with_(5, kv.n_pages.T.contiguous().T),
+                with_(4, kv.entries[..., :3].contiguous() if False else kv.entries.float())):
+        with pytest.raises(ValueError):
+            F.PagedKV(*bad)
+    with pytest.raises(NotImplementedError):
+        F.PagedKV(*[torch.zeros(20, 16, 96, dtype=torch.bfloat16, device=DEV)] * 2, *parts[2:])
+    with pytest.raises(ValueError, match='page size'):
+        F.PagedKV(*[torch.zeros(20, 8, 64, dtype=torch.bfloat16, device=DEV)] * 2, *parts[2:])
+    k = t.randn(2, 2, 3, 64)
+    for call in (lambda: F.paged_append(kv, k[:1], k[:1], None, 32), lambda: F.paged_append(kv, k, k[:, :, :2], None, 32),
+                 lambda: F.paged_append(kv, k, k, torch.zeros(2, 2, 1, device=DEV), 32),
+                 lambda: F.paged_append(kv, k, k, None, 32, n_new=torch.zeros(2, device=DEV)),
+                 lambda: F.paged_attention(kv, t.randn(2, 3, 1, 64)), lambda: F.paged_attention(kv, t.randn(2, 4, 1, 128)),
+                 lambda: F.paged_attention(kv, k, sm_scale=0.0), lambda: F.paged_attention(kv, k, sm_scale=float('nan')),
+                 lambda: F.paged_reorder(kv, torch.zeros(2, dtype=torch.long, device=DEV)), lambda: F.paged_reorder(kv, torch.zeros(3, dtype=torch.int32, device=DEV))):
+        with pytest.raises(ValueError):
+            call()
+    from neuralattentionsearch_b200 import _lib
+    for call in (lambda: F.paged_append(kv, k, k, None, 24), lambda: F.paged_append(kv, k.cpu(), k, None, 32), lambda: F.paged_attention(kv, k.cpu())):
+        with pytest.raises(_lib.NatsB200Error):
+            call()
+    t.compare()
