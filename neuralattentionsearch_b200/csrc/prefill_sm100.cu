@@ -26,9 +26,7 @@
 //
 // TMEM (512 columns): see PrefillTmem.  Every mbarrier wait is bounded: on a time-out the CTA raises the caller's status
 // word, drains and exits.
-#include <cuda.h>
-
-#include "common.cuh"
+#include "sm100.cuh"
 
 namespace nats {
 
@@ -42,23 +40,11 @@ constexpr int kPrefillThreads = 384;
 // setmaxnreg split: 128 * low + 256 * high must not exceed the 384 * 168 registers of the launch
 constexpr int kRegsLow = NATS_REGS_LOW, kRegsHigh = NATS_REGS_HIGH;
 static_assert(128 * kRegsLow + 256 * kRegsHigh <= 384 * 168, "setmaxnreg budget");
-constexpr uint32_t kBoxBytes = 128 * 64 * 2;            // one TMA box: 128 rows x 64 bf16, 128-byte swizzled
-#ifndef NATS_RELAX_NS
-#define NATS_RELAX_NS 200
-#endif
-constexpr int kRelaxNs = NATS_RELAX_NS;
 #ifndef NATS_RELAX_PROD_NS
 #define NATS_RELAX_PROD_NS 0
 #endif
 constexpr int kRelaxProdNs = NATS_RELAX_PROD_NS;
 constexpr float kRescaleThreshold = 8.0f;               // log2 units: O is rescaled only when the row max grows by more
-#ifndef NATS_WAIT_LIMIT_NS
-#define NATS_WAIT_LIMIT_NS (400ull * 1000ull * 1000ull)
-#endif
-constexpr unsigned long long kWaitLimitNs = NATS_WAIT_LIMIT_NS;
-
-enum : int { kErrQ = 1, kErrKvFull, kErrKvEmpty, kErrSFull, kErrPFull, kErrOFull, kErrList, kErrOEmpty, kErrSmemAlign, kErrPipeLock, kErrSEmpty };
-
 struct PrefillParams {
     void* o;                          // [B,Hq,N,D], or with the heads inside the tokens [B,N,Hq,D]: strides in elements
     long long o_batch, o_head, o_row;
@@ -84,216 +70,6 @@ struct PrefillParams {
 
     float scale_log2;
 };
-
-// ---- PTX wrappers -------------------------------------------------------------------------------
-__device__ __forceinline__ uint32_t smem_u32(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
-
-__device__ __forceinline__ void mbar_init(uint32_t bar, uint32_t count) {
-    asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(bar), "r"(count) : "memory");
-}
-__device__ __forceinline__ void mbar_expect_tx(uint32_t bar, uint32_t bytes) {
-    asm volatile("mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;" ::"r"(bar), "r"(bytes) : "memory");
-}
-__device__ __forceinline__ void mbar_arrive(uint32_t bar) {
-    asm volatile("mbarrier.arrive.shared::cta.b64 _, [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ bool mbar_try_wait(uint32_t bar, uint32_t parity) {
-    uint32_t ok;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t"
-        "mbarrier.try_wait.parity.shared::cta.b64 p, [%1], %2;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t}"
-        : "=r"(ok) : "r"(bar), "r"(parity) : "memory");
-    return ok != 0;
-}
-__device__ __forceinline__ unsigned long long global_ns() {
-    unsigned long long t;
-    asm volatile("mov.u64 %0, %globaltimer;" : "=l"(t));
-    return t;
-}
-__device__ __forceinline__ uint32_t sm_cycles() {         // wraps every 2.2 s at 1965 MHz
-    uint32_t t;
-    asm volatile("mov.u32 %0, %clock;" : "=r"(t));
-    return t;
-}
-// Bounded wait.  Returns false when the wait was given up (by this thread or, earlier, by another one of the CTA).
-// With abort_flag == nullptr only the time limit ends the wait (used to drain copies after the CTA has given up).
-// RELAX > 0: sleep that many nanoseconds between polls (roles that run ahead of the critical path and should not take
-// issue slots from the softmax warps of their scheduler).  Every lane of a waiting warp polls: letting one lane poll and
-// broadcast the result was measured 25 % slower for the whole kernel.
-template <int RELAX = 0>
-__device__ __forceinline__ bool mbar_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status, int code) {
-    if (mbar_try_wait(bar, parity)) return true;
-    const unsigned long long t0 = global_ns();
-#pragma unroll 1
-    for (uint32_t it = 0;; ++it) {
-        if (RELAX > 0) __nanosleep(RELAX);
-        if (mbar_try_wait(bar, parity)) return true;
-        if ((it & 63u) == 63u) {
-            if (abort_flag != nullptr && *abort_flag) return false;
-            if (global_ns() - t0 > kWaitLimitNs) {
-                if (abort_flag != nullptr) *abort_flag = 1;
-                atomicCAS(status, 0, code);
-                return false;
-            }
-        }
-    }
-}
-
-// L2 eviction priority of a TMA load: K / V tiles are read again by the CTAs that work on neighbouring query tiles and
-// should stay, Q tiles are read once
-__device__ __forceinline__ uint64_t l2_policy_evict_last() {
-    uint64_t pol;
-    asm volatile("createpolicy.fractional.L2::evict_last.b64 %0, 1.0;" : "=l"(pol));
-    return pol;
-}
-__device__ __forceinline__ uint64_t l2_policy_evict_first() {
-    uint64_t pol;
-    asm volatile("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(pol));
-    return pol;
-}
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, uint32_t bar, int c0, int c1, int c2, uint64_t policy) {
-    asm volatile(
-        "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%3, %4, %5}], [%2], %6;"
-        ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "l"(policy) : "memory");
-}
-__device__ __forceinline__ void prefetch_tmap(const CUtensorMap* map) {
-    asm volatile("prefetch.tensormap [%0];" ::"l"(reinterpret_cast<uint64_t>(map)) : "memory");
-}
-
-__device__ __forceinline__ void tmem_alloc(uint32_t smem_dst, uint32_t ncols) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_dst), "r"(ncols) : "memory");
-}
-__device__ __forceinline__ void tmem_relinquish() {
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
-}
-__device__ __forceinline__ void tmem_dealloc(uint32_t taddr, uint32_t ncols) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(taddr), "r"(ncols) : "memory");
-}
-__device__ __forceinline__ void tc_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-__device__ __forceinline__ void tc_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(bar) : "memory");
-}
-__device__ __forceinline__ void tc_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
-__device__ __forceinline__ void tc_wait_st() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
-
-// D[tmem] (+)= A[tmem] * B[smem desc]
-__device__ __forceinline__ void mma_ts(uint32_t d_tmem, uint32_t a_tmem, uint64_t b_desc, uint32_t idesc, uint32_t accumulate) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\tsetp.ne.b32 p, %4, 0;\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_tmem), "l"(b_desc), "r"(idesc), "r"(accumulate) : "memory");
-}
-
-// D[tmem] (+)= A[smem desc] * B[smem desc], and the above, with the descriptors given as (low word, shared high word): within one kernel only
-// the start address and the leading byte offset (low word) differ between operands, so the issuing thread adds small constants to 32-bit
-// registers instead of carrying 64-bit descriptors around.  ACC is a compile-time flag so that no predicate has to be computed per MMA.
-template <int ACC>
-__device__ __forceinline__ void mma_ss_lo(uint32_t d_tmem, uint32_t a_lo, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 da, db;\n\tsetp.ne.b32 p, %5, 0;\n\t"
-        "mov.b64 da, {%1, %3};\n\tmov.b64 db, {%2, %3};\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], da, db, %4, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_lo), "r"(b_lo), "r"(desc_hi), "r"(idesc), "n"(ACC) : "memory");
-}
-template <int ACC>
-__device__ __forceinline__ void mma_ts_lo(uint32_t d_tmem, uint32_t a_tmem, uint32_t b_lo, uint32_t desc_hi, uint32_t idesc) {
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b64 db;\n\tsetp.ne.b32 p, %5, 0;\n\t"
-        "mov.b64 db, {%2, %3};\n\t"
-        "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], db, %4, p;\n\t}"
-        ::"r"(d_tmem), "r"(a_tmem), "r"(b_lo), "r"(desc_hi), "r"(idesc), "n"(ACC) : "memory");
-}
-
-// 32 lanes x 32 consecutive 32-bit columns: thread i of the warp gets its lane's columns
-__device__ __forceinline__ void tmem_ld32(uint32_t taddr, uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
-        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,"
-        "%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
-        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]),
-          "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]),
-          "=r"(r[16]), "=r"(r[17]), "=r"(r[18]), "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]),
-          "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]), "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
-        : "r"(taddr) : "memory");
-}
-__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t (&r)[32]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,"
-        "%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};"
-        ::"r"(taddr),
-          "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]),
-          "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]),
-          "r"(r[24]), "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
-        : "memory");
-}
-__device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16]) {
-    asm volatile(
-        "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
-        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};"
-        ::"r"(taddr),
-          "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
-          "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15])
-        : "memory");
-}
-
-// 32-byte store (one sector) to a 32-byte aligned global address
-__device__ __forceinline__ void st32(void* p, const uint32_t (&w)[8]) {
-    asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};"
-                 ::"l"(p), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
-}
-
-__device__ __forceinline__ float ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-__device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
-    uint32_t r;
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
-    return r;
-}
-
-// ---- descriptors ----------------------------------------------------------------------------------
-// Shared-memory matrix descriptor of a 128-byte swizzled tile whose rows are 128 bytes (what one TMA box leaves):
-// start address >> 4 in [0,14), leading byte offset >> 4 in [16,30), stride byte offset >> 4 in [32,46),
-// descriptor version 1 in [46,48), swizzle mode 2 (128 B) in [61,64).
-__device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
-    return (uint64_t)((addr & 0x3ffffu) >> 4) | ((uint64_t)(lbo_bytes >> 4) << 16) | ((uint64_t)(sbo_bytes >> 4) << 32) |
-           (1ull << 46) | (2ull << 61);
-}
-// Instruction descriptor, kind::f16: fp32 accumulate, bf16 A and B, A K-major, B K-major or MN-major, M = 128.
-__host__ __device__ constexpr uint32_t instr_desc(int n, bool b_mn_major) {
-    return (1u << 4) | (1u << 7) | (1u << 10) | ((b_mn_major ? 1u : 0u) << 16) | ((uint32_t)(n >> 3) << 17) | ((uint32_t)(128 >> 4) << 24);
-}
-
-// packed fp32 pairs: one instruction for two lanes of a multiply-add or add
-__device__ __forceinline__ uint64_t pack2(float lo, float hi) {
-    uint64_t r;
-    asm("mov.b64 %0, {%1, %2};" : "=l"(r) : "f"(lo), "f"(hi));
-    return r;
-}
-__device__ __forceinline__ void unpack2(uint64_t v, float& lo, float& hi) {
-    asm("mov.b64 {%0, %1}, %2;" : "=f"(lo), "=f"(hi) : "l"(v));
-}
-__device__ __forceinline__ uint64_t fma2(uint64_t a, uint64_t b, uint64_t c) {
-    uint64_t d;
-    asm("fma.rn.ftz.f32x2 %0, %1, %2, %3;" : "=l"(d) : "l"(a), "l"(b), "l"(c));
-    return d;
-}
-__device__ __forceinline__ uint64_t add2(uint64_t a, uint64_t b) {
-    uint64_t d;
-    asm("add.rn.ftz.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
-    return d;
-}
-__device__ __forceinline__ float max3(float a, float b, float c) {
-    float d;
-    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
-    return d;
-}
 
 // ---- shared memory --------------------------------------------------------------------------------
 struct ItemHeader {
@@ -369,51 +145,6 @@ struct TileWalk {
         return w * 32 + b;
     }
 };
-
-// A bounded wait whose outcome is the same for every lane of the warp (all 32 lanes call it): lanes may see a time-out
-// or the CTA's abort flag at different polls, and what follows (.sync.aligned instructions, __syncwarp) needs the
-// whole warp on one path.
-template <int RELAX = 0>
-__device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status, int code) {
-    const bool ok = mbar_wait<RELAX>(bar, parity, abort_flag, status, code);
-    return __all_sync(0xffffffffu, ok);
-}
-// The same for the softmax warps, whose code has to stay short: a loop around the look, the SM's cycle counter as the clock, and what
-// follows a time-out in a function of its own.  They wait about twice as long as the other warps (0.8 s at 1965 MHz): where a softmax
-// warp waits for an issuer that waits in turn, the status names the issuer's wait.  Behind the last item of a CTA nobody else is left to
-// give up: the epilogue's wait for the last P.V ends by this limit only.  A look in front of the loop saves the others reading the clock;
-// with FINE the shorter code is worth more: us per call, a limit on the number of looks (none in time) / this with / this without the look in
-// front, forward of 8 x 4096 tokens with chunks of 16 187.8 / 189.9 / 182.4, 32k tokens with chunks of 128 1053 / 1048 / 1061, 8 x 15001
-// 3211 / 3200 / 3240, 2 x 131k 19270 / 19260 / 19290.
-constexpr uint32_t kSoftmaxWaitCycles = (uint32_t)(4 * kWaitLimitNs);
-static_assert(4 * kWaitLimitNs < (1ull << 32), "the cycle counter is read with 32 bits");
-__device__ __noinline__ bool give_up(volatile int* abort_flag, int32_t* status, int code) {
-    if (*abort_flag == 0) {
-        *abort_flag = 1;
-        atomicCAS(status, 0, code);
-    }
-    return false;
-}
-template <bool FINE>
-__device__ __forceinline__ bool warp_wait_short(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status, int code) {
-    if (!FINE && __builtin_expect(__all_sync(0xffffffffu, mbar_try_wait(bar, parity)), 1)) return true;
-    const uint32_t t0 = sm_cycles();
-#pragma unroll 1
-    do {
-        if (__builtin_expect(__all_sync(0xffffffffu, mbar_try_wait(bar, parity)), 1)) return true;
-    } while (__all_sync(0xffffffffu, sm_cycles() - t0 < kSoftmaxWaitCycles && *abort_flag == 0));
-    return give_up(abort_flag, status, code);
-}
-
-// Waits of the producer, the issuers and the scheduler: a look and a branch in their code, the loop is a function of its own.
-__device__ __noinline__ bool util_wait_loop(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status, int code, bool relax) {
-    return __all_sync(0xffffffffu, relax ? mbar_wait<kRelaxNs>(bar, parity, abort_flag, status, code) : mbar_wait(bar, parity, abort_flag, status, code));
-}
-template <int RELAX = 0>
-__device__ __forceinline__ bool util_wait(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status, int code) {
-    if (__all_sync(0xffffffffu, mbar_try_wait(bar, parity))) return true;
-    return util_wait_loop(bar, parity, abort_flag, status, code, RELAX > 0);
-}
 
 // Persistent kernel: every CTA takes work items (query tile x kv-head x head pair) from a global counter until none is
 // left.  Per-item set-up (kept-tile bitmap, Q load) and tear-down (O -> global) overlap the main loops of the
@@ -1011,24 +742,6 @@ prefill_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant_
 namespace nats {
 
 // ---- host side ------------------------------------------------------------------------------------
-typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
-                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
-                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-
-static EncodeTiledFn get_encode_fn() {
-    static EncodeTiledFn fn = nullptr;
-    if (fn) return fn;
-    void* ptr = nullptr;
-    cudaDriverEntryPointQueryResult qres;
-    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &ptr, cudaEnableDefault, &qres) != cudaSuccess ||
-        qres != cudaDriverEntryPointSuccess) {
-        (void)cudaGetLastError();
-        return nullptr;
-    }
-    fn = (EncodeTiledFn)ptr;
-    return fn;
-}
-
 // [heads, N, D] bf16 viewed as a 3-D tensor (D innermost); box = 64 x box_rows x 1 with 128-byte swizzle; rows past N read zero
 // 3-D map over [heads, rows, D] bf16; consecutive heads are head_stride_rows rows apart (>= rows: a cache buffer is
 // longer than the part of it that is valid; rows behind `rows` read as zero).
