@@ -379,7 +379,8 @@ int nats_b200_paged_append(const NatsPagedKV* kv, const void* d_k, const void* d
  * split by it; where it is too low the result stays right).  A value that is not finite in a V row reaches the rows of the call that
  * share a 128-key tile with it from its own position on or not at all only where its page is hidden from all of them.
  */
-size_t nats_b200_paged_attention_workspace_bytes(int slots, int n_heads, int n_kv_heads, int N, int head_dim, int page_size, int max_pages);
+size_t nats_b200_paged_attention_workspace_bytes(int slots, int n_heads, int n_kv_heads, int N, int head_dim, int page_size, int max_pages,
+                                                  int max_entries);
 int nats_b200_paged_attention(const NatsPagedKV* kv, const void* d_q, long long q_slot_stride, long long q_head_stride, long long q_token_stride,
                               void* d_o, long long o_slot_stride, long long o_head_stride, long long o_token_stride, int o_f32,
                               const int32_t* d_n_new, int n_heads, int N, int max_pages, float sm_scale, void* d_workspace,

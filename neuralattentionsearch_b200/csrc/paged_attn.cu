@@ -9,7 +9,7 @@
 // paged_rows_kernel: sixteen query rows per block and a split of the row's pages; four warps take 16-key tiles of it in turn, each with a ring
 // of cp.async stages of its own.  S = Q.K^T and O += P.V are mma.sync m16n8k16, whose score fragments are the A fragments of P.V.  With few
 // rows the kernel is bound by HBM.  Splits leave (max, sum, O) in the workspace and the block that arrives last joins them, in a fixed order.
-#include "paged.cuh"
+#include "paged_attn.cuh"
 
 namespace nats {
 
@@ -19,24 +19,6 @@ constexpr int kRowStages = 3;
 constexpr int kRows = 16;                        // query rows per block
 constexpr int kMaxTickets = 4096;               // joins of a launch; the workspace begins with as many words, which are zero between calls
 constexpr int kBatchTiles = 64;                  // tiles whose entries a block holds at a time, 16 per warp
-
-struct PagedAttnParams {
-    PagedKv kv;
-    const __nv_bfloat16* q;
-    long long q_slot, q_head, q_token;           // strides in elements
-    void* o;
-    long long o_slot, o_head, o_token;
-    int o_f32;
-    const int32_t* n_new;                        // [S] or nullptr: N everywhere
-    int N, G;
-    int splits;                                  // of the pages of a row
-    int split_pages;                             // pages per split (rows kernel)
-    int row_tiles;                               // tiles of query rows per (slot, kv-head)
-    float scale_log2;
-    int32_t* tickets;
-    float* partials;
-    int32_t* status;
-};
 
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
@@ -292,18 +274,30 @@ __global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const PagedAttn
 }
 
 // ---- host side ------------------------------------------------------------------------------------
-struct AttnPlan { int row_tiles, split_pages, splits; size_t tickets, partials; };
-// max_pages: bound of the pages of a row
-static AttnPlan attn_plan(int S, int H, int G, int N, int D, int P, int max_pages) {
+struct AttnPlan { bool tiles; int row_tiles, split_pages, splits; size_t counter, partials, bytes; };
+// max_pages: bound of the pages of a row that the host knows; M: entries of a row
+static AttnPlan attn_plan(int S, int H, int G, int N, int D, int P, int max_pages, int M) {
     AttnPlan a;
-    a.row_tiles = cdiv(N * G, kRows);
-    const long long units = (long long)S * H * a.row_tiles;
-    const int pages_per_k = 1024 / P;
-    a.split_pages = units >= 4 * 148 ? max(pages_per_k, max_pages) : pages_per_k;
-    static_assert(4 * 148 <= kMaxTickets, "splits are joined");
-    a.splits = max(1, cdiv(max_pages, a.split_pages));
-    a.tickets = kMaxTickets * 4;
-    a.partials = a.splits == 1 ? 0 : (size_t)units * a.splits * kRows * (D + 2) * 4;
+    a.tiles = (long long)N * G > kRows && G <= kTile;
+    a.counter = kMaxTickets * 4;
+    a.partials = a.counter + 256;
+    if (a.tiles) {
+        a.row_tiles = cdiv(N, tile_tokens(G));
+        a.split_pages = 0;
+        // one item per SM as long as an item has four tiles of keys, and no more pages than an item can look at
+        const long long items = (long long)S * H * cdiv(a.row_tiles, 2);
+        const int wanted = (int)max(1ll, min(148 / items, (long long)max_pages * P / (4 * kTile)));
+        a.splits = max(wanted, cdiv(M, kTileMaxPages));
+        a.bytes = a.partials + paged_tile_partial_floats(S, H * G, N, D, a.splits) * 4;
+    } else {
+        a.row_tiles = cdiv(N * G, kRows);
+        const long long units = (long long)S * H * a.row_tiles;
+        const int pages_per_k = 1024 / P;
+        a.split_pages = units >= 4 * 148 ? max(pages_per_k, max_pages) : pages_per_k;
+        static_assert(4 * 148 <= kMaxTickets, "splits are joined");
+        a.splits = max(1, cdiv(max_pages, a.split_pages));
+        a.bytes = a.partials + (a.splits == 1 ? 0 : (size_t)units * a.splits * kRows * (D + 2) * 4);
+    }
     return a;
 }
 
@@ -328,10 +322,10 @@ using namespace nats;
 
 #define NATS_EXPORT extern "C" __attribute__((visibility("default")))
 
-NATS_EXPORT size_t nats_b200_paged_attention_workspace_bytes(int slots, int n_heads, int n_kv_heads, int N, int head_dim, int page_size, int max_pages) {
-    if (slots <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || N <= 0 || head_dim <= 0 || page_size <= 0 || max_pages < 0) return 0;
-    const AttnPlan a = attn_plan(slots, n_kv_heads, n_heads / n_kv_heads, N, head_dim, page_size, max_pages);
-    return a.tickets + a.partials;
+NATS_EXPORT size_t nats_b200_paged_attention_workspace_bytes(int slots, int n_heads, int n_kv_heads, int N, int head_dim, int page_size, int max_pages,
+                                                            int max_entries) {
+    if (slots <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || N <= 0 || head_dim <= 0 || page_size <= 0 || max_pages < 0 || max_entries <= 0) return 0;
+    return attn_plan(slots, n_kv_heads, n_heads / n_kv_heads, N, head_dim, page_size, max_pages, max_entries).bytes;
 }
 
 NATS_EXPORT int nats_b200_paged_attention(const NatsPagedKV* kv, const void* d_q, long long q_slot_stride, long long q_head_stride,
@@ -348,17 +342,18 @@ NATS_EXPORT int nats_b200_paged_attention(const NatsPagedKV* kv, const void* d_q
     NATS_CHECK_ARG((q_slot_stride | q_head_stride | q_token_stride | o_slot_stride | o_head_stride | o_token_stride) % 8 == 0,
                    "strides must keep 16-byte alignment");
     const int G = n_heads / p.kv.H;
-    const AttnPlan a = attn_plan(p.kv.S, p.kv.H, G, N, p.kv.D, p.kv.P, max_pages);
-    if (workspace_bytes < a.tickets + a.partials)
-        return fail(NATS_ERR_WORKSPACE, "paged attention workspace: %zu bytes given, %zu needed", workspace_bytes, a.tickets + a.partials);
-    NATS_CHECK_ARG(a.row_tiles <= 65535, "%d new tokens of %d heads per kv-head are too many", N, G);
+    const AttnPlan a = attn_plan(p.kv.S, p.kv.H, G, N, p.kv.D, p.kv.P, max_pages, p.kv.M);
+    if (workspace_bytes < a.bytes) return fail(NATS_ERR_WORKSPACE, "paged attention workspace: %zu bytes given, %zu needed", workspace_bytes, a.bytes);
+    NATS_CHECK_ARG(a.tiles || a.row_tiles <= 65535, "%d new tokens of %d heads per kv-head are too many", N, G);
     p.q = (const __nv_bfloat16*)d_q; p.q_slot = q_slot_stride; p.q_head = q_head_stride; p.q_token = q_token_stride;
     p.o = d_o; p.o_slot = o_slot_stride; p.o_head = o_head_stride; p.o_token = o_token_stride; p.o_f32 = o_f32;
     p.n_new = d_n_new; p.N = N; p.G = G; p.splits = a.splits; p.split_pages = a.split_pages; p.row_tiles = a.row_tiles;
     p.scale_log2 = sm_scale * 1.4426950408889634f;
     p.tickets = (int32_t*)d_workspace;
-    p.partials = (float*)((uint8_t*)d_workspace + a.tickets);
+    p.counter = (int32_t*)((uint8_t*)d_workspace + a.counter);
+    p.partials = (float*)((uint8_t*)d_workspace + a.partials);
     p.status = d_status;
+    if (a.tiles) return launch_paged_tiles(p, (cudaStream_t)stream);
     const dim3 grid(a.splits, a.row_tiles, p.kv.S * p.kv.H);
     return p.kv.D == 64 ? launch_rows<64>(p, grid, (cudaStream_t)stream) : launch_rows<128>(p, grid, (cudaStream_t)stream);
 }

@@ -245,7 +245,7 @@ __device__ __forceinline__ bool warp_wait(uint32_t bar, uint32_t parity, volatil
 // 3211 / 3200 / 3240, 2 x 131k 19270 / 19260 / 19290.
 constexpr uint32_t kSoftmaxWaitCycles = (uint32_t)(4 * kWaitLimitNs);
 static_assert(4 * kWaitLimitNs < (1ull << 32), "the cycle counter is read with 32 bits");
-__device__ __noinline__ bool give_up(volatile int* abort_flag, int32_t* status, int code) {
+static __device__ __noinline__ bool give_up(volatile int* abort_flag, int32_t* status, int code) {
     if (*abort_flag == 0) {
         *abort_flag = 1;
         atomicCAS(status, 0, code);
@@ -264,7 +264,7 @@ __device__ __forceinline__ bool warp_wait_short(uint32_t bar, uint32_t parity, v
 }
 
 // Waits of the producer, the issuers and the scheduler: a look and a branch in their code, the loop is a function of its own.
-__device__ __noinline__ bool util_wait_loop(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status, int code, bool relax) {
+static __device__ __noinline__ bool util_wait_loop(uint32_t bar, uint32_t parity, volatile int* abort_flag, int32_t* status, int code, bool relax) {
     return __all_sync(0xffffffffu, relax ? mbar_wait<kRelaxNs>(bar, parity, abort_flag, status, code) : mbar_wait(bar, parity, abort_flag, status, code));
 }
 template <int RELAX = 0>

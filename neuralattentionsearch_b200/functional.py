@@ -84,6 +84,8 @@ def _raise_status(device: torch.device, code: int) -> None:
     status_word(device).zero_()
     if code in PAGED_STATUS:
         raise _lib.NatsB200Error(f'{PAGED_STATUS[code]} (code {code}); its contents are invalid')
+    if code > 32:
+        raise _lib.NatsB200Error(f'the paged attention kernel gave up a bounded wait (code {code}); its output is invalid')
     raise _lib.NatsB200Error(f'the prefill kernel gave up a bounded wait (code {code}); its output is invalid')
 
 
@@ -756,10 +758,11 @@ def paged_attention(kv: PagedKV, q: torch.Tensor, sm_scale: float | None = None,
         o = o.transpose(1, 2)
     if N > 0:
         qb = q if q.dtype == torch.bfloat16 else q.to(torch.bfloat16)
-        if not _strided_ok(qb):
+        if not _strided_ok(qb) or 0 in qb.stride():
             qb = qb.contiguous()
         bound = kv.max_entries if max_pages is None else max(0, min(int(max_pages), kv.max_entries))
-        ws = _paged_workspace('paged_attention', dev, _lib.lib().nats_b200_paged_attention_workspace_bytes(S, Hq, kv.n_kv_heads, N, D, kv.page_size, bound))
+        ws = _paged_workspace('paged_attention', dev, _lib.lib().nats_b200_paged_attention_workspace_bytes(S, Hq, kv.n_kv_heads, N, D, kv.page_size, bound,
+                                                                                                           kv.max_entries))
         _call(dev, 'nats_b200_paged_attention', kv._ref, qb.data_ptr(), *qb.stride()[:3], o.data_ptr(), *o.stride()[:3],
               int(dtype == torch.float32), lens, Hq, N, bound, scale, ws.data_ptr(), ws.numel(), status_word(dev).data_ptr(), _stream(dev))
     return o if o.dtype == q.dtype else o.to(q.dtype)
