@@ -20,6 +20,8 @@ class NatsPagedKV(_c.Structure):
                [(n, _I) for n in ('num_pages', 'page_size', 'head_dim', 'slots', 'n_kv_heads', 'max_entries')]
 
 
+_KV = _c.POINTER(NatsPagedKV)
+
 # name -> (restype, argtypes); mirrors include/nats_b200.h
 SIGNATURES = {
     'nats_b200_last_error': (_c.c_char_p, []),
@@ -55,12 +57,12 @@ SIGNATURES = {
     'nats_b200_decode_step_place': (_I, [_P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     'nats_b200_decode_step': (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _SZ, _P]),
     'nats_b200_paged_append_workspace_bytes': (_SZ, [_I, _I, _I, _I]),
-    'nats_b200_paged_append': (_I, [_P, _P, _P, _LL, _LL, _LL, _LL, _LL, _LL, _I, _P, _I, _P, _I, _I, _I, _P, _SZ, _P, _P]),
+    'nats_b200_paged_append': (_I, [_KV, _P, _P, _LL, _LL, _LL, _LL, _LL, _LL, _I, _P, _I, _P, _I, _I, _I, _P, _SZ, _P, _P]),
     'nats_b200_paged_attention_workspace_bytes': (_SZ, [_I, _I, _I, _I, _I, _I, _I, _I]),
-    'nats_b200_paged_attention': (_I, [_P, _P, _LL, _LL, _LL, _P, _LL, _LL, _LL, _I, _P, _I, _I, _I, _F, _P, _SZ, _P, _P]),
-    'nats_b200_paged_evict': (_I, [_P, _P]),
+    'nats_b200_paged_attention': (_I, [_KV, _P, _LL, _LL, _LL, _P, _LL, _LL, _LL, _I, _P, _I, _I, _I, _F, _P, _SZ, _P, _P]),
+    'nats_b200_paged_evict': (_I, [_KV, _P]),
     'nats_b200_paged_reorder_workspace_bytes': (_SZ, [_I, _I, _I]),
-    'nats_b200_paged_reorder': (_I, [_P, _P, _P, _SZ, _P, _P]),
+    'nats_b200_paged_reorder': (_I, [_KV, _P, _P, _SZ, _P, _P]),
     'nats_b200_decode_place': (_I, [_P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
 }
 

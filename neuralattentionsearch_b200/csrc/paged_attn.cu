@@ -278,7 +278,13 @@ struct AttnPlan { bool tiles; int row_tiles, split_pages, splits; size_t counter
 // max_pages: bound of the pages of a row that the host knows; M: entries of a row
 static AttnPlan attn_plan(int S, int H, int G, int N, int D, int P, int max_pages, int M) {
     AttnPlan a;
-    a.tiles = (long long)N * G > kRows && G <= kTile;
+#ifndef NATS_ROWS_MAX
+#define NATS_ROWS_MAX kRows
+#endif
+#ifndef NATS_SPLIT
+#define NATS_SPLIT 1024
+#endif
+    a.tiles = (long long)N * G > NATS_ROWS_MAX && G <= kTile;
     a.counter = kMaxTickets * 4;
     a.partials = a.counter + 256;
     if (a.tiles) {
@@ -292,9 +298,9 @@ static AttnPlan attn_plan(int S, int H, int G, int N, int D, int P, int max_page
     } else {
         a.row_tiles = cdiv(N * G, kRows);
         const long long units = (long long)S * H * a.row_tiles;
-        const int pages_per_k = 1024 / P;
-        a.split_pages = units >= 4 * 148 ? max(pages_per_k, max_pages) : pages_per_k;
-        static_assert(4 * 148 <= kMaxTickets, "splits are joined");
+        const int pages_per_k = max(1, NATS_SPLIT / P);
+        a.split_pages = units >= 4096 ? max(pages_per_k, max_pages) : pages_per_k;
+        static_assert(4096 <= kMaxTickets, "splits are joined");
         a.splits = max(1, cdiv(max_pages, a.split_pages));
         a.bytes = a.partials + (a.splits == 1 ? 0 : (size_t)units * a.splits * kRows * (D + 2) * 4);
     }

@@ -44,32 +44,61 @@ __device__ __forceinline__ void block_sum2(int& a, int& b, int (&s_a)[kTabWarps]
     __syncthreads();
 }
 
-// Walks the free pages of rank [r0, r1), the lowest free page having rank 0: f(rank, page).  Returns min(r1, free pages) - r0 (or less than 0).
-template <class F>
-__device__ __forceinline__ int for_free(const PagedKv& kv, int r0, int r1, int (&s_part)[kTabWarps], F f) {
+// The free pages in the order of their numbers, kFreeWords words of the bitmap at a time, four per thread; the first batch is on its way from
+// the start of a kernel.
+constexpr int kFreeWords = 4 * kTabThreads;
+struct FreeBits { uint32_t w[4]; };
+__device__ __forceinline__ FreeBits load_free(const PagedKv& kv, int w0) {
     const int words = (kv.num_pages + 31) / 32;
-    int base = 0;
-    for (int w0 = 0; w0 < words && base < r1; w0 += 4 * kTabThreads) {
-        uint32_t word[4];
-        int n = 0;
+    FreeBits f;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int w = w0 + 4 * threadIdx.x + j;
-            word[j] = w < words ? kv.free_bits[w] : 0u;
-            if (w == words - 1 && (kv.num_pages & 31)) word[j] &= (1u << (kv.num_pages & 31)) - 1u;
-            n += __popc(word[j]);
-        }
+    for (int j = 0; j < 4; ++j) {
+        const int w = w0 + 4 * threadIdx.x + j;
+        f.w[j] = w < words ? kv.free_bits[w] : 0u;
+        if (w == words - 1 && (kv.num_pages & 31)) f.w[j] &= (1u << (kv.num_pages & 31)) - 1u;
+    }
+    return f;
+}
+__device__ __forceinline__ int count_free(const FreeBits& f) { return __popc(f.w[0]) + __popc(f.w[1]) + __popc(f.w[2]) + __popc(f.w[3]); }
+
+// position of the n-th set bit (n = 0: the lowest) of a word with more than n of them
+__device__ __forceinline__ int nth_bit(uint32_t word, int n) {
+    int at = 0;
+#pragma unroll
+    for (int width = 16; width > 0; width >>= 1) {
+        const int low = __popc(word & ((1u << width) - 1u));
+        if (n >= low) { n -= low; word >>= width; at += width; }
+    }
+    return at;
+}
+
+struct PickScratch { int part[kTabWarps]; int rank[kTabThreads]; uint32_t words[kFreeWords]; };
+// The page of the calling thread's rank among the free ones (the lowest has rank 0), -1 if there are not so many or the rank is below 0.
+// Every thread of the block calls it; a thread looks its rank up in the prefix sums of the threads' words.
+__device__ __forceinline__ int pick_free(const PagedKv& kv, const FreeBits& first, int rank, PickScratch& sc) {
+    const int words = (kv.num_pages + 31) / 32;
+    int base = 0, page = -1;
+    for (int w0 = 0; w0 < words; w0 += kFreeWords) {
+        if (!__syncthreads_or(rank >= base)) break;
+        const FreeBits f = w0 == 0 ? first : load_free(kv, w0);
         int total;
-        int rank = base + block_scan(n, total, s_part);
-        if (rank + n > r0 && rank < r1) {
+        sc.rank[threadIdx.x] = block_scan(count_free(f), total, sc.part);
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-                for (uint32_t m = word[j]; m != 0u; m &= m - 1u, ++rank)
-                    if (rank >= r0 && rank < r1) f(rank, (w0 + 4 * (int)threadIdx.x + j) * 32 + __ffs(m) - 1);
+        for (int j = 0; j < 4; ++j) sc.words[4 * threadIdx.x + j] = f.w[j];
+        __syncthreads();
+        if (rank >= base && rank < base + total) {
+            int n = rank - base, t = 0;
+#pragma unroll
+            for (int step = kTabThreads / 2; step > 0; step >>= 1)
+                if (sc.rank[t + step] <= n) t += step;
+            n -= sc.rank[t];
+            int j = 0;
+            for (int c; n >= (c = __popc(sc.words[4 * t + j])); ++j) n -= c;
+            page = (w0 + 4 * t + j) * 32 + nth_bit(sc.words[4 * t + j], n);
         }
         base += total;
     }
-    return min(base, r1) - r0;
+    return page;
 }
 
 // The block that ends last takes the lowest `total` free pages out of the free ones (all others have picked theirs).
@@ -86,7 +115,29 @@ __device__ __forceinline__ bool last_block(int32_t* ticket, int n_blocks) {
     return s_last != 0;
 }
 __device__ __forceinline__ void take_lowest(const PagedKv& kv, int total, int (&s_part)[kTabWarps]) {
-    if (total > 0) for_free(kv, 0, total, s_part, [&](int, int page) { atomicAnd(&kv.free_bits[page >> 5], ~(1u << (page & 31))); });
+    const int words = (kv.num_pages + 31) / 32;
+    for (int w0 = 0; w0 < words && total > 0; w0 += kFreeWords) {
+        const FreeBits f = load_free(kv, w0);
+        int n;
+        int left = total - block_scan(count_free(f), n, s_part);       // pages to take from this thread's words on
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            uint32_t m = f.w[j];
+            const int c = __popc(m);
+            if (c == 0 || left <= 0) continue;
+            if (left >= c) m = 0u;
+            else for (int i = 0; i < left; ++i) m &= m - 1u;
+            kv.free_bits[w0 + 4 * threadIdx.x + j] = m;
+            left -= c;
+        }
+        total -= n;
+    }
+}
+
+// A kernel that follows another one of this file in a stream is launched while that one ends, and looks at memory only behind this wait.
+__device__ __forceinline__ void wait_for_launch_before() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
 __device__ __forceinline__ void give_back(const PagedKv& kv, int page) {
@@ -108,7 +159,6 @@ struct AppendParams {
     int copy_here;                               // the blocks of the table kernel copy the tokens as well
     int32_t* ticket;
     int32_t* counts;                             // [S * H]           new pages of a row (only where hidden chunks are skipped)
-    int32_t* ids;                                // [S * H, n_chunks] pages that a row takes
     int32_t* map;                                // [S * H, n_chunks] page of every chunk of the call, -1: not stored
     int32_t* status;
 };
@@ -132,8 +182,8 @@ __device__ __forceinline__ int pages_taken(const AppendParams& p, int s) {
 // Goes over the chunks of a call, tile by tile from the last one: f(i, chunk is there, last query position that may see it).
 // Returns the first completed global chunk of the call (-1: none).  limit of a chunk c: none if it is global or unfinished,
 // c P + SW + P - 1 if sliding, the end of the next completed global chunk if local.
-template <class F>
-__device__ __forceinline__ int for_chunks(const AppendParams& p, const AppendRow& r, F f) {
+template <class F, class G>
+__device__ __forceinline__ int for_chunks(const AppendParams& p, const AppendRow& r, F f, G first_of_all) {
     __shared__ unsigned s_global[kTabWarps];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, P = p.kv.P, c0 = r.old / P;
     const uint8_t* roles = p.roles + ((size_t)r.s * p.kv.H + r.h) * p.n_roles;
@@ -145,6 +195,7 @@ __device__ __forceinline__ int for_chunks(const AppendParams& p, const AppendRow
         const bool done = there && (long long)(c + 1) * P <= (long long)r.old + r.n;
         const unsigned own = __ballot_sync(0xffffffffu, done && role == NATS_ROLE_GLOBAL);
         if (lane == 0) s_global[warp] = own;
+        if (t0 + kTabThreads >= r.chunks) first_of_all();
         __syncthreads();
         int next = -1, first = after;
         if (own >> lane) next = c + __ffs(own >> lane) - 1;
@@ -170,52 +221,64 @@ __device__ __forceinline__ int for_chunks(const AppendParams& p, const AppendRow
 // Pages that a row takes if chunks that no later query sees are not stored
 __global__ void __launch_bounds__(kTabThreads) paged_count_kernel(const AppendParams p) {
     __shared__ int s_a[kTabWarps], s_b[kTabWarps];
+    wait_for_launch_before();
     const AppendRow r = append_row(p, blockIdx.x);
     int n = 0, none = 0;
-    for_chunks(p, r, [&](int i, bool there, int limit) { n += there && !(i == 0 && r.fill > 0) && limit >= r.old + r.n; });
+    for_chunks(p, r, [&](int i, bool there, int limit) { n += there && !(i == 0 && r.fill > 0) && limit >= r.old + r.n; }, [] {});
     block_sum2(n, none, s_a, s_b);
     if (threadIdx.x == 0) p.counts[blockIdx.x] = n;
 }
 
-// Token rows [t0, t1) of a row into their pages.  Four vectors of K and of V are on their way before the first is stored.
 __device__ __forceinline__ uint4 load_row8(const uint8_t* base, long long at, int f32) {
     if (!f32) return ld16_stream(base + 2 * at);
     return round8(ld16_stream(base + 4 * at), ld16_stream(base + 4 * at + 16));
 }
-__device__ __forceinline__ void copy_tokens(const AppendParams& p, const AppendRow& r, int row, int t0, int t1) {
-    const int vecs = p.kv.D / 8, P = p.kv.P, c0 = r.old / P;
-    const int32_t* map = p.map + (size_t)row * p.n_chunks;
-    const long long kb = r.s * p.k_slot + r.h * p.k_head, vb = r.s * p.v_slot + r.h * p.v_head;
-    const int n = (t1 - t0) * vecs;
-    for (int i0 = threadIdx.x; i0 < n; i0 += 4 * kTabThreads) {
-        uint4 a[4], b[4];
-        size_t to[4];
-        bool ok[4];
+// Token rows [t0, t0 + 4 * kTabThreads / vectors per row) of a row into their pages: four vectors of K and of V per thread, all on their way
+// before the first is stored
+struct TokenVecs { uint4 k[4], v[4]; };
+__device__ __forceinline__ TokenVecs load_tokens(const AppendParams& p, int s, int h, int t0, int t1) {
+    const int vecs = p.kv.D / 8;
+    const long long kb = s * p.k_slot + h * p.k_head, vb = s * p.v_slot + h * p.v_head;
+    TokenVecs x;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int i = i0 + j * kTabThreads, t = t0 + i / vecs, c = i % vecs;
-            ok[j] = i < n;
-            if (!ok[j]) continue;
-            const int pos = r.old + t, page = map[pos / P - c0];
-            ok[j] = page >= 0;
-            to[j] = (((size_t)page * P + pos % P) * p.kv.D + c * 8) * 2;
-            if (!ok[j]) continue;
-            a[j] = load_row8(p.k, kb + t * p.k_token + c * 8, p.f32);
-            b[j] = load_row8(p.v, vb + t * p.v_token + c * 8, p.f32);
-        }
+    for (int j = 0; j < 4; ++j) {
+        const int i = threadIdx.x + j * kTabThreads, t = t0 + i / vecs, c = i % vecs;
+        if (t >= t1) break;
+        x.k[j] = load_row8(p.k, kb + t * p.k_token + c * 8, p.f32);
+        x.v[j] = load_row8(p.v, vb + t * p.v_token + c * 8, p.f32);
+    }
+    return x;
+}
+__device__ __forceinline__ void store_tokens(const AppendParams& p, const TokenVecs& x, int old, int t0, int t1, const int32_t* map) {
+    const int vecs = p.kv.D / 8, P = p.kv.P, c0 = old / P;
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
-            if (ok[j]) { st16(p.kv.k + to[j], a[j]); st16(p.kv.v + to[j], b[j]); }
+    for (int j = 0; j < 4; ++j) {
+        const int i = threadIdx.x + j * kTabThreads, t = t0 + i / vecs, c = i % vecs;
+        if (t >= t1) break;
+        const int pos = old + t, page = map[pos / P - c0];
+        if (page < 0) continue;
+        const size_t to = (((size_t)page * P + pos % P) * p.kv.D + c * 8) * 2;
+        st16(p.kv.k + to, x.k[j]);
+        st16(p.kv.v + to, x.v[j]);
     }
 }
 
 // One block per (slot, kv-head): takes pages, writes the entries of the call's chunks, closes the open local ones, copies few tokens.
+// What a step waits for is a chain of memory latencies, so whatever can be asked for at once is asked for first.
 template <bool SKIP>
-__global__ void __launch_bounds__(kTabThreads) paged_append_kernel(const AppendParams p) {
+__global__ void __launch_bounds__(kTabThreads, 4) paged_append_kernel(const AppendParams p) {
     __shared__ int s_a[kTabWarps], s_b[kTabWarps];
+    __shared__ int32_t s_map[kCopyTokens / 16 + 2];
+    __shared__ PickScratch s_pick;
     const PagedKv& kv = p.kv;
     const int row = blockIdx.x, tid = threadIdx.x, rows = kv.S * kv.H;
+    wait_for_launch_before();
     const AppendRow r = append_row(p, row);
+    const FreeBits bits = load_free(kv, 0);
+    const int n0 = min(max(kv.n_pages[row], 0), kv.M);
+    const int4* last = kv.entries + (size_t)row * kv.M + max(n0 - 1, 0);
+    TokenVecs vecs;
+    if (p.copy_here) vecs = load_tokens(p, r.s, r.h, 0, r.n);
     // ranks of this row's pages among all that the call takes
     int base = 0, total = 0;
     if (SKIP) {
@@ -223,26 +286,15 @@ __global__ void __launch_bounds__(kTabThreads) paged_append_kernel(const AppendP
     } else {
         for (int s = tid; s < kv.S; s += kTabThreads) { const int n = pages_taken(p, s) * kv.H; total += n; if (s < r.s) base += n; }
     }
+    const int4 unfinished = *last;
     block_sum2(base, total, s_a, s_b);
     const int take = SKIP ? p.counts[row] : pages_taken(p, r.s);
     if (!SKIP) base += r.h * take;
-    int32_t* ids = p.ids + (size_t)row * p.n_chunks;
-    int room = 0;
-    if (take > 0) {
-        const int found = for_free(kv, base, base + take, s_a, [&](int rank, int page) { ids[rank - base] = page; });
-        room = min(max(found, 0), take);
-        __syncthreads();
-    }
     int4* entries = kv.entries + (size_t)row * kv.M;
-    const int n0 = min(max(kv.n_pages[row], 0), kv.M);
-    if (tid == 0 && room < take) paged_status(p.status, kErrNoPage);
-    if (room > kv.M - n0) {
-        if (tid == 0) paged_status(p.status, kErrNoEntry);
-        room = kv.M - n0;
-    }
-    const bool tail = r.fill > 0 && n0 > 0 && entries[n0 - 1].y == r.old - r.fill;
-    int32_t* map = p.map + (size_t)row * p.n_chunks;
-    int behind = 0;                              // SKIP: stored chunks behind the tile
+    const int room = min(take, kv.M - n0);
+    const bool tail = r.fill > 0 && n0 > 0 && unfinished.y == r.old - r.fill;
+    int32_t* map = p.copy_here ? s_map : p.map + (size_t)row * p.n_chunks;
+    int behind = 0, placed = room;               // SKIP: stored chunks behind the tile
     const int closing = for_chunks(p, r, [&](int i, bool there, int limit) {
         const bool fresh = there && !(i == 0 && r.fill > 0);
         int k = i - (r.fill > 0);
@@ -254,36 +306,43 @@ __global__ void __launch_bounds__(kTabThreads) paged_append_kernel(const AppendP
             k = take - behind - in_tile + in_front;
             behind += in_tile;
         }
+        const int page_new = pick_free(kv, bits, stored && k < room ? base + k : -1, s_pick);
         int page = -1;
-        if (stored && k < room) {
-            page = ids[k];
+        if (stored && page_new >= 0) {
+            page = page_new;
             entries[n0 + k] = make_int4(page, (r.old / kv.P + i) * kv.P, limit, 0);
             kv.refs[page] = 1;
+        } else if (stored && k < room) {
+            paged_status(p.status, kErrNoPage);
+            atomicMin(&s_b[0], k);               // the pages end here
         } else if (there && !fresh && tail) {
-            page = entries[n0 - 1].x;
+            page = unfinished.x;
             entries[n0 - 1].z = limit;
             if ((unsigned)page >= (unsigned)kv.num_pages) page = -1;
         }
         if (there) map[i] = page;
-    });
+    }, [&] { if (tid == 0) s_b[0] = room; });
+    placed = r.chunks > 0 ? s_b[0] : 0;
     if (closing >= 0)
         for (int e = tid; e < n0; e += kTabThreads)
             if (entries[e].z == kOpenLocal) entries[e].z = (int)min((long long)(closing + 1) * kv.P - 1, (long long)kOpenLocal - 1);
-    if (tid == 0) kv.n_pages[row] = n0 + room;
-    if (p.copy_here) {
-        __syncthreads();
-        copy_tokens(p, r, row, 0, r.n);
+    if (tid == 0) {
+        if (room < take) paged_status(p.status, kErrNoEntry);
+        if (placed > 0) kv.n_pages[row] = n0 + placed;
     }
+    if (p.copy_here) store_tokens(p, vecs, r.old, 0, r.n, s_map);
     if (!last_block(p.ticket, rows)) return;
     take_lowest(kv, total, s_a);
     for (int s = tid; s < kv.S; s += kTabThreads) kv.length[s] += new_tokens(p, s);
 }
 
 __global__ void __launch_bounds__(kTabThreads) paged_copy_kernel(const AppendParams p) {
-    AppendRow r = append_row(p, blockIdx.y);
-    r.old -= r.n;                                // the table kernel has moved the lengths on
-    const int t0 = blockIdx.x * kCopyTokens;
-    if (t0 < r.n) copy_tokens(p, r, blockIdx.y, t0, min(t0 + kCopyTokens, r.n));
+    const int s = blockIdx.y / p.kv.H, h = blockIdx.y - s * p.kv.H, per_pass = 4 * kTabThreads / (p.kv.D / 8);
+    wait_for_launch_before();
+    const int n = new_tokens(p, s), t1 = min((int)(blockIdx.x + 1) * kCopyTokens, n);
+    const int old = p.kv.length[s] - n;          // the table kernel has moved the lengths on
+    for (int t0 = blockIdx.x * kCopyTokens; t0 < t1; t0 += per_pass)
+        store_tokens(p, load_tokens(p, s, h, t0, t1), old, t0, t1, p.map + (size_t)blockIdx.y * p.n_chunks);
 }
 
 // =================================================================================================
@@ -294,6 +353,7 @@ __global__ void __launch_bounds__(kTabThreads) paged_evict_kernel(const PagedKv 
     __shared__ int s_part[kTabWarps];
     const int row = blockIdx.x, s = row / kv.H;
     int4* entries = kv.entries + (size_t)row * kv.M;
+    wait_for_launch_before();
     const int next = kv.length[s], n = min(max(kv.n_pages[row], 0), kv.M);
     int out = 0;
     for (int t0 = 0; t0 < n; t0 += kTabThreads) {
@@ -329,6 +389,8 @@ __global__ void __launch_bounds__(kTabThreads) paged_release_kernel(const Reorde
     __shared__ int s_a[kTabWarps], s_b[kTabWarps];
     const PagedKv& kv = p.kv;
     const int row = blockIdx.x, s = row / kv.H, tid = threadIdx.x;
+    wait_for_launch_before();
+    const int n = min(max(kv.n_pages[row], 0), kv.M), length = kv.length[s];
     int uses = 0, bad = 0;
     for (int i = tid; i < kv.S; i += kTabThreads) {
         const int o = p.src[i];
@@ -337,7 +399,6 @@ __global__ void __launch_bounds__(kTabThreads) paged_release_kernel(const Reorde
     }
     block_sum2(uses, bad, s_a, s_b);
     if (bad && tid == 0) paged_status(p.status, kErrSlot);
-    const int n = min(max(kv.n_pages[row], 0), kv.M), length = kv.length[s];
     const bool moves = uses > (p.src[s] == s ? 1 : 0);
     if (tid == 0) {
         p.n_pages[row] = n;
@@ -358,11 +419,13 @@ __global__ void __launch_bounds__(kTabThreads) paged_release_kernel(const Reorde
 __global__ void __launch_bounds__(kTabThreads) paged_move_kernel(const ReorderParams p) {
     __shared__ int s_a[kTabWarps], s_b[kTabWarps];
     __shared__ int s_page;
+    __shared__ PickScratch s_pick;
     extern __shared__ int s_first[];             // [S]: the slot that an unfinished page stays with
     const PagedKv& kv = p.kv;
     const int row = blockIdx.x, s = row / kv.H, h = row - s * kv.H, tid = threadIdx.x;
+    wait_for_launch_before();
+    const FreeBits bits = load_free(kv, 0);
     for (int o = tid; o < kv.S; o += kTabThreads) s_first[o] = p.src[o] == o ? -1 : kv.S;
-    if (tid == 0) s_page = -1;
     __syncthreads();
     for (int i = tid; i < kv.S; i += kTabThreads) {
         const int o = p.src[i];
@@ -382,8 +445,8 @@ __global__ void __launch_bounds__(kTabThreads) paged_move_kernel(const ReorderPa
         const int n = empty ? 0 : p.n_pages[(size_t)o * kv.H + h], length = empty ? 0 : p.length[o];
         const bool copy = copies(s) != 0 && n > 0;
         if (copy) {
-            const int rank = base + h;
-            for_free(kv, rank, rank + 1, s_a, [&](int, int page) { s_page = page; });
+            const int page = pick_free(kv, bits, tid == 0 ? base + h : -1, s_pick);
+            if (tid == 0) s_page = page;
             __syncthreads();
         }
         const int4* from = empty ? nullptr : p.entries + ((size_t)o * kv.H + h) * kv.M;
@@ -401,10 +464,20 @@ __global__ void __launch_bounds__(kTabThreads) paged_move_kernel(const ReorderPa
                 if (tid == 0) { to[n - 1] = e; kv.refs[page] = 1; }
                 const int vecs = length % kv.P * (kv.D / 8);
                 const size_t page_bytes = (size_t)kv.P * kv.D * 2;
-                for (int i = tid; i < vecs; i += kTabThreads) {
-                    const uint4 a = ld16(kv.k + old_page * page_bytes + i * 16), b = ld16(kv.v + old_page * page_bytes + i * 16);
-                    st16(kv.k + page * page_bytes + i * 16, a);
-                    st16(kv.v + page * page_bytes + i * 16, b);
+                const uint8_t *ks = kv.k + old_page * page_bytes, *vs = kv.v + old_page * page_bytes;
+                uint8_t *kd = kv.k + page * page_bytes, *vd = kv.v + page * page_bytes;
+                for (int i0 = tid; i0 < vecs; i0 += 4 * kTabThreads) {
+                    uint4 a[4], b[4];
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int i = i0 + j * kTabThreads;
+                        if (i < vecs) { a[j] = ld16(ks + i * 16); b[j] = ld16(vs + i * 16); }
+                    }
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const int i = i0 + j * kTabThreads;
+                        if (i < vecs) { st16(kd + i * 16, a[j]); st16(vd + i * 16, b[j]); }
+                    }
                 }
             }
         }
@@ -432,6 +505,22 @@ int paged_kv(const NatsPagedKV* d, PagedKv& kv) {
     return NATS_OK;
 }
 
+// Launches a kernel that waits for the one in front of it by itself (wait_for_launch_before)
+template <class... K, class... A>
+static cudaError_t launch_behind(void (*kernel)(K...), dim3 grid, size_t smem, cudaStream_t st, const A&... args) {
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(kTabThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, args...);
+}
+
 static int append_chunks(int N, int P) { return (N + 2 * P - 2) / P; }
 
 }  // namespace nats
@@ -443,7 +532,7 @@ using namespace nats;
 NATS_EXPORT size_t nats_b200_paged_append_workspace_bytes(int slots, int n_kv_heads, int N, int page_size) {
     if (slots <= 0 || n_kv_heads <= 0 || N <= 0 || page_size <= 0) return 0;
     const size_t rows = (size_t)slots * n_kv_heads;
-    return 256 + align_up(rows * 4, 256) + 2 * align_up(rows * append_chunks(N, page_size) * 4, 256);
+    return 256 + align_up(rows * 4, 256) + align_up(rows * append_chunks(N, page_size) * 4, 256);
 }
 
 NATS_EXPORT int nats_b200_paged_append(const NatsPagedKV* kv, const void* d_k, const void* d_v, long long k_slot_stride, long long k_head_stride,
@@ -469,26 +558,19 @@ NATS_EXPORT int nats_b200_paged_append(const NatsPagedKV* kv, const void* d_k, c
     uint8_t* ws = (uint8_t*)d_workspace;
     p.ticket = (int32_t*)ws;
     p.counts = (int32_t*)(ws + 256);
-    p.ids = (int32_t*)(ws + 256 + align_up(rows * 4, 256));
-    p.map = p.ids + align_up(rows * p.n_chunks * 4, 256) / 4;
+    p.map = (int32_t*)(ws + 256 + align_up(rows * 4, 256));
     p.status = d_status;
     const cudaStream_t st = (cudaStream_t)stream;
-    if (skip_hidden) {
-        paged_count_kernel<<<(unsigned)rows, kTabThreads, 0, st>>>(p);
-        paged_append_kernel<true><<<(unsigned)rows, kTabThreads, 0, st>>>(p);
-    } else {
-        paged_append_kernel<false><<<(unsigned)rows, kTabThreads, 0, st>>>(p);
-    }
-    if (!p.copy_here) paged_copy_kernel<<<dim3(cdiv(N, kCopyTokens), (unsigned)rows), kTabThreads, 0, st>>>(p);
-    NATS_CHECK_CUDA(cudaGetLastError());
+    if (skip_hidden) NATS_CHECK_CUDA(launch_behind(paged_count_kernel, (unsigned)rows, 0, st, p));
+    NATS_CHECK_CUDA(launch_behind(skip_hidden ? paged_append_kernel<true> : paged_append_kernel<false>, (unsigned)rows, 0, st, p));
+    if (!p.copy_here) NATS_CHECK_CUDA(launch_behind(paged_copy_kernel, dim3(cdiv(N, kCopyTokens), (unsigned)rows), 0, st, p));
     return NATS_OK;
 }
 
 NATS_EXPORT int nats_b200_paged_evict(const NatsPagedKV* d, void* stream) {
     PagedKv kv;
     if (const int e = paged_kv(d, kv)) return e;
-    paged_evict_kernel<<<kv.S * kv.H, kTabThreads, 0, (cudaStream_t)stream>>>(kv);
-    NATS_CHECK_CUDA(cudaGetLastError());
+    NATS_CHECK_CUDA(launch_behind(paged_evict_kernel, kv.S * kv.H, 0, (cudaStream_t)stream, kv));
     return NATS_OK;
 }
 
@@ -514,8 +596,7 @@ NATS_EXPORT int nats_b200_paged_reorder(const NatsPagedKV* kv, const int32_t* d_
     p.entries = (int4*)(ws + 256 + align_up((size_t)p.kv.S * 4, 256) + align_up(rows * 4, 256));
     p.status = d_status;
     const cudaStream_t st = (cudaStream_t)stream;
-    paged_release_kernel<<<(unsigned)rows, kTabThreads, 0, st>>>(p);
-    paged_move_kernel<<<(unsigned)rows, kTabThreads, p.kv.S * 4, st>>>(p);
-    NATS_CHECK_CUDA(cudaGetLastError());
+    NATS_CHECK_CUDA(launch_behind(paged_release_kernel, (unsigned)rows, 0, st, p));
+    NATS_CHECK_CUDA(launch_behind(paged_move_kernel, (unsigned)rows, p.kv.S * 4, st, p));
     return NATS_OK;
 }

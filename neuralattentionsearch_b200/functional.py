@@ -14,7 +14,6 @@ with PyTorch ops: if the CUDA library is missing the import of ``_lib`` raises.
 """
 from __future__ import annotations
 
-import ctypes
 import math
 
 import torch
@@ -663,32 +662,69 @@ class PagedKV:
     def __init__(self, pages_k: torch.Tensor, pages_v: torch.Tensor, refs: torch.Tensor, free_bits: torch.Tensor, entries: torch.Tensor,
                  n_pages: torch.Tensor, length: torch.Tensor):
         tensors = (pages_k, pages_v, refs, free_bits, entries, n_pages, length)
-        self.device = _need_cuda(*tensors)
         n, P, D = pages_k.shape
         S, H, M, four = entries.shape
-        if pages_k.dtype != torch.bfloat16 or pages_v.dtype != torch.bfloat16 or pages_v.shape != pages_k.shape:
+        if pages_k.dtype is not torch.bfloat16 or pages_v.dtype is not torch.bfloat16 or pages_v.shape != pages_k.shape:
             raise ValueError('pages_k and pages_v must be bf16 [pages, page_size, head_dim]')
-        for t, shape, name in ((refs, (n,), 'refs'), (free_bits, (-(-n // 32),), 'free_bits'), (entries, (S, H, M, 4), 'entries'),
+        for t, shape, name in ((refs, (n,), 'refs'), (free_bits, ((n + 31) // 32,), 'free_bits'), (entries, (S, H, M, 4), 'entries'),
                                (n_pages, (S, H), 'n_pages'), (length, (S,), 'length')):
-            if t.dtype != torch.int32 or t.shape != shape:
+            if t.dtype is not torch.int32 or t.shape != shape:
                 raise ValueError(f'{name} must be int32 {list(shape)}, got {t.dtype} {list(t.shape)}')
-        if not all(t.is_contiguous() for t in tensors):
-            raise ValueError('the tensors of a paged cache must be contiguous')
+        self.index = index = pages_k.get_device()
+        for t in tensors:
+            if t.get_device() != index or index < 0:
+                _need_cuda(*tensors)
+            if not t.is_contiguous():
+                raise ValueError('the tensors of a paged cache must be contiguous')
         if P not in PAGE_SIZES:
             raise ValueError(f'page size {P}: {PAGE_SIZES} are supported')
         if D not in PAGED_HEAD_DIMS:
             raise NotImplementedError(f'head_dim {D}: the paged cache is built for {PAGED_HEAD_DIMS}')
         self.pages_k, self.pages_v, self.refs, self.free_bits, self.entries, self.n_pages, self.length = tensors
         self.num_pages, self.page_size, self.head_dim, self.slots, self.n_kv_heads, self.max_entries = n, P, D, S, H, M
-        self._c = _lib.NatsPagedKV(*(t.data_ptr() for t in tensors), n, P, D, S, H, M)
-        self._ref = ctypes.byref(self._c)
+        self._c = _lib.NatsPagedKV(pages_k.data_ptr(), pages_v.data_ptr(), refs.data_ptr(), free_bits.data_ptr(), entries.data_ptr(),
+                                   n_pages.data_ptr(), length.data_ptr(), n, P, D, S, H, M)
+
+    @property
+    def device(self) -> torch.device:
+        return self.pages_k.device
+
+    def _check(self, *tensors: torch.Tensor) -> None:
+        for t in tensors:
+            if t.get_device() != self.index:
+                _need_cuda(self.pages_k, t)
 
 
-def _paged_workspace(kind: str, device: torch.device, nbytes: int) -> torch.Tensor:
-    """Zeroed scratch of the current stream.  While a graph is recorded it is the graph's own, so that two recorded graphs never share it."""
+_paged_bytes: dict[tuple, int] = {}
+
+
+def _paged_scratch(name: str, index: int, stream: int, *sizes: int) -> torch.Tensor:
+    """Zeroed scratch for the entry point ``nats_b200_paged_<name>``, one per stream.  While a graph is recorded it is the graph's own, so that two
+    recorded graphs never share it."""
+    key = (name, *sizes)
+    nbytes = _paged_bytes.get(key)
+    if nbytes is None:
+        nbytes = _paged_bytes[key] = getattr(_lib.lib(), f'nats_b200_paged_{name}_workspace_bytes')(*sizes)
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=device)
-    return _workspace(kind, device, nbytes, zero=True)
+        return torch.zeros(nbytes, dtype=torch.uint8, device=index)
+    key = (name, index, stream)
+    ws = _workspaces.get(key)
+    if ws is None or ws.numel() < nbytes:
+        ws = _workspaces[key] = torch.zeros(nbytes, dtype=torch.uint8, device=index)
+    return ws
+
+
+def _on(index: int, fn, *args):
+    """``fn(*args)`` with the device of the cache current."""
+    if index == torch.cuda.current_device():
+        return fn(*args)
+    with torch.cuda.device(index):
+        return fn(*args)
+
+
+def _status_ptr(index: int) -> int:
+    t = _status.get(index)
+    return (t if t is not None else status_word(torch.device('cuda', index))).data_ptr()
 
 
 def _strided_ok(t: torch.Tensor) -> bool:
@@ -701,7 +737,7 @@ def _strided_ok(t: torch.Tensor) -> bool:
 def _check_n_new(kv: PagedKV, n_new: torch.Tensor | None) -> int | None:
     if n_new is None:
         return None
-    if n_new.dtype != torch.int32 or n_new.shape != (kv.slots,) or n_new.device != kv.device or not n_new.is_contiguous():
+    if n_new.dtype is not torch.int32 or n_new.shape != (kv.slots,) or n_new.get_device() != kv.index or not n_new.is_contiguous():
         raise ValueError(f'n_new must be int32 [{kv.slots}] on {kv.device}')
     return n_new.data_ptr()
 
@@ -714,27 +750,34 @@ def paged_append(kv: PagedKV, k_new: torch.Tensor, v_new: torch.Tensor, roles: t
     global.  A chunk that a call completes gets its limit from its role; a completed global one closes the local ones in front.
     ``skip_hidden``: whole chunks that no query behind this call sees are not stored -- for a prompt whose attention does not
     read the pages.  Running out of pages or of entries raises the device's status word (``check_status``)."""
-    dev = _need_cuda(kv.pages_k, k_new, v_new)
-    S, H, N, D = k_new.shape
-    if (S, H, D) != (kv.slots, kv.n_kv_heads, kv.head_dim) or v_new.shape != k_new.shape:
+    kv._check(k_new, v_new)
+    S, H, N, D = shape = k_new.shape
+    if S != kv.slots or H != kv.n_kv_heads or D != kv.head_dim or v_new.shape != shape:
         raise ValueError(f'k_new / v_new must be [{kv.slots},{kv.n_kv_heads},N,{kv.head_dim}], got {tuple(k_new.shape)} / {tuple(v_new.shape)}')
-    if roles is not None and (roles.dtype != torch.uint8 or roles.dim() != 3 or roles.shape[:2] != (S, H) or roles.device != dev):
-        raise ValueError(f'roles must be uint8 [{S},{H},chunks] on {dev}')
-    lens = _check_n_new(kv, n_new)
-    if N == 0:
-        return
-    if k_new.dtype != v_new.dtype or k_new.dtype not in (torch.bfloat16, torch.float32):
-        k_new, v_new = k_new.to(torch.bfloat16), v_new.to(torch.bfloat16)
-    if not _strided_ok(k_new):
-        k_new = k_new.contiguous()
-    if not _strided_ok(v_new):
-        v_new = v_new.contiguous()
-    if roles is not None and not roles.is_contiguous():
+    n_roles, roles_ptr = 0, None
+    if roles is not None:
+        if roles.dtype is not torch.uint8 or roles.dim() != 3 or roles.shape[:2] != shape[:2] or roles.get_device() != kv.index:
+            raise ValueError(f'roles must be uint8 [{S},{H},chunks] on {kv.device}')
         roles = roles.contiguous()
-    ws = _paged_workspace('paged_append', dev, _lib.lib().nats_b200_paged_append_workspace_bytes(S, H, N, kv.page_size))
-    _call(dev, 'nats_b200_paged_append', kv._ref, k_new.data_ptr(), v_new.data_ptr(), *k_new.stride()[:3], *v_new.stride()[:3],
-          int(k_new.dtype == torch.float32), _p(roles), 0 if roles is None else roles.shape[2], lens, N, sliding_window, int(skip_hidden),
-          ws.data_ptr(), ws.numel(), status_word(dev).data_ptr(), _stream(dev))
+        n_roles, roles_ptr = roles.shape[2], roles.data_ptr()
+    lens = _check_n_new(kv, n_new)
+    if N > 0:
+        _on(kv.index, _paged_append, kv, k_new, v_new, n_roles, roles_ptr, lens, N, sliding_window, skip_hidden)
+
+
+def _paged_append(kv, k, v, n_roles, roles_ptr, lens, N, sliding_window, skip_hidden):
+    if k.dtype is not v.dtype or (k.dtype is not torch.bfloat16 and k.dtype is not torch.float32):
+        k, v = k.to(torch.bfloat16), v.to(torch.bfloat16)
+    if not _strided_ok(k):
+        k = k.contiguous()
+    if not _strided_ok(v):
+        v = v.contiguous()
+    stream = torch._C._cuda_getCurrentRawStream(kv.index)
+    ws = _paged_scratch('append', kv.index, stream, kv.slots, kv.n_kv_heads, N, kv.page_size)
+    ka, kb, kc, _ = k.stride()
+    va, vb, vc, _ = v.stride()
+    _lib.call('nats_b200_paged_append', kv._c, k.data_ptr(), v.data_ptr(), ka, kb, kc, va, vb, vc, k.dtype is torch.float32, roles_ptr, n_roles,
+              lens, N, sliding_window, skip_hidden, ws.data_ptr(), ws.numel(), _status_ptr(kv.index), stream)
 
 
 def paged_attention(kv: PagedKV, q: torch.Tensor, sm_scale: float | None = None, n_new: torch.Tensor | None = None,
@@ -744,7 +787,7 @@ def paged_attention(kv: PagedKV, q: torch.Tensor, sm_scale: float | None = None,
     (``n_new`` int32 [S]; None: N everywhere).  A key is seen from its own position on up to the limit of its page.  Rows behind a slot's
     new tokens and rows that see nothing are zero.  ``max_pages``: a bound of ``n_pages`` the host knows (the work is split by it; the
     result does not depend on its being right).  Returns o [S,Hq,N,D] in q's dtype; ``token_major``: a view of a [S,N,Hq,D] tensor."""
-    dev = _need_cuda(kv.pages_k, q)
+    kv._check(q)
     S, Hq, N, D = q.shape
     if S != kv.slots or D != kv.head_dim or Hq == 0 or Hq % kv.n_kv_heads:
         raise ValueError(f'q must be [{kv.slots},multiple of {kv.n_kv_heads},N,{kv.head_dim}], got {tuple(q.shape)}')
@@ -752,25 +795,35 @@ def paged_attention(kv: PagedKV, q: torch.Tensor, sm_scale: float | None = None,
     scale = D ** -0.5 if sm_scale is None else float(sm_scale)
     if not scale > 0.0:
         raise ValueError('sm_scale must be positive')
-    dtype = torch.float32 if q.dtype == torch.float32 else torch.bfloat16      # fp32 callers: the kernel writes fp32 itself
-    o = torch.empty((S, N, Hq, D) if token_major else (S, Hq, N, D), dtype=dtype, device=dev)
-    if token_major:
-        o = o.transpose(1, 2)
+    bound = kv.max_entries if max_pages is None else max(0, min(int(max_pages), kv.max_entries))
+    return _on(kv.index, _paged_attention, kv, q, scale, lens, bound, token_major)
+
+
+def _paged_attention(kv, q, scale, lens, bound, token_major):
+    S, Hq, N, D = q.shape
+    f32 = q.dtype is torch.float32                       # fp32 callers: the kernel writes fp32 itself
+    dtype = torch.float32 if f32 else torch.bfloat16
+    o = torch.empty((S, N, Hq, D), dtype=dtype, device=kv.device).transpose(1, 2) if token_major else torch.empty((S, Hq, N, D), dtype=dtype, device=kv.device)
     if N > 0:
-        qb = q if q.dtype == torch.bfloat16 else q.to(torch.bfloat16)
+        qb = q if q.dtype is torch.bfloat16 else q.to(torch.bfloat16)
         if not _strided_ok(qb) or 0 in qb.stride():
             qb = qb.contiguous()
-        bound = kv.max_entries if max_pages is None else max(0, min(int(max_pages), kv.max_entries))
-        ws = _paged_workspace('paged_attention', dev, _lib.lib().nats_b200_paged_attention_workspace_bytes(S, Hq, kv.n_kv_heads, N, D, kv.page_size, bound,
-                                                                                                           kv.max_entries))
-        _call(dev, 'nats_b200_paged_attention', kv._ref, qb.data_ptr(), *qb.stride()[:3], o.data_ptr(), *o.stride()[:3],
-              int(dtype == torch.float32), lens, Hq, N, bound, scale, ws.data_ptr(), ws.numel(), status_word(dev).data_ptr(), _stream(dev))
-    return o if o.dtype == q.dtype else o.to(q.dtype)
+        stream = torch._C._cuda_getCurrentRawStream(kv.index)
+        ws = _paged_scratch('attention', kv.index, stream, S, Hq, kv.n_kv_heads, N, D, kv.page_size, bound, kv.max_entries)
+        qs, qh, qt, _ = qb.stride()
+        os, oh, ot, _ = o.stride()
+        _lib.call('nats_b200_paged_attention', kv._c, qb.data_ptr(), qs, qh, qt, o.data_ptr(), os, oh, ot, f32, lens, Hq, N, bound, scale,
+                  ws.data_ptr(), ws.numel(), _status_ptr(kv.index), stream)
+    return o if o.dtype is q.dtype else o.to(q.dtype)
 
 
 def paged_evict(kv: PagedKV) -> None:
     """Pages that the next query position (``length``) cannot see leave the rows; those that lose their last holder are free again."""
-    _call(kv.device, 'nats_b200_paged_evict', kv._ref, _stream(kv.device))
+    _on(kv.index, _paged_evict, kv)
+
+
+def _paged_evict(kv):
+    _lib.call('nats_b200_paged_evict', kv._c, torch._C._cuda_getCurrentRawStream(kv.index))
 
 
 def paged_reorder(kv: PagedKV, src: torch.Tensor) -> None:
@@ -778,8 +831,12 @@ def paged_reorder(kv: PagedKV, src: torch.Tensor) -> None:
     survivors of a beam step, sequences dropped.  Whole pages are shared; the unfinished page stays with its own slot if that keeps its
     sequence, else with the first one that takes it, and is copied for the others.  A number out of range raises the device's status
     word (``check_status``) and leaves the slot empty."""
-    if src.dtype != torch.int32 or src.shape != (kv.slots,) or src.device != kv.device or not src.is_contiguous():
+    if src.dtype is not torch.int32 or src.shape != (kv.slots,) or src.get_device() != kv.index or not src.is_contiguous():
         raise ValueError(f'src must be int32 [{kv.slots}] on {kv.device}')
-    dev = kv.device
-    ws = _paged_workspace('paged_reorder', dev, _lib.lib().nats_b200_paged_reorder_workspace_bytes(kv.slots, kv.n_kv_heads, kv.max_entries))
-    _call(dev, 'nats_b200_paged_reorder', kv._ref, src.data_ptr(), ws.data_ptr(), ws.numel(), status_word(dev).data_ptr(), _stream(dev))
+    _on(kv.index, _paged_reorder, kv, src)
+
+
+def _paged_reorder(kv, src):
+    stream = torch._C._cuda_getCurrentRawStream(kv.index)
+    ws = _paged_scratch('reorder', kv.index, stream, kv.slots, kv.n_kv_heads, kv.max_entries)
+    _lib.call('nats_b200_paged_reorder', kv._c, src.data_ptr(), ws.data_ptr(), ws.numel(), _status_ptr(kv.index), stream)
