@@ -29,4 +29,10 @@ int paged_kv(const NatsPagedKV* d, PagedKv& kv);
 
 __device__ __forceinline__ void paged_status(int32_t* status, int code) { atomicCAS(status, 0, code); }
 
+// A kernel that follows another one of the paged cache in a stream is launched while that one ends, and looks at memory only behind this wait.
+__device__ __forceinline__ void wait_for_launch_before() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 }  // namespace nats

@@ -6,9 +6,9 @@
 // The query rows of a kv-head are its G heads of every token, token by token (row r = G token + head in the group), so that one read of
 // a page serves the whole group and, with several new tokens, all of them.
 //
-// paged_rows_kernel: sixteen query rows per block and a split of the row's pages; four warps take 16-key tiles of it in turn, each with a ring
-// of cp.async stages of its own.  S = Q.K^T and O += P.V are mma.sync m16n8k16, whose score fragments are the A fragments of P.V.  With few
-// rows the kernel is bound by HBM.  Splits leave (max, sum, O) in the workspace and the block that arrives last joins them, in a fixed order.
+// paged_rows_kernel: sixteen or thirty-two query rows at a time; the four warps of a block take 16-key tiles of a stretch of pages in turn, each
+// with a ring of cp.async stages of its own.  S = Q.K^T and O += P.V are mma.sync m16n8k16, whose score fragments are the A fragments of P.V.
+// With few rows the kernel is bound by HBM.
 #include "paged_attn.cuh"
 
 namespace nats {
@@ -16,9 +16,12 @@ namespace nats {
 constexpr int kRowThreads = 128, kRowWarps = kRowThreads / 32;
 constexpr int kRowTile = 16;                     // keys per warp tile
 constexpr int kRowStages = 3;
-constexpr int kRows = 16;                        // query rows per block
-constexpr int kMaxTickets = 4096;               // joins of a launch; the workspace begins with as many words, which are zero between calls
-constexpr int kBatchTiles = 64;                  // tiles whose entries a block holds at a time, 16 per warp
+constexpr int kRows = 16;                        // query rows of an A fragment
+constexpr int kMaxTickets = 640;                 // blocks of a launch; the workspace begins with as many words, which are zero between calls
+#ifndef NATS_MIN_STRETCH
+#define NATS_MIN_STRETCH 64
+#endif
+constexpr int kMinStretch = NATS_MIN_STRETCH;    // keys of a block's stretch at least
 
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
@@ -50,243 +53,380 @@ __device__ __forceinline__ uint32_t pack_pair(float lo, float hi) {
     return r;
 }
 
-__device__ __forceinline__ void store_o(const PagedAttnParams& p, int s, int h, int r, int d, float x) {
+// four columns of a query row
+__device__ __forceinline__ void store_o(const PagedAttnParams& p, int s, int h, int r, int d, float4 x) {
     const int t = r / p.G, head = h * p.G + r - t * p.G;
     const long long at = s * p.o_slot + head * p.o_head + t * p.o_token + d;
-    if (p.o_f32) ((float*)p.o)[at] = x;
-    else ((__nv_bfloat16*)p.o)[at] = __float2bfloat16_rn(x);
+    if (p.o_f32) *reinterpret_cast<float4*>((float*)p.o + at) = x;
+    else *reinterpret_cast<uint2*>((__nv_bfloat16*)p.o + at) = make_uint2(pack_pair(x.x, x.y), pack_pair(x.z, x.w));
+}
+__device__ __forceinline__ void add_scaled(float4& a, const float4& x, float f) {
+    a.x = fmaf(x.x, f, a.x); a.y = fmaf(x.y, f, a.y); a.z = fmaf(x.z, f, a.z); a.w = fmaf(x.w, f, a.w);
+}
+__device__ __forceinline__ float4 divided(const float4& a, float l) {      // a row that has seen nothing: zero
+    return l != 0.f ? make_float4(a.x / l, a.y / l, a.z / l, a.w / l) : make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
-template <int D>
-__global__ void __launch_bounds__(kRowThreads) paged_rows_kernel(const PagedAttnParams p) {
+// Joins the parts of a unit: s_max has room for kRowThreads floats
+template <int D, int R>
+__device__ __forceinline__ void join_parts(const PagedAttnParams& p, int s, int h, int r0, int n_rows, int live, int unit_begin, int chunk,
+                                           int first, int last, float* s_max) {
+    const int tid = threadIdx.x;
+    auto part_of = [&](int x) { return p.partials + ((size_t)x * 2 + (unit_begin < x * chunk ? 0 : 1)) * R * (D + 2); };
+    // maxima of the rows over the parts: kRowThreads / R threads per row
+    const int mr = tid % R;
+    float mx = -INFINITY;
+    for (int x = first + tid / R; x <= last; x += kRowThreads / R)
+        if (mr < live) mx = fmaxf(mx, __ldcg(part_of(x) + R * D + 2 * mr));
+    s_max[tid] = mx;
+    __syncthreads();
+    for (int i = tid; i < n_rows * (D / 4); i += kRowThreads) {
+        const int r = i / (D / 4), d = i % (D / 4) * 4;
+        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+        float l = 0.f, mu = -INFINITY;
+        if (r < live) {
+#pragma unroll
+            for (int k = 0; k < kRowThreads / R; ++k) mu = fmaxf(mu, s_max[k * R + r]);
+            mu = mu == -INFINITY ? 0.f : mu;
+            constexpr int AT_ONCE = 8;             // parts on their way at a time
+            for (int x0 = first; x0 <= last; x0 += AT_ONCE) {
+                float4 o[AT_ONCE];
+                float2 ml[AT_ONCE];
+#pragma unroll
+                for (int k = 0; k < AT_ONCE; ++k) {
+                    const float* part = part_of(min(x0 + k, last));
+                    o[k] = __ldcg(reinterpret_cast<const float4*>(part + r * D + d));
+                    ml[k] = __ldcg(reinterpret_cast<const float2*>(part + R * D + 2 * r));
+                }
+#pragma unroll
+                for (int k = 0; k < AT_ONCE; ++k) {
+                    if (x0 + k > last) break;
+                    const float f = exp2_approx(ml[k].x - mu);
+                    add_scaled(a, o[k], f);
+                    l = fmaf(ml[k].y, f, l);
+                }
+            }
+        }
+        store_o(p, s, h, r0 + r, d, divided(a, l));
+    }
+}
+
+// Work is dealt in pages: the row tiles ("units": sixteen or thirty-two query rows of a (slot, kv-head)) with their pages form one line, of which
+// every block takes a stretch of the same length.  A stretch covers parts of one or more units; a unit within one stretch is written out
+// at once, of the others every part goes to the workspace, and the block that finishes the last of them joins them in order.
+// A unit without pages or without real tokens counts as one page: its zeros have to be written, too.
+struct RowShared {
+    int warp_sum[kRowWarps];
+    int row, at, pages, last;
+    int2 meta[kRowWarps][kRowStages];              // position of the first key, limit of a stage's tile
+};
+
+__device__ __forceinline__ int row_tokens(const PagedAttnParams& p, int s) { return p.n_new == nullptr ? p.N : min(max(p.n_new[s], 0), p.N); }
+// pages of a unit on the line
+__device__ __forceinline__ int unit_pages(const PagedKv& kv, int row, bool live) { return live ? max(min(kv.n_pages[row], kv.M), 1) : 1; }
+
+template <int D, int MT>
+__global__ void __launch_bounds__(kRowThreads, MT == 1 && D == 64 ? 4 : 2) paged_rows_kernel(const PagedAttnParams p) {
     constexpr int ROWB = D * 2, CHUNKS = ROWB / 16, TILE_BYTES = kRowTile * ROWB, STAGE_BYTES = 2 * TILE_BYTES;
-    constexpr int CP_PER_LANE = kRowTile * CHUNKS / 32, ROWS_PER_CP = 32 / CHUNKS, PSTRIDE = D + 2;
+    constexpr int CP_PER_LANE = kRowTile * CHUNKS / 32, ROWS_PER_CP = 32 / CHUNKS, PSTRIDE = D + 2, R = 16 * MT;
     constexpr unsigned FULL = 0xffffffffu;
     extern __shared__ __align__(128) uint8_t dsm[];
-    __shared__ int s_last;
-    float (*s_acc)[kRows][D] = reinterpret_cast<float (*)[kRows][D]>(dsm);
-    float (*s_m)[kRows] = reinterpret_cast<float (*)[kRows]>(dsm + kRowWarps * kRows * D * 4);
-    float (*s_l)[kRows] = reinterpret_cast<float (*)[kRows]>(dsm + kRowWarps * kRows * (D + 1) * 4);
-    static_assert(kRowWarps * kRows * (D + 2) * 4 <= kRowWarps * kRowStages * STAGE_BYTES, "the join's scratch must fit into the ring");
+    __shared__ RowShared sh;
+    float (*s_acc)[R][D] = reinterpret_cast<float (*)[R][D]>(dsm);
+    float (*s_m)[R] = reinterpret_cast<float (*)[R]>(dsm + kRowWarps * R * D * 4);
+    float (*s_l)[R] = reinterpret_cast<float (*)[R]>(dsm + kRowWarps * R * (D + 1) * 4);
+    static_assert(kRowWarps * R * (D + 2) * 4 <= kRowWarps * kRowStages * STAGE_BYTES, "the join's scratch must fit into the ring");
 
     const PagedKv& kv = p.kv;
-    const int split = blockIdx.x, rt = blockIdx.y, row = blockIdx.z, s = row / kv.H, h = row - s * kv.H;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    const int P = kv.P, n = p.n_new == nullptr ? p.N : min(max(p.n_new[s], 0), p.N);
-    const int r0 = rt * kRows, n_rows = min(kRows, p.N * p.G - r0);              // query rows of this block, padded ones among them
-    const int q0 = kv.length[s] - n;                                            // position of the first new token
-    const int4* entries = kv.entries + (size_t)row * kv.M;
-    const int n_pages = min(max(kv.n_pages[row], 0), kv.M);
-    const int live = min(n_rows, n * p.G - r0);                                 // query rows of real tokens
-    const int nsplit = live > 0 ? max(1, min((n_pages + p.split_pages - 1) / p.split_pages, p.splits)) : 1;
-    if (split >= nsplit) return;
-    if (live <= 0) {
-        for (int i = tid; i < n_rows * D; i += kRowThreads) store_o(p, s, h, r0 + i / D, i % D, 0.f);
-        return;
-    }
-    const int first_pos = q0 + r0 / p.G, last_pos = q0 + (r0 + live - 1) / p.G;
-    const int e_end = split == p.splits - 1 ? n_pages : min(n_pages, (split + 1) * p.split_pages);
+    const int P = kv.P, tpp = P / kRowTile, n_rows_all = kv.S * kv.H;
+    wait_for_launch_before();
 
-    // Q as A fragments: rows quad_row and quad_row + 8
-    const int qr = lane >> 2, quad = lane & 3;
-    uint32_t qa[D / 16][4];
-    int qpos[2];
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        const int r = qr + 8 * i;
-        const bool ok = r < live;
-        const int t = (r0 + r) / p.G, head = h * p.G + (r0 + r) - t * p.G;
-        qpos[i] = ok ? q0 + t : -1;
-        const __nv_bfloat16* src = p.q + s * p.q_slot + head * p.q_head + t * p.q_token + quad * 2;
-#pragma unroll
-        for (int ks = 0; ks < D / 16; ++ks) {
-            qa[ks][i] = ok ? *reinterpret_cast<const uint32_t*>(src + ks * 16) : 0u;
-            qa[ks][2 + i] = ok ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8) : 0u;
-        }
+    // ---- the line: its length, and the unit at the beginning of this block's stretch ----
+    const int per = (n_rows_all + kRowThreads - 1) / kRowThreads;
+    auto row_pages = [&](int row) {
+        const int n = row_tokens(p, row / kv.H), live = min((n * p.G + R - 1) / R, p.row_tiles);
+        return live * unit_pages(kv, row, true) + p.row_tiles - live;
+    };
+    int sum = 0;
+    for (int i = 0; i < per; ++i) {
+        const int row = tid * per + i;
+        if (row < n_rows_all) sum += row_pages(row);
     }
-    float oacc[D / 8][4];
+    const int incl = warp_incl_scan(sum, lane);
+    if (lane == 31) sh.warp_sum[warp] = incl;
+    __syncthreads();
+    int before = incl - sum, total = 0;
 #pragma unroll
-    for (int i = 0; i < D / 8; ++i) { oacc[i][0] = oacc[i][1] = oacc[i][2] = oacc[i][3] = 0.f; }
-    float m_run[2] = {-INFINITY, -INFINITY}, l_run[2] = {0.f, 0.f};
+    for (int w = 0; w < kRowWarps; ++w) { if (w < warp) before += sh.warp_sum[w]; total += sh.warp_sum[w]; }
+    const int chunk = max((total + (int)gridDim.x - 1) / (int)gridDim.x, p.split_pages);
+    const int begin = (int)min((long long)blockIdx.x * chunk, (long long)total), end = (int)min((long long)begin + chunk, (long long)total);
+    if (begin >= end) return;
+    if (before <= begin && begin < before + sum) {
+        int at = before, row = tid * per;
+        for (int w; at + (w = row_pages(row)) <= begin; ++row) at += w;
+        sh.row = row;
+        sh.at = at;
+        sh.pages = kv.n_pages[row];
+    }
+    __syncthreads();
+    int row = sh.row, row_begin = sh.at;           // where the row begins on the line
+    int next_pages = sh.pages, next_length = kv.length[row / kv.H], next_n = row_tokens(p, row / kv.H);
 
-    const uint32_t ring = (uint32_t)__cvta_generic_to_shared(dsm) + warp * kRowStages * STAGE_BYTES;
-    const int tpp = P / kRowTile;                                               // tiles per page
-    for (int e0 = split * p.split_pages; e0 < e_end; e0 += kBatchTiles / tpp) {
-        // lane i < 16 holds the entry of this warp's i-th tile of the batch: tiles warp, warp + 4, ...
-        const int tile = warp + kRowWarps * lane, ei = e0 + tile / tpp;
-        int4 e = make_int4(-1, 0, -1, 0);
-        if (lane < kBatchTiles / kRowWarps && ei < e_end) {
-            e = entries[ei];
-            e.y += tile % tpp * kRowTile;                                       // position of the tile's first key
-            e.w = tile % tpp * kRowTile;                                        // its row in the page
-            if ((unsigned)e.x >= (unsigned)kv.num_pages) e.z = -1;
+    for (int line = begin; line < end; ++row) {
+        const int s = row / kv.H, h = row - s * kv.H, n = next_n;
+        const int q0 = next_length - n, n_pages = min(max(next_pages, 0), kv.M);
+        if (row + 1 < n_rows_all) {                // asked for while this row is worked on
+            const int s1 = (row + 1) / kv.H;
+            next_pages = kv.n_pages[row + 1]; next_length = kv.length[s1]; next_n = row_tokens(p, s1);
         }
-        const unsigned seen = __ballot_sync(FULL, lane < kBatchTiles / kRowWarps && e.z >= first_pos && e.y <= last_pos);
-        const int tiles = __popc(seen);
-        unsigned to_load = seen, to_use = seen;
-        auto issue = [&](int it) {
-            const int from = __ffs(to_load) - 1;
-            to_load &= to_load - 1u;
-            const int page = __shfl_sync(FULL, e.x, from), pos = __shfl_sync(FULL, e.y, from), at = __shfl_sync(FULL, e.w, from);
-            const size_t off = ((size_t)page * P + at) * ROWB + (lane % CHUNKS) * 16;
-            const uint32_t dst = ring + (it % kRowStages) * STAGE_BYTES;
-#pragma unroll
-            for (int x = 0; x < CP_PER_LANE; ++x) {
-                const int r = x * ROWS_PER_CP + lane / CHUNKS, c = lane % CHUNKS;
-                const bool ok = pos + r <= last_pos;                            // rows that nobody sees yet may hold anything: zeros instead
-                const uint32_t to = dst + r * ROWB + ((c ^ (r & 7)) << 4);
-                cp16(to, kv.k + off + (size_t)r * ROWB, ok);
-                cp16(to + TILE_BYTES, kv.v + off + (size_t)r * ROWB, ok);
+        const int4* entries = kv.entries + (size_t)row * kv.M;
+        int unit_begin = row_begin;
+        for (int rt = 0; rt < p.row_tiles && line < end; ++rt) {
+            const int r0 = rt * R, n_rows = min(R, p.N * p.G - r0), live = min(n_rows, n * p.G - r0);   // rows of the unit, those of real tokens
+            const int pages = live > 0 ? max(n_pages, 1) : 1, unit_end = unit_begin + pages;
+            if (unit_end <= line) { unit_begin = unit_end; continue; }
+            const int first_block = unit_begin / chunk, last_block = (unit_end - 1) / chunk;
+            const int e_first = line - unit_begin, e_end = min(min(end, unit_end) - unit_begin, n_pages);
+            if (live <= 0) {
+                for (int i = tid; i < n_rows * (D / 4); i += kRowThreads) store_o(p, s, h, r0 + i / (D / 4), i % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
+                line = unit_end;
+                unit_begin = unit_end;
+                continue;
             }
-        };
+            const int first_pos = q0 + r0 / p.G, last_pos = q0 + (r0 + live - 1) / p.G;
+
+            // ---- Q as A fragments, sixteen rows each: rows qr and qr + 8 ----
+            const int qr = lane >> 2, quad = lane & 3;
+            uint32_t qa[MT][D / 16][4];
+            int qpos[MT][2];
 #pragma unroll
-        for (int it = 0; it < kRowStages - 1; ++it) {
-            if (it < tiles) issue(it);
-            cp_commit();
-        }
-        for (int it = 0; it < tiles; ++it) {
-            __syncwarp();                                                       // everybody has read the stage that is filled now
-            if (it + kRowStages - 1 < tiles) issue(it + kRowStages - 1);
-            cp_commit();
-            cp_wait<kRowStages - 1>();
-            __syncwarp();
-            const int from = __ffs(to_use) - 1;
-            to_use &= to_use - 1u;
-            const int pos = __shfl_sync(FULL, e.y, from), limit = __shfl_sync(FULL, e.z, from);
-            const uint32_t sk = ring + (it % kRowStages) * STAGE_BYTES, sv = sk + TILE_BYTES;
-            float sc[2][4];
+            for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int nt = 0; nt < 2; ++nt) {
-                sc[nt][0] = sc[nt][1] = sc[nt][2] = sc[nt][3] = 0.f;
-                const int r = nt * 8 + (lane & 7);
+                for (int i = 0; i < 2; ++i) {
+                    const int r = 16 * m + qr + 8 * i;
+                    const bool ok = r < live;
+                    const int t = (r0 + r) / p.G, head = h * p.G + (r0 + r) - t * p.G;
+                    qpos[m][i] = ok ? q0 + t : -1;
+                    const __nv_bfloat16* src = p.q + s * p.q_slot + head * p.q_head + t * p.q_token + quad * 2;
 #pragma unroll
-                for (int kp = 0; kp < D / 32; ++kp) {
-                    uint32_t kb[4];
-                    const int chunk = kp * 4 + (lane >> 3);
-                    ldsm4(sk + r * ROWB + ((chunk ^ (r & 7)) << 4), kb);
-                    mma16816(sc[nt], qa[2 * kp], kb[0], kb[1]);
-                    mma16816(sc[nt], qa[2 * kp + 1], kb[2], kb[3]);
+                    for (int ks = 0; ks < D / 16; ++ks) {
+                        qa[m][ks][i] = ok ? *reinterpret_cast<const uint32_t*>(src + ks * 16) : 0u;
+                        qa[m][ks][2 + i] = ok ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + 8) : 0u;
+                    }
+                }
+            float oacc[MT][D / 8][4];
+            float m_run[MT][2], l_run[MT][2];
+#pragma unroll
+            for (int m = 0; m < MT; ++m) {
+#pragma unroll
+                for (int i = 0; i < D / 8; ++i) { oacc[m][i][0] = oacc[m][i][1] = oacc[m][i][2] = oacc[m][i][3] = 0.f; }
+                m_run[m][0] = m_run[m][1] = -INFINITY;
+                l_run[m][0] = l_run[m][1] = 0.f;
+            }
+
+            // ---- this warp's tiles: warp, warp + 4, ... of the stretch's; lane i holds the entry of the i-th of a window of 32 ----
+            const int n_tiles = max(e_end - e_first, 0) * tpp, my_tiles = (n_tiles - warp + kRowWarps - 1) / kRowWarps;
+            const uint32_t ring = (uint32_t)__cvta_generic_to_shared(dsm) + warp * kRowStages * STAGE_BYTES;
+            auto window = [&](int w0) {
+                int4 e = make_int4(-1, 0, -1, 0);
+                const int tile = warp + kRowWarps * (w0 + lane);
+                if (w0 + lane < my_tiles) {
+                    e = entries[e_first + tile / tpp];
+                    e.w = tile % tpp * kRowTile;                                    // the tile's first row in the page
+                    e.y += e.w;                                                     // ... and its position
+                    if ((unsigned)e.x >= (unsigned)kv.num_pages) e.z = -1;
+                }
+                return e;
+            };
+            int4 e = window(0), ahead = window(32);
+            int w0 = 0;
+            unsigned seen = __ballot_sync(FULL, e.z >= first_pos && e.y <= last_pos);
+            int stage_in = 0;
+            // copies of the next tile that some row sees; false: there is none left
+            auto issue = [&]() {
+                while (seen == 0u) {
+                    w0 += 32;
+                    if (w0 >= my_tiles) return false;
+                    e = ahead;
+                    ahead = window(w0 + 32);
+                    seen = __ballot_sync(FULL, e.z >= first_pos && e.y <= last_pos);
+                }
+                const int from = __ffs(seen) - 1;
+                seen &= seen - 1u;
+                const int page = __shfl_sync(FULL, e.x, from), pos = __shfl_sync(FULL, e.y, from), at = __shfl_sync(FULL, e.w, from);
+                const int limit = __shfl_sync(FULL, e.z, from);
+                const size_t off = ((size_t)page * P + at) * ROWB + (lane % CHUNKS) * 16;
+                const uint32_t dst = ring + stage_in * STAGE_BYTES;
+#pragma unroll
+                for (int x = 0; x < CP_PER_LANE; ++x) {
+                    const int r = x * ROWS_PER_CP + lane / CHUNKS, c = lane % CHUNKS;
+                    const bool ok = pos + r <= last_pos;                            // rows that nobody sees yet may hold anything: zeros instead
+                    const uint32_t to = dst + r * ROWB + ((c ^ (r & 7)) << 4);
+                    cp16(to, kv.k + off + (size_t)r * ROWB, ok);
+                    cp16(to + TILE_BYTES, kv.v + off + (size_t)r * ROWB, ok);
+                }
+                if (lane == 0) sh.meta[warp][stage_in] = make_int2(pos, limit);
+                stage_in = stage_in + 1 == kRowStages ? 0 : stage_in + 1;
+                return true;
+            };
+            int in_flight = 0;
+            bool more = true;
+#pragma unroll
+            for (int i = 0; i < kRowStages - 1; ++i) {
+                more = more && issue();
+                in_flight += more;
+                cp_commit();
+            }
+            for (int stage = 0; in_flight > 0; stage = stage + 1 == kRowStages ? 0 : stage + 1) {
+                __syncwarp();                                                       // everybody has read the stage that is filled now
+                more = more && issue();
+                in_flight += (int)more - 1;
+                cp_commit();
+                cp_wait<kRowStages - 1>();
+                __syncwarp();
+                const int2 meta = sh.meta[warp][stage];
+                const int pos = meta.x, limit = meta.y;
+                const uint32_t sk = ring + stage * STAGE_BYTES, sv = sk + TILE_BYTES;
+                float sc[MT][2][4];
+#pragma unroll
+                for (int nt = 0; nt < 2; ++nt) {
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) sc[m][nt][0] = sc[m][nt][1] = sc[m][nt][2] = sc[m][nt][3] = 0.f;
+                    const int r = nt * 8 + (lane & 7);
+#pragma unroll
+                    for (int kp = 0; kp < D / 32; ++kp) {
+                        uint32_t kb[4];
+                        const int c = kp * 4 + (lane >> 3);
+                        ldsm4(sk + r * ROWB + ((c ^ (r & 7)) << 4), kb);
+#pragma unroll
+                        for (int m = 0; m < MT; ++m) {
+                            mma16816(sc[m][nt], qa[m][2 * kp], kb[0], kb[1]);
+                            mma16816(sc[m][nt], qa[m][2 * kp + 1], kb[2], kb[3]);
+                        }
+                    }
+                }
+                const bool whole = pos + kRowTile - 1 <= first_pos && limit >= last_pos && live == R;
+                uint32_t pa[MT][4];
+#pragma unroll
+                for (int m = 0; m < MT; ++m) {
+                    float alpha[2];
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        float x[4];
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) {
+                            const int key = pos + (j >> 1) * 8 + quad * 2 + (j & 1);
+                            const bool ok = whole || (key <= qpos[m][i] && qpos[m][i] <= limit);
+                            x[j] = ok ? sc[m][j >> 1][2 * i + (j & 1)] * p.scale_log2 : -INFINITY;
+                        }
+                        float mt = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
+                        mt = fmaxf(mt, __shfl_xor_sync(FULL, mt, 1));
+                        mt = fmaxf(mt, __shfl_xor_sync(FULL, mt, 2));
+                        const float m_new = fmaxf(m_run[m][i], mt), mu = m_new == -INFINITY ? 0.f : m_new;
+                        alpha[i] = exp2_approx(m_run[m][i] - mu);
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) x[j] = exp2_approx(x[j] - mu);
+                        l_run[m][i] = l_run[m][i] * alpha[i] + (x[0] + x[1]) + (x[2] + x[3]);
+                        m_run[m][i] = m_new;
+                        pa[m][i] = pack_pair(x[0], x[1]);                           // P in bf16: the other operand of the product is
+                        pa[m][2 + i] = pack_pair(x[2], x[3]);
+                    }
+                    if (__any_sync(FULL, alpha[0] != 1.f || alpha[1] != 1.f)) {
+#pragma unroll
+                        for (int i = 0; i < D / 8; ++i) {
+                            oacc[m][i][0] *= alpha[0]; oacc[m][i][1] *= alpha[0];
+                            oacc[m][i][2] *= alpha[1]; oacc[m][i][3] *= alpha[1];
+                        }
+                    }
+                }
+#pragma unroll
+                for (int np = 0; np < D / 16; ++np) {
+                    uint32_t vb[4];
+                    const int r = ((lane >> 3) & 1) * 8 + (lane & 7), c = np * 2 + (lane >> 4);
+                    ldsm4_t(sv + r * ROWB + ((c ^ (r & 7)) << 4), vb);
+#pragma unroll
+                    for (int m = 0; m < MT; ++m) {
+                        mma16816(oacc[m][2 * np], pa[m], vb[0], vb[1]);
+                        mma16816(oacc[m][2 * np + 1], pa[m], vb[2], vb[3]);
+                    }
                 }
             }
-            const bool whole = pos + kRowTile - 1 <= first_pos && limit >= last_pos && live == kRows;
-            uint32_t pa[4];
-            float alpha[2];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) {
-                float x[4];
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    const int key = pos + (j >> 1) * 8 + quad * 2 + (j & 1);
-                    const bool ok = whole || (key <= qpos[i] && qpos[i] <= limit);
-                    x[j] = ok ? sc[j >> 1][2 * i + (j & 1)] * p.scale_log2 : -INFINITY;
-                }
-                float mt = fmaxf(fmaxf(x[0], x[1]), fmaxf(x[2], x[3]));
-                mt = fmaxf(mt, __shfl_xor_sync(FULL, mt, 1));
-                mt = fmaxf(mt, __shfl_xor_sync(FULL, mt, 2));
-                const float m_new = fmaxf(m_run[i], mt), mu = m_new == -INFINITY ? 0.f : m_new;
-                alpha[i] = exp2_approx(m_run[i] - mu);
-#pragma unroll
-                for (int j = 0; j < 4; ++j) x[j] = exp2_approx(x[j] - mu);
-                l_run[i] = l_run[i] * alpha[i] + (x[0] + x[1]) + (x[2] + x[3]);
-                m_run[i] = m_new;
-                pa[i] = pack_pair(x[0], x[1]);                                  // P in bf16: the other operand of the product is
-                pa[2 + i] = pack_pair(x[2], x[3]);
-            }
-            if (__any_sync(FULL, alpha[0] != 1.f || alpha[1] != 1.f)) {
-#pragma unroll
-                for (int i = 0; i < D / 8; ++i) { oacc[i][0] *= alpha[0]; oacc[i][1] *= alpha[0]; oacc[i][2] *= alpha[1]; oacc[i][3] *= alpha[1]; }
-            }
-#pragma unroll
-            for (int np = 0; np < D / 16; ++np) {
-                uint32_t vb[4];
-                const int r = ((lane >> 3) & 1) * 8 + (lane & 7), chunk = np * 2 + (lane >> 4);
-                ldsm4_t(sv + r * ROWB + ((chunk ^ (r & 7)) << 4), vb);
-                mma16816(oacc[2 * np], pa, vb[0], vb[1]);
-                mma16816(oacc[2 * np + 1], pa, vb[2], vb[3]);
-            }
-        }
-        cp_wait<0>();
-        __syncwarp();
-    }
+            cp_wait<0>();
 
-    // ---- the warps of this block joined (the ring's memory is reused) ----
-    __syncthreads();
+            // ---- the warps of this block joined (the ring's memory is reused) ----
+            __syncthreads();
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-        l_run[i] += __shfl_xor_sync(FULL, l_run[i], 1);
-        l_run[i] += __shfl_xor_sync(FULL, l_run[i], 2);
-        const int r = qr + 8 * i;
-        if (r < live) {
-            if (quad == 0) { s_m[warp][r] = m_run[i]; s_l[warp][r] = l_run[i]; }
+            for (int m = 0; m < MT; ++m)
 #pragma unroll
-            for (int x = 0; x < D / 8; ++x)
-                *reinterpret_cast<float2*>(&s_acc[warp][r][x * 8 + quad * 2]) = make_float2(oacc[x][2 * i], oacc[x][2 * i + 1]);
-        }
-    }
-    __syncthreads();
-    const size_t unit = (size_t)row * p.row_tiles + rt;
-    float* part = p.partials + (unit * p.splits + split) * kRows * PSTRIDE;
-    for (int i = tid; i < n_rows * D; i += kRowThreads) {
-        const int r = i / D, d = i % D;
-        float a = 0.f, l = 0.f, m = -INFINITY;
-        if (r < live) {
+                for (int i = 0; i < 2; ++i) {
+                    float l = l_run[m][i];
+                    l += __shfl_xor_sync(FULL, l, 1);
+                    l += __shfl_xor_sync(FULL, l, 2);
+                    const int r = 16 * m + qr + 8 * i;
+                    if (r < live) {
+                        if (quad == 0) { s_m[warp][r] = m_run[m][i]; s_l[warp][r] = l; }
 #pragma unroll
-            for (int w = 0; w < kRowWarps; ++w) m = fmaxf(m, s_m[w][r]);
-            const float mu = m == -INFINITY ? 0.f : m;
+                        for (int x = 0; x < D / 8; ++x)
+                            *reinterpret_cast<float2*>(&s_acc[warp][r][x * 8 + quad * 2]) = make_float2(oacc[m][x][2 * i], oacc[m][x][2 * i + 1]);
+                    }
+                }
+            __syncthreads();
+            const bool alone = first_block == last_block;
+            // a block has at most two units that it shares: the one that began before its stretch, and the one that ends behind it
+            float* part = p.partials + ((size_t)blockIdx.x * 2 + (unit_begin < begin ? 0 : 1)) * R * PSTRIDE;
+            for (int i = tid; i < n_rows * (D / 4); i += kRowThreads) {
+                const int r = i / (D / 4), d = i % (D / 4) * 4;
+                float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
+                float l = 0.f, mx = -INFINITY;
+                if (r < live) {
 #pragma unroll
-            for (int w = 0; w < kRowWarps; ++w) {
-                const float f = exp2_approx(s_m[w][r] - mu);
-                a = fmaf(s_acc[w][r][d], f, a);
-                l = fmaf(s_l[w][r], f, l);
+                    for (int w = 0; w < kRowWarps; ++w) mx = fmaxf(mx, s_m[w][r]);
+                    const float mu = mx == -INFINITY ? 0.f : mx;
+#pragma unroll
+                    for (int w = 0; w < kRowWarps; ++w) {
+                        const float f = exp2_approx(s_m[w][r] - mu);
+                        add_scaled(a, *reinterpret_cast<const float4*>(&s_acc[w][r][d]), f);
+                        l = fmaf(s_l[w][r], f, l);
+                    }
+                }
+                if (alone) {
+                    store_o(p, s, h, r0 + r, d, divided(a, l));
+                } else if (r < live) {
+                    *reinterpret_cast<float4*>(part + r * D + d) = a;
+                    if (d == 0) *reinterpret_cast<float2*>(part + R * D + 2 * r) = make_float2(mx, l);
+                }
             }
+            __syncthreads();                                                        // the ring may be filled again
+            if (!alone) {
+                if (tid == 0) {
+                    __threadfence();
+                    sh.last = atomicAdd(&p.tickets[first_block], 1) == last_block - first_block;
+                    if (sh.last) p.tickets[first_block] = 0;
+                    __threadfence();
+                }
+                __syncthreads();
+                if (sh.last) join_parts<D, R>(p, s, h, r0, n_rows, live, unit_begin, chunk, first_block, last_block, &s_m[0][0]);
+                __syncthreads();                                                    // sh.last and the scratch have been read
+            }
+            line = min(end, unit_end);
+            unit_begin = unit_end;
         }
-        if (nsplit == 1) {
-            store_o(p, s, h, r0 + r, d, l != 0.f ? a / l : 0.f);
-        } else {
-            part[r * PSTRIDE + d] = a;
-            if (d == 0) { part[r * PSTRIDE + D] = m; part[r * PSTRIDE + D + 1] = l; }
-        }
-    }
-    if (nsplit == 1) return;
-    __syncthreads();
-    if (tid == 0) {
-        __threadfence();
-        s_last = atomicAdd(&p.tickets[unit], 1) == nsplit - 1;
-        if (s_last) p.tickets[unit] = 0;
-        __threadfence();
-    }
-    __syncthreads();
-    if (!s_last) return;
-    const float* parts = p.partials + unit * p.splits * kRows * PSTRIDE;
-    for (int i = tid; i < n_rows * D; i += kRowThreads) {
-        const int r = i / D, d = i % D;
-        float m = -INFINITY, a = 0.f, l = 0.f;
-        for (int x = 0; x < nsplit; ++x) m = fmaxf(m, __ldcg(parts + (x * kRows + r) * PSTRIDE + D));
-        const float mu = m == -INFINITY ? 0.f : m;
-        for (int x = 0; x < nsplit; ++x) {
-            const float* px = parts + (x * kRows + r) * PSTRIDE;
-            const float f = exp2_approx(__ldcg(px + D) - mu);
-            a = fmaf(__ldcg(px + d), f, a);
-            l = fmaf(__ldcg(px + D + 1), f, l);
-        }
-        store_o(p, s, h, r0 + r, d, l != 0.f ? a / l : 0.f);
+        row_begin = unit_begin;
     }
 }
 
 // ---- host side ------------------------------------------------------------------------------------
-struct AttnPlan { bool tiles; int row_tiles, split_pages, splits; size_t counter, partials, bytes; };
+struct AttnPlan { bool tiles; long long line; int mt, row_tiles, split_pages, splits; size_t counter, partials, bytes; };
 // max_pages: bound of the pages of a row that the host knows; M: entries of a row
 static AttnPlan attn_plan(int S, int H, int G, int N, int D, int P, int max_pages, int M) {
-    AttnPlan a;
-#ifndef NATS_ROWS_MAX
-#define NATS_ROWS_MAX kRows
-#endif
-#ifndef NATS_SPLIT
-#define NATS_SPLIT 1024
-#endif
-    a.tiles = (long long)N * G > NATS_ROWS_MAX && G <= kTile;
+    AttnPlan a = {};
+    // Query rows up to which paged_rows_kernel is faster.  us, rows / tiles: head_dim 64 32 rows (16 sequences of 4 heads, 2200 keys each) 24.6 / 29.1,
+    // (16 of 8, 4700 keys) 41.7 / 48.7, 64 rows (one of 4, 1300 keys) 19.5 / 16.2; head_dim 128 32 rows (8 of 8, 2600 keys) 47.2 / 33.7.
+    a.tiles = (long long)N * G > (D == 64 ? 2 : 1) * kRows && G <= kTile;
     a.counter = kMaxTickets * 4;
-    a.partials = a.counter + 256;
+    a.partials = 4096;
+    static_assert(kMaxTickets * 4 + 4 <= 4096, "the front of the workspace holds the tickets and the counter");
     if (a.tiles) {
         a.row_tiles = cdiv(N, tile_tokens(G));
         a.split_pages = 0;
@@ -296,29 +436,42 @@ static AttnPlan attn_plan(int S, int H, int G, int N, int D, int P, int max_page
         a.splits = max(wanted, cdiv(M, kTileMaxPages));
         a.bytes = a.partials + paged_tile_partial_floats(S, H * G, N, D, a.splits) * 4;
     } else {
-        a.row_tiles = cdiv(N * G, kRows);
-        const long long units = (long long)S * H * a.row_tiles;
-        const int pages_per_k = max(1, NATS_SPLIT / P);
-        a.split_pages = units >= 4096 ? max(pages_per_k, max_pages) : pages_per_k;
-        static_assert(4096 <= kMaxTickets, "splits are joined");
-        a.splits = max(1, cdiv(max_pages, a.split_pages));
-        a.bytes = a.partials + (a.splits == 1 ? 0 : (size_t)units * a.splits * kRows * (D + 2) * 4);
+        a.mt = D == 64 && (long long)N * G > kRows ? 2 : 1;
+        a.row_tiles = (int)(((long long)N * G + 16 * a.mt - 1) / (16 * a.mt));
+        a.split_pages = max(1, kMinStretch / P);
+        a.splits = 1;
+        a.line = (long long)S * H * a.row_tiles * max(M, 1);
+        a.bytes = a.partials + (size_t)kMaxTickets * 2 * 16 * a.mt * (D + 2) * 4;
     }
     return a;
 }
 
-template <int D>
-static int launch_rows(const PagedAttnParams& p, dim3 grid, cudaStream_t st) {
+template <int D, int MT>
+static int launch_rows(const PagedAttnParams& p, cudaStream_t st) {
     constexpr int smem = kRowWarps * kRowStages * 2 * kRowTile * D * 2;
-    static bool ready[64] = {};
-    int dev = 0;
+    static int places[64] = {};                    // blocks that fit on the device at once
+    int dev = 0, n = 0;
     NATS_CHECK_CUDA(cudaGetDevice(&dev));
-    if (dev >= 64 || !ready[dev]) {
-        NATS_CHECK_CUDA(cudaFuncSetAttribute(paged_rows_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
-        if (dev < 64) ready[dev] = true;
+    if (dev < 64) n = places[dev];
+    if (n == 0) {
+        int sms = 0, per_sm = 0;
+        NATS_CHECK_CUDA(cudaFuncSetAttribute(paged_rows_kernel<D, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+        NATS_CHECK_CUDA(cudaDeviceGetAttribute(&sms, cudaDevAttrMultiProcessorCount, dev));
+        NATS_CHECK_CUDA(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, paged_rows_kernel<D, MT>, kRowThreads, smem));
+        n = min(sms * max(per_sm, 1), kMaxTickets);
+        if (dev < 64) places[dev] = n;
     }
-    paged_rows_kernel<D><<<grid, kRowThreads, smem, st>>>(p);
-    NATS_CHECK_CUDA(cudaGetLastError());
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(n);
+    cfg.blockDim = dim3(kRowThreads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    NATS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_rows_kernel<D, MT>, p));
     return NATS_OK;
 }
 
@@ -350,7 +503,7 @@ NATS_EXPORT int nats_b200_paged_attention(const NatsPagedKV* kv, const void* d_q
     const int G = n_heads / p.kv.H;
     const AttnPlan a = attn_plan(p.kv.S, p.kv.H, G, N, p.kv.D, p.kv.P, max_pages, p.kv.M);
     if (workspace_bytes < a.bytes) return fail(NATS_ERR_WORKSPACE, "paged attention workspace: %zu bytes given, %zu needed", workspace_bytes, a.bytes);
-    NATS_CHECK_ARG(a.tiles || a.row_tiles <= 65535, "%d new tokens of %d heads per kv-head are too many", N, G);
+    NATS_CHECK_ARG(a.line < (1ll << 31), "%d new tokens of %d heads per kv-head are too many", N, G);
     p.q = (const __nv_bfloat16*)d_q; p.q_slot = q_slot_stride; p.q_head = q_head_stride; p.q_token = q_token_stride;
     p.o = d_o; p.o_slot = o_slot_stride; p.o_head = o_head_stride; p.o_token = o_token_stride; p.o_f32 = o_f32;
     p.n_new = d_n_new; p.N = N; p.G = G; p.splits = a.splits; p.split_pages = a.split_pages; p.row_tiles = a.row_tiles;
@@ -360,6 +513,6 @@ NATS_EXPORT int nats_b200_paged_attention(const NatsPagedKV* kv, const void* d_q
     p.partials = (float*)((uint8_t*)d_workspace + a.partials);
     p.status = d_status;
     if (a.tiles) return launch_paged_tiles(p, (cudaStream_t)stream);
-    const dim3 grid(a.splits, a.row_tiles, p.kv.S * p.kv.H);
-    return p.kv.D == 64 ? launch_rows<64>(p, grid, (cudaStream_t)stream) : launch_rows<128>(p, grid, (cudaStream_t)stream);
+    if (p.kv.D == 64) return a.mt == 1 ? launch_rows<64, 1>(p, (cudaStream_t)stream) : launch_rows<64, 2>(p, (cudaStream_t)stream);
+    return launch_rows<128, 1>(p, (cudaStream_t)stream);
 }

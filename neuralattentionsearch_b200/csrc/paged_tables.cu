@@ -134,12 +134,6 @@ __device__ __forceinline__ void take_lowest(const PagedKv& kv, int total, int (&
     }
 }
 
-// A kernel that follows another one of this file in a stream is launched while that one ends, and looks at memory only behind this wait.
-__device__ __forceinline__ void wait_for_launch_before() {
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-
 __device__ __forceinline__ void give_back(const PagedKv& kv, int page) {
     if ((unsigned)page < (unsigned)kv.num_pages && atomicSub(&kv.refs[page], 1) == 1) atomicOr(&kv.free_bits[page >> 5], 1u << (page & 31));
 }

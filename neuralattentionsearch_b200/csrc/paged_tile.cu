@@ -106,6 +106,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     volatile int* abort_flag = &sm.abort_flag;
 
+    wait_for_launch_before();
     if (tid == 0) {
         int bad = *reinterpret_cast<volatile int32_t*>(p.status) != 0;
         if ((smem_u32(smem_raw) & 1023u) != 0u) {
@@ -159,9 +160,11 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             const int slot = ic & 1, use = ic >> 1;
             if (use > 0) ok = util_wait<kRelaxNs>(smem_u32(&sm.bar_list_empty[slot]), (use - 1) & 1, abort_flag, p.status, kPtErr + kErrList);
             if (!ok) break;
-            int w = 0;
-            if (lane == 0) w = atomicAdd(p.counter, 1);
-            w = __shfl_sync(0xffffffffu, w, 0);
+            int w = blockIdx.x;                          // the first item is the CTA's own, others come from the counter
+            if (ic > 0) {
+                if (total > (int)gridDim.x && lane == 0) w = atomicAdd(p.counter, 1);
+                w = (int)gridDim.x + __shfl_sync(0xffffffffu, w, 0);
+            }
             const bool have = w < total;
             PtHeader hd;
             hd.valid = have;
@@ -582,26 +585,42 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     }
 }
 
-// Joins the splits of a query row: a warp per row, D / 32 columns per lane
+// Joins the splits of a query row: a warp per row, D / 32 columns per lane.  The splits' maxima and sums are read by as many lanes, their columns
+// eight splits at a time.
 template <int D>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p) {
     constexpr int W = D / 32;
     const size_t rows = (size_t)p.kv.S * p.kv.H * p.G * p.N, lin = (size_t)blockIdx.x * 8 + threadIdx.x / 32;
+    wait_for_launch_before();
     if (lin >= rows) return;
     const int lane = threadIdx.x & 31;
-    const float* ml = p.partials + (size_t)p.splits * rows * D;
+    const float2* ml = reinterpret_cast<const float2*>(p.partials + (size_t)p.splits * rows * D);
     float m = -INFINITY;
-    for (int x = 0; x < p.splits; ++x) m = fmaxf(m, ml[(x * rows + lin) * 2]);
+    for (int x = lane; x < p.splits; x += 32) m = fmaxf(m, ml[x * rows + lin].x);
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
     const float mu = m == -INFINITY ? 0.f : m;
     float a[W] = {}, l = 0.f;
-    for (int x = 0; x < p.splits; ++x) {
-        const float2 v = *reinterpret_cast<const float2*>(ml + (x * rows + lin) * 2);
-        if (v.y == 0.f) continue;                        // nothing visible in this split: no O was written
-        const float f = ex2(v.x - mu);
-        l = fmaf(v.y, f, l);
-        const float* o = p.partials + (x * rows + lin) * D + lane * W;
+    for (int x0 = 0; x0 < p.splits; x0 += 8) {
+        float2 v[8];
+        float o[8][W];
 #pragma unroll
-        for (int i = 0; i < W; ++i) a[i] = fmaf(o[i], f, a[i]);
+        for (int x = 0; x < 8; ++x) {
+            v[x] = x0 + x < p.splits ? ml[(x0 + x) * rows + lin] : make_float2(0.f, 0.f);
+            if (x0 + x < p.splits) {
+                const float* from = p.partials + ((x0 + x) * rows + lin) * D + lane * W;
+#pragma unroll
+                for (int i = 0; i < W; ++i) o[x][i] = from[i];
+            }
+        }
+#pragma unroll
+        for (int x = 0; x < 8; ++x) {
+            if (v[x].y == 0.f) continue;                 // nothing visible in this split: no O was written
+            const float f = ex2(v[x].x - mu);
+            l = fmaf(v[x].y, f, l);
+#pragma unroll
+            for (int i = 0; i < W; ++i) a[i] = fmaf(o[x][i], f, a[i]);
+        }
     }
     const float inv = l != 0.f ? 1.f / l : 0.f;
     const int t = (int)(lin % p.N);
@@ -657,13 +676,24 @@ static int launch_tiles(const PagedAttnParams& p, cudaStream_t st) {
         if (dev < 64) sms[dev] = n_sm;
     }
     const long long items = (long long)p.kv.S * p.kv.H * p.splits * ((p.row_tiles + 1) / 2);
-    NATS_CHECK_CUDA(cudaMemsetAsync(p.counter, 0, 4, st));
-    paged_tile_kernel<D><<<(unsigned)min(items, (long long)n_sm), kPtThreads, sizeof(PtSmem<D>), st>>>(map_q, map_k, map_v, p);
-    NATS_CHECK_CUDA(cudaGetLastError());
+    if (items > n_sm) NATS_CHECK_CUDA(cudaMemsetAsync(p.counter, 0, 4, st));
+    cudaLaunchAttribute attr = {};
+    attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr.val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)min(items, (long long)n_sm));
+    cfg.blockDim = dim3(kPtThreads);
+    cfg.dynamicSmemBytes = sizeof(PtSmem<D>);
+    cfg.stream = st;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    NATS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_tile_kernel<D>, map_q, map_k, map_v, p));
     if (p.splits > 1) {
         const size_t rows = (size_t)p.kv.S * p.kv.H * p.G * p.N;
-        paged_join_kernel<D><<<(unsigned)((rows + 7) / 8), 256, 0, st>>>(p);
-        NATS_CHECK_CUDA(cudaGetLastError());
+        cfg.gridDim = dim3((unsigned)((rows + 7) / 8));
+        cfg.blockDim = dim3(256);
+        cfg.dynamicSmemBytes = 0;
+        NATS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<D>, p));
     }
     return NATS_OK;
 }

@@ -696,6 +696,7 @@ class PagedKV:
 
 
 _paged_bytes: dict[tuple, int] = {}
+PAGED_HEADER = 4096                        # bytes at the front of a workspace that have to be zero before its first use
 
 
 def _paged_scratch(name: str, index: int, stream: int, *sizes: int) -> torch.Tensor:
@@ -706,11 +707,14 @@ def _paged_scratch(name: str, index: int, stream: int, *sizes: int) -> torch.Ten
     if nbytes is None:
         nbytes = _paged_bytes[key] = getattr(_lib.lib(), f'nats_b200_paged_{name}_workspace_bytes')(*sizes)
     if torch.cuda.is_current_stream_capturing():
-        return torch.zeros(nbytes, dtype=torch.uint8, device=index)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=index)
+        ws[:PAGED_HEADER].zero_()
+        return ws
     key = (name, index, stream)
     ws = _workspaces.get(key)
     if ws is None or ws.numel() < nbytes:
-        ws = _workspaces[key] = torch.zeros(nbytes, dtype=torch.uint8, device=index)
+        ws = _workspaces[key] = torch.empty(nbytes, dtype=torch.uint8, device=index)
+        ws[:PAGED_HEADER].zero_()
     return ws
 
 
