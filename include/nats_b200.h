@@ -374,6 +374,10 @@ int nats_b200_paged_append(const NatsPagedKV* kv, const void* d_k, const void* d
                            int f32, const uint8_t* d_roles, int n_roles, const int32_t* d_n_new, int N, int SW, int skip_hidden,
                            void* d_workspace, size_t workspace_bytes, int32_t* d_status, void* stream);
 
+/* d_counts int32 [slots, n_kv_heads]: pages that nats_b200_paged_append with skip_hidden would take for a row.  Changes nothing. */
+int nats_b200_paged_append_count(const NatsPagedKV* kv, const uint8_t* d_roles, int n_roles, const int32_t* d_n_new, int N, int SW,
+                                 int32_t* d_counts, void* stream);
+
 /* Attention of the last d_n_new[slot] (NULL: N) tokens of every slot, whose K and V are in the pages.  q bf16 and o (bf16, or fp32 with
  * o_f32 != 0) are [slots, n_heads, N, head_dim] with the strides given, the last axis dense.  Row i of a slot is the token at position
  * length - n_new + i; rows behind the slot's new tokens, and rows that see no key, are written as zero.  max_pages: a bound of d_n_pages (work is

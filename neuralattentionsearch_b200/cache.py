@@ -24,6 +24,7 @@ from typing import Any
 import torch
 
 from . import functional as F_
+from .paged import KVPagePool, NAtSPagedLayerCache
 
 
 def get_pad_size(x_len: int, chunk_size: int) -> int:
@@ -432,15 +433,41 @@ class NAtSCache:
     exactly; the reference defers placement by up to ``update_chunk_size = 16`` steps (:196-223, 300-310), during which
     tokens stay visible past their rule, and agrees with this cache on the step after each of its batched updates."""
 
-    def __init__(self, sliding_window_size: int, chunk_size: int = 1):
-        self.cache_model: list[NAtSChunkLayerCache] = []
+    def __init__(self, sliding_window_size: int, chunk_size: int = 1, pages: KVPagePool | None = None):
+        """``pages``: keep every layer in pages of this pool (of ``chunk_size`` tokens each) instead of a buffer of its own."""
+        if pages is not None and pages.page_size != chunk_size:
+            raise ValueError(f'a cache in pages has one chunk per page: chunk size {chunk_size}, page size {pages.page_size}')
+        self.pages = pages
+        self.cache_model: list[NAtSChunkLayerCache | NAtSPagedLayerCache] = []
         self.sliding_window_size = sliding_window_size
         self.chunk_size = chunk_size
         self.cached_x: list[torch.Tensor | None] = []
 
     def reset_cache(self):
+        if self.pages is not None:
+            for layer in self.cache_model:
+                layer.reset_cache()
         self.cache_model = []
         self.cached_x = []
+
+    # what beam search and several replies to one prompt ask of the object passed as ``past_key_values``
+    def reorder_cache(self, beam_idx: torch.Tensor):
+        """Sequence b of every layer becomes a copy of what sequence ``beam_idx[b]`` was.  Only with ``pages``."""
+        self._need_pages()
+        for layer in self.cache_model:
+            layer.reorder(beam_idx)
+        self.cached_x = [None if x is None else x.index_select(0, beam_idx.to(x.device)) for x in self.cached_x]
+
+    def batch_repeat_interleave(self, repeats: int):
+        """Every sequence ``repeats`` times, one after the other.  Only with ``pages``."""
+        self._need_pages()
+        for layer in self.cache_model:
+            layer.repeat_interleave(repeats)
+        self.cached_x = [None if x is None else x.repeat_interleave(repeats, 0) for x in self.cached_x]
+
+    def _need_pages(self):
+        if self.pages is None:
+            raise NotImplementedError('sequences of a cache are moved and repeated in pages only: NAtSCache(..., pages=KVPagePool(...))')
 
     def get_seq_length(self, layer_idx: int = 0) -> int:
         if len(self.cache_model) <= layer_idx:
@@ -524,6 +551,9 @@ class NAtSCache:
                cache_kwargs: dict[str, Any] | None = None):
         while len(self.cache_model) <= layer_idx:
             bsz, n_kv_heads = key_states.shape[:2]
+            if self.pages is not None:
+                self.cache_model.append(NAtSPagedLayerCache(bsz, n_kv_heads, self.sliding_window_size, self.pages, layer_id=len(self.cache_model)))
+                continue
             self.cache_model.append(NAtSChunkLayerCache(bsz, n_kv_heads, self.sliding_window_size,
                                                         layer_id=len(self.cache_model), chunk_size=self.chunk_size,
                                                         device=key_states.device))

@@ -561,6 +561,18 @@ NATS_EXPORT int nats_b200_paged_append(const NatsPagedKV* kv, const void* d_k, c
     return NATS_OK;
 }
 
+NATS_EXPORT int nats_b200_paged_append_count(const NatsPagedKV* kv, const uint8_t* d_roles, int n_roles, const int32_t* d_n_new, int N, int SW,
+                                             int32_t* d_counts, void* stream) {
+    AppendParams p = {};
+    if (const int e = paged_kv(kv, p.kv)) return e;
+    NATS_CHECK_ARG(d_counts && (d_roles || n_roles == 0), "null pointer");
+    NATS_CHECK_ARG(N > 0 && N <= (1 << 24) && n_roles >= 0, "bad sizes N=%d n_roles=%d", N, n_roles);
+    NATS_CHECK_ARG(SW > 0 && SW % p.kv.P == 0, "sliding window %d must be a positive multiple of the page size %d", SW, p.kv.P);
+    p.roles = d_roles; p.n_roles = n_roles; p.n_new = d_n_new; p.N = N; p.SW = SW; p.counts = d_counts;
+    NATS_CHECK_CUDA(launch_behind(paged_count_kernel, (unsigned)(p.kv.S * p.kv.H), 0, (cudaStream_t)stream, p));
+    return NATS_OK;
+}
+
 NATS_EXPORT int nats_b200_paged_evict(const NatsPagedKV* d, void* stream) {
     PagedKv kv;
     if (const int e = paged_kv(d, kv)) return e;

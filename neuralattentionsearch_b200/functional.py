@@ -657,7 +657,8 @@ class PagedKV:
     ``pages_k`` / ``pages_v`` bf16 [n,P,D]; ``refs`` int32 [n]: rows that hold a page; ``free_bits`` int32 [ceil(n/32)]: bit p % 32 of word
     p // 32 is set where page p is free; ``entries`` int32 [S,Hkv,M,4]: (page, position of its first token, last query position that
     may see it, 0), the first ``n_pages`` int32 [S,Hkv] of a row in use, in the order of positions; ``length`` int32 [S]: tokens so far.
-    All contiguous.  ``paged_append``, ``paged_attention``, ``paged_evict`` and ``paged_reorder`` work on it; nothing is copied."""
+    All contiguous.  ``scratch``: None, or a dict in which the calls on this cache keep their workspaces; its owner then sees to it that no two calls
+    run at the same time, recorded ones among them.  ``paged_append``, ``paged_attention``, ``paged_evict`` and ``paged_reorder`` work on it; nothing is copied."""
 
     def __init__(self, pages_k: torch.Tensor, pages_v: torch.Tensor, refs: torch.Tensor, free_bits: torch.Tensor, entries: torch.Tensor,
                  n_pages: torch.Tensor, length: torch.Tensor):
@@ -682,6 +683,7 @@ class PagedKV:
             raise NotImplementedError(f'head_dim {D}: the paged cache is built for {PAGED_HEAD_DIMS}')
         self.pages_k, self.pages_v, self.refs, self.free_bits, self.entries, self.n_pages, self.length = tensors
         self.num_pages, self.page_size, self.head_dim, self.slots, self.n_kv_heads, self.max_entries = n, P, D, S, H, M
+        self.scratch: dict | None = None
         self._c = _lib.NatsPagedKV(pages_k.data_ptr(), pages_v.data_ptr(), refs.data_ptr(), free_bits.data_ptr(), entries.data_ptr(),
                                    n_pages.data_ptr(), length.data_ptr(), n, P, D, S, H, M)
 
@@ -699,22 +701,22 @@ _paged_bytes: dict[tuple, int] = {}
 PAGED_HEADER = 4096                        # bytes at the front of a workspace that have to be zero before its first use
 
 
-def _paged_scratch(name: str, index: int, stream: int, *sizes: int) -> torch.Tensor:
-    """Zeroed scratch for the entry point ``nats_b200_paged_<name>``, one per stream.  While a graph is recorded it is the graph's own, so that two
-    recorded graphs never share it."""
+def _paged_scratch(kv: PagedKV, name: str, stream: int, *sizes: int) -> torch.Tensor:
+    """Scratch for the entry point ``nats_b200_paged_<name>``: the cache's own where it has some, else one per stream.  While a graph is
+    recorded scratch that is not the cache's own is the graph's, so that two recorded graphs never share it."""
     key = (name, *sizes)
     nbytes = _paged_bytes.get(key)
     if nbytes is None:
         nbytes = _paged_bytes[key] = getattr(_lib.lib(), f'nats_b200_paged_{name}_workspace_bytes')(*sizes)
-    if torch.cuda.is_current_stream_capturing():
-        ws = torch.empty(nbytes, dtype=torch.uint8, device=index)
+    own = kv.scratch
+    kept, key = (_workspaces, ('paged', name, kv.index, stream)) if own is None else (own, name)
+    ws = kept.get(key)
+    recording = torch.cuda.is_current_stream_capturing()
+    if ws is None or ws.numel() < nbytes or (recording and own is None):
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=kv.device)
         ws[:PAGED_HEADER].zero_()
-        return ws
-    key = (name, index, stream)
-    ws = _workspaces.get(key)
-    if ws is None or ws.numel() < nbytes:
-        ws = _workspaces[key] = torch.empty(nbytes, dtype=torch.uint8, device=index)
-        ws[:PAGED_HEADER].zero_()
+        if not recording:
+            kept[key] = ws
     return ws
 
 
@@ -758,18 +760,33 @@ def paged_append(kv: PagedKV, k_new: torch.Tensor, v_new: torch.Tensor, roles: t
     S, H, N, D = shape = k_new.shape
     if S != kv.slots or H != kv.n_kv_heads or D != kv.head_dim or v_new.shape != shape:
         raise ValueError(f'k_new / v_new must be [{kv.slots},{kv.n_kv_heads},N,{kv.head_dim}], got {tuple(k_new.shape)} / {tuple(v_new.shape)}')
-    n_roles, roles_ptr = 0, None
-    if roles is not None:
-        if roles.dtype is not torch.uint8 or roles.dim() != 3 or roles.shape[:2] != shape[:2] or roles.get_device() != kv.index:
-            raise ValueError(f'roles must be uint8 [{S},{H},chunks] on {kv.device}')
-        roles = roles.contiguous()
-        n_roles, roles_ptr = roles.shape[2], roles.data_ptr()
+    roles = _check_roles(kv, roles)
     lens = _check_n_new(kv, n_new)
     if N > 0:
-        _on(kv.index, _paged_append, kv, k_new, v_new, n_roles, roles_ptr, lens, N, sliding_window, skip_hidden)
+        _on(kv.index, _paged_append, kv, k_new, v_new, roles, lens, N, sliding_window, skip_hidden)
 
 
-def _paged_append(kv, k, v, n_roles, roles_ptr, lens, N, sliding_window, skip_hidden):
+def paged_append_count(kv: PagedKV, N: int, roles: torch.Tensor | None, sliding_window: int, n_new: torch.Tensor | None = None) -> torch.Tensor:
+    """int32 [S,Hkv]: the pages that ``paged_append`` of ``N`` tokens with ``skip_hidden`` would take for a row."""
+    roles = _check_roles(kv, roles)
+    counts = torch.zeros(kv.slots, kv.n_kv_heads, dtype=torch.int32, device=kv.device)
+    if N > 0:
+        n_roles, roles_ptr = (0, None) if roles is None else (roles.shape[2], roles.data_ptr())
+        _on(kv.index, _lib.call, 'nats_b200_paged_append_count', kv._c, roles_ptr, n_roles, _check_n_new(kv, n_new), N, sliding_window, counts.data_ptr(),
+            torch._C._cuda_getCurrentRawStream(kv.index))
+    return counts
+
+
+def _check_roles(kv: PagedKV, roles: torch.Tensor | None) -> torch.Tensor | None:
+    if roles is None:
+        return None
+    if roles.dtype is not torch.uint8 or roles.dim() != 3 or roles.shape[0] != kv.slots or roles.shape[1] != kv.n_kv_heads or roles.get_device() != kv.index:
+        raise ValueError(f'roles must be uint8 [{kv.slots},{kv.n_kv_heads},chunks] on {kv.device}')
+    return roles.contiguous()
+
+
+def _paged_append(kv, k, v, roles, lens, N, sliding_window, skip_hidden):
+    n_roles, roles_ptr = (0, None) if roles is None else (roles.shape[2], roles.data_ptr())
     if k.dtype is not v.dtype or (k.dtype is not torch.bfloat16 and k.dtype is not torch.float32):
         k, v = k.to(torch.bfloat16), v.to(torch.bfloat16)
     if not _strided_ok(k):
@@ -777,7 +794,7 @@ def _paged_append(kv, k, v, n_roles, roles_ptr, lens, N, sliding_window, skip_hi
     if not _strided_ok(v):
         v = v.contiguous()
     stream = torch._C._cuda_getCurrentRawStream(kv.index)
-    ws = _paged_scratch('append', kv.index, stream, kv.slots, kv.n_kv_heads, N, kv.page_size)
+    ws = _paged_scratch(kv, 'append', stream, kv.slots, kv.n_kv_heads, N, kv.page_size)
     ka, kb, kc, _ = k.stride()
     va, vb, vc, _ = v.stride()
     _lib.call('nats_b200_paged_append', kv._c, k.data_ptr(), v.data_ptr(), ka, kb, kc, va, vb, vc, k.dtype is torch.float32, roles_ptr, n_roles,
@@ -785,12 +802,13 @@ def _paged_append(kv, k, v, n_roles, roles_ptr, lens, N, sliding_window, skip_hi
 
 
 def paged_attention(kv: PagedKV, q: torch.Tensor, sm_scale: float | None = None, n_new: torch.Tensor | None = None,
-                    max_pages: int | None = None, token_major: bool = False) -> torch.Tensor:
+                    max_pages: int | None = None, token_major: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of the newest tokens of every slot over its pages, which hold their K and V already.  q [S,Hq,N,D] (cast to bf16 if needed;
     any strides that keep rows dense and 16-byte aligned); row i of slot s is the token at position ``length[s] - n_new[s] + i``
     (``n_new`` int32 [S]; None: N everywhere).  A key is seen from its own position on up to the limit of its page.  Rows behind a slot's
     new tokens and rows that see nothing are zero.  ``max_pages``: a bound of ``n_pages`` the host knows (the work is split by it; the
-    result does not depend on its being right).  Returns o [S,Hq,N,D] in q's dtype; ``token_major``: a view of a [S,N,Hq,D] tensor."""
+    result does not depend on its being right).  Returns o [S,Hq,N,D] in q's dtype; ``token_major``: a view of a [S,N,Hq,D] tensor;
+    ``out``: written and returned, of q's shape and type (bf16 or fp32)."""
     kv._check(q)
     S, Hq, N, D = q.shape
     if S != kv.slots or D != kv.head_dim or Hq == 0 or Hq % kv.n_kv_heads:
@@ -800,20 +818,27 @@ def paged_attention(kv: PagedKV, q: torch.Tensor, sm_scale: float | None = None,
     if not scale > 0.0:
         raise ValueError('sm_scale must be positive')
     bound = kv.max_entries if max_pages is None else max(0, min(int(max_pages), kv.max_entries))
-    return _on(kv.index, _paged_attention, kv, q, scale, lens, bound, token_major)
+    if out is not None:
+        kv._check(out)
+        if out.shape != q.shape or out.dtype is not q.dtype or out.dtype not in (torch.bfloat16, torch.float32) or not _strided_ok(out) or 0 in out.stride():
+            raise ValueError('out must be bf16 or fp32, shaped and typed like q, with dense rows and 16-byte alignment')
+    return _on(kv.index, _paged_attention, kv, q, scale, lens, bound, token_major, out)
 
 
-def _paged_attention(kv, q, scale, lens, bound, token_major):
+def _paged_attention(kv, q, scale, lens, bound, token_major, o):
     S, Hq, N, D = q.shape
     f32 = q.dtype is torch.float32                       # fp32 callers: the kernel writes fp32 itself
     dtype = torch.float32 if f32 else torch.bfloat16
-    o = torch.empty((S, N, Hq, D), dtype=dtype, device=kv.device).transpose(1, 2) if token_major else torch.empty((S, Hq, N, D), dtype=dtype, device=kv.device)
+    if o is None:
+        o = torch.empty((S, N, Hq, D) if token_major else (S, Hq, N, D), dtype=dtype, device=kv.device)
+        if token_major:
+            o = o.transpose(1, 2)
     if N > 0:
         qb = q if q.dtype is torch.bfloat16 else q.to(torch.bfloat16)
         if not _strided_ok(qb) or 0 in qb.stride():
             qb = qb.contiguous()
         stream = torch._C._cuda_getCurrentRawStream(kv.index)
-        ws = _paged_scratch('attention', kv.index, stream, S, Hq, kv.n_kv_heads, N, D, kv.page_size, bound, kv.max_entries)
+        ws = _paged_scratch(kv, 'attention', stream, S, Hq, kv.n_kv_heads, N, D, kv.page_size, bound, kv.max_entries)
         qs, qh, qt, _ = qb.stride()
         os, oh, ot, _ = o.stride()
         _lib.call('nats_b200_paged_attention', kv._c, qb.data_ptr(), qs, qh, qt, o.data_ptr(), os, oh, ot, f32, lens, Hq, N, bound, scale,
@@ -842,5 +867,5 @@ def paged_reorder(kv: PagedKV, src: torch.Tensor) -> None:
 
 def _paged_reorder(kv, src):
     stream = torch._C._cuda_getCurrentRawStream(kv.index)
-    ws = _paged_scratch('reorder', kv.index, stream, kv.slots, kv.n_kv_heads, kv.max_entries)
+    ws = _paged_scratch(kv, 'reorder', stream, kv.slots, kv.n_kv_heads, kv.max_entries)
     _lib.call('nats_b200_paged_reorder', kv._c, src.data_ptr(), ws.data_ptr(), ws.numel(), _status_ptr(kv.index), stream)

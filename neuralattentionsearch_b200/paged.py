@@ -1,0 +1,224 @@
+"""The NAtS cache in pages: eviction gives pages back instead of moving rows, replies that are forked off a prompt share its pages.
+
+``NAtSChunkLayerCache`` keeps every (sequence, kv-head) in a buffer as long as the longest one and compacts it by copying.  Here K and V lie in
+pages of one chunk each, out of one ``KVPagePool`` for all layers, and a (sequence, kv-head) holds a row of entries: a chunk that no later query sees
+leaves the row.  ``NAtSPagedLayerCache`` has the protocol of ``NAtSChunkLayerCache`` (``update`` -> attention -> ``post_update``, decode steps
+with static launch parameters) and the same visibility rule, so that the attention layers, the Hugging Face patch and
+``GraphedGreedyDecoder`` run on it unchanged: ``NAtSCache(window, chunk_size, pages=KVPagePool(...))``.  What it adds is ``reorder`` and
+``repeat_interleave``: beams and several replies to one prompt.  The reference has no counterpart.
+
+There is no dense view of the cache: ``update`` returns the new K and V, and ``cache_k``, ``valid_tokens``, ``size_global_kv`` do not exist.
+"""
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from . import functional as F_
+
+
+class KVPagePool:
+    """Pages for the K and V of any number of layer caches on one device: ``num_pages`` pages of ``page_size`` tokens of one kv-head."""
+
+    def __init__(self, num_pages: int, page_size: int, head_dim: int, device: torch.device = torch.device('cuda')):
+        if page_size not in F_.PAGE_SIZES:
+            raise ValueError(f'page size {page_size}: {F_.PAGE_SIZES} are supported')
+        if head_dim not in F_.PAGED_HEAD_DIMS:
+            raise NotImplementedError(f'head_dim {head_dim}: the paged cache is built for {F_.PAGED_HEAD_DIMS}')
+        if num_pages < 1:
+            raise ValueError('a pool has at least one page')
+        self.num_pages, self.page_size, self.head_dim, self.device = num_pages, page_size, head_dim, torch.device(device)
+        self.pages_k = torch.empty(num_pages, page_size, head_dim, dtype=torch.bfloat16, device=device)
+        self.pages_v = torch.empty_like(self.pages_k)
+        self.refs = torch.zeros(num_pages, dtype=torch.int32, device=device)
+        self.free_bits = torch.full((-(-num_pages // 32),), -1, dtype=torch.int32, device=device)
+        if num_pages % 32:
+            self.free_bits[-1:].fill_((1 << num_pages % 32) - 1)
+        self._free_bound = num_pages                  # pages that are free at least; the exact number is on the device
+
+    def free_pages(self) -> int:
+        """Pages that nobody holds (waits for the device)."""
+        self._free_bound = int((self.refs == 0).sum().item())
+        return self._free_bound
+
+    def take(self, n: int) -> None:
+        """Accounts for at most ``n`` pages that the next kernels take; raises before anything is launched if there may be fewer."""
+        if n > self._free_bound and n > self.free_pages():
+            raise _lib.NatsB200Error(f'a paged cache may need {n} pages, {self._free_bound} of {self.num_pages} are free')
+        self._free_bound -= n
+
+
+class NAtSPagedLayerCache:
+    """One layer's cache in pages of ``pool``; chunks are pages.  All calls on a cache are ordered by the caller (one stream at a time)."""
+
+    def __init__(self, bsz: int, n_msks: int, sliding_window_size: int, pool: KVPagePool, layer_id: int = 0):
+        if sliding_window_size <= 0 or sliding_window_size % pool.page_size != 0:
+            raise ValueError(f'sliding window {sliding_window_size} must be a positive multiple of the page size {pool.page_size}')
+        self.layer_id, self.bsz, self.n_msks, self.pool = layer_id, bsz, n_msks, pool
+        self.chunk_size = pool.page_size
+        self.sliding_window_size = sliding_window_size
+        self.device = pool.device
+        self.kv = None
+        self._make_tables(bsz, sliding_window_size // pool.page_size + 16)
+        self._clear()
+
+    # ------------------------------------------------------------------ state
+    def _clear(self) -> None:
+        self._seen_tokens = 0
+        self.chunk_fill_size = 0
+        self._pending = None
+        self._roles = None
+        self._bound = self._synced = 0                # pages of the longest row at most; the last value read back
+        self._static_steps_left = 0
+
+    def _make_tables(self, bsz: int, max_entries: int) -> None:
+        """Tables of ``bsz`` slots with room for ``max_entries`` pages per row; what the old ones hold is kept in the first slots."""
+        p, old = self.pool, self.kv
+        entries = torch.zeros(bsz, self.n_msks, max_entries, 4, dtype=torch.int32, device=self.device)
+        n_pages = torch.zeros(bsz, self.n_msks, dtype=torch.int32, device=self.device)
+        length = torch.zeros(bsz, dtype=torch.int32, device=self.device)
+        if old is not None:
+            entries[:old.slots, :, :old.max_entries] = old.entries
+            n_pages[:old.slots] = old.n_pages
+            length[:old.slots] = old.length
+        self.kv = F_.PagedKV(p.pages_k, p.pages_v, p.refs, p.free_bits, entries, n_pages, length)
+        self.kv.scratch = {} if old is None else old.scratch
+        self.bsz = bsz
+
+    def _longest_row(self) -> int:
+        self._bound = self._synced = int(self.kv.n_pages.max().item())
+        F_.check_status(self.device)                  # the host waits for the device here anyway
+        return self._bound
+
+    def _room(self, chunks: int, pages: int | None = None) -> None:
+        """Makes sure that every row can take ``chunks`` more pages and that the pool has them (``pages`` in all, if not as many for every row)."""
+        self.pool.take(self.bsz * self.n_msks * chunks if pages is None else pages)
+        if self._bound + chunks > self.kv.max_entries and self._longest_row() + chunks > self.kv.max_entries:
+            self._make_tables(self.bsz, max(self._bound + chunks, self.kv.max_entries + self.kv.max_entries // 2))
+        self._bound += chunks
+
+    def get_seq_length(self) -> int:
+        return self._seen_tokens
+
+    def get_chunk_fill_size(self) -> int:
+        return self.chunk_fill_size
+
+    def kv_bytes(self) -> int:
+        """Bytes of K and V in the pages that this cache holds (shared pages once per row), as a decode step reads them."""
+        unfinished = self.chunk_fill_size * self.bsz * self.n_msks
+        whole = int(self.kv.n_pages.sum().item()) - (self.bsz * self.n_msks if self.chunk_fill_size else 0)
+        return (whole * self.chunk_size + unfinished) * self.pool.head_dim * 2 * 2
+
+    def reset_cache(self) -> None:
+        """Gives all pages back."""
+        F_.paged_reorder(self.kv, torch.full((self.bsz,), -1, dtype=torch.int32, device=self.device))
+        self._clear()
+
+    # ------------------------------------------------------------------ protocol
+    def update(self, key_states: torch.Tensor, value_states: torch.Tensor, token_states_info: torch.Tensor | None, fused: bool = False):
+        """Takes new K/V [B,Hkv,n,D] and returns them.  The first call of a sequence only keeps them: its attention reads them as they are, and
+        ``post_update`` stores the chunks that stay visible.  Later ones write them into pages, which ``prefill_attention`` and
+        ``decode_attention`` read."""
+        bsz, n_heads, x_len, head_dim = key_states.shape
+        if (bsz, n_heads, head_dim) != (self.bsz, self.n_msks, self.pool.head_dim):
+            raise ValueError(f'K/V must be [{self.bsz},{self.n_msks},n,{self.pool.head_dim}], got {tuple(key_states.shape)}')
+        fill = self.chunk_fill_size + x_len
+        if token_states_info is None:
+            assert fill < self.chunk_size, 'a new token_states_info must be given once the cached tokens fill a chunk'
+        self._roles = None
+        if fill >= self.chunk_size:                   # below, the only chunk stays unfinished and counts as global
+            roles = F_.roles_from_token_states_info(token_states_info)
+            chunks = -(-fill // self.chunk_size)
+            if roles.shape != (bsz, n_heads, chunks):
+                raise ValueError(f'token_states_info must describe {chunks} chunks')
+            self._roles = roles
+        if x_len == 0:
+            return key_states, value_states
+        if self._seen_tokens == 0:
+            self._pending = (key_states, value_states)
+        else:
+            self._append(key_states, value_states, skip_hidden=False)
+        self.chunk_fill_size = fill
+        return key_states, value_states
+
+    def _append(self, k: torch.Tensor, v: torch.Tensor, skip_hidden: bool) -> None:
+        fill = self._seen_tokens % self.chunk_size
+        if skip_hidden and k.shape[2] > self.chunk_size:          # how many chunks of a prompt stay depends on the roles: one read-back
+            counts = F_.paged_append_count(self.kv, k.shape[2], self._roles, self.sliding_window_size)
+            longest, pages = torch.stack((counts.max(), counts.sum())).tolist()
+            F_.check_status(self.device)              # the host waits for the device here anyway
+            self._room(longest, pages)
+            self._synced = self._bound
+        else:
+            self._room(-(-(fill + k.shape[2]) // self.chunk_size) - (fill > 0))
+        F_.paged_append(self.kv, k, v, self._roles, self.sliding_window_size, skip_hidden=skip_hidden)
+
+    def prefill_attention(self, xq: torch.Tensor, sm_scale: float | None = None) -> torch.Tensor:
+        """Attention of several new tokens over the cache, which holds them since ``update``: [B,Hq,n,D] -> [B,Hq,n,D], the outputs that one
+        call over the whole sequence would give."""
+        return F_.paged_attention(self.kv, xq, sm_scale, max_pages=self._bound, token_major=True)
+
+    def decode_attention(self, xq: torch.Tensor, sm_scale: float | None = None) -> torch.Tensor:
+        return F_.paged_attention(self.kv, xq, sm_scale, max_pages=self._bound)
+
+    def post_update(self, x_len: int) -> None:
+        if x_len == 0:
+            return
+        if self._pending is not None:
+            self._append(*self._pending, skip_hidden=True)
+            self._pending = None
+        elif self.chunk_fill_size >= self.chunk_size:
+            F_.paged_evict(self.kv)
+            if self._bound - self._synced >= 16:
+                self._longest_row()                   # the bound drifts up while chunks are dropped: refreshed now and then
+        self._seen_tokens += x_len
+        self.chunk_fill_size = self._seen_tokens % self.chunk_size
+
+    # ------------------------------------------------------------------ decode steps with static launch parameters
+    def prepare_static_decode(self, n_steps: int, n_heads: int, head_dim: int) -> None:
+        """Gets the cache ready for ``n_steps`` calls of ``decode_step_static`` that neither allocate nor read anything back."""
+        self._room((self.chunk_fill_size + n_steps) // self.chunk_size + 1)
+        kv, stream = self.kv, torch.cuda.current_stream(self.device).cuda_stream
+        F_._paged_scratch(kv, 'append', stream, kv.slots, kv.n_kv_heads, 1, kv.page_size)
+        F_._paged_scratch(kv, 'attention', stream, kv.slots, n_heads, kv.n_kv_heads, 1, head_dim, kv.page_size, self._bound, kv.max_entries)
+        self._static_steps_left = n_steps
+
+    def decode_step_static(self, xq: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, roles: torch.Tensor, out: torch.Tensor,
+                           sm_scale: float | None = None, recording: bool = False) -> torch.Tensor:
+        """One decode step -- append, attention, pages given back -- whose launch parameters do not change from step to step.  xq / out
+        [B,Hq,1,D], k_new / v_new [B,Hkv,1,D]; roles uint8 [B,Hkv] = role of the chunk this token completes (read on the device only
+        if it does).  While a graph is being recorded pass ``recording=True``; after replaying the step n times call ``note_static_steps(n)``."""
+        F_.paged_append(self.kv, k_new, v_new, roles.view(self.bsz, self.n_msks, 1), self.sliding_window_size)
+        F_.paged_attention(self.kv, xq, sm_scale, max_pages=self._bound, out=out)
+        F_.paged_evict(self.kv)
+        if not recording:
+            self.note_static_steps(1)
+        return out
+
+    def note_static_steps(self, n: int) -> None:
+        """Advances the host's view of the cache by ``n`` decode steps that ran on the device (recorded and replayed)."""
+        if n > self._static_steps_left:
+            raise RuntimeError('more static decode steps than prepare_static_decode() made room for')
+        self._static_steps_left -= n
+        self._seen_tokens += n
+        self.chunk_fill_size = self._seen_tokens % self.chunk_size
+
+    # ------------------------------------------------------------------ sequences
+    def reorder(self, src: torch.Tensor) -> None:
+        """Sequence b becomes a copy of what sequence ``src[b]`` was (int [B]); whole pages are shared, the unfinished one is copied where
+        several sequences go on from it."""
+        if src.shape != (self.bsz,):
+            raise ValueError(f'src must have shape [{self.bsz}]')
+        if self._pending is not None:
+            raise RuntimeError('post_update() has not been called for the first call yet')
+        if self.chunk_fill_size:
+            self.pool.take(self.bsz * self.n_msks)
+        F_.paged_reorder(self.kv, src.to(device=self.device, dtype=torch.int32).contiguous())
+
+    def repeat_interleave(self, repeats: int) -> None:
+        """Every sequence ``repeats`` times, one after the other: several replies to each prompt."""
+        if repeats < 1:
+            raise ValueError('repeats must be positive')
+        old = self.bsz
+        self._make_tables(old * repeats, self.kv.max_entries)
+        self.reorder(torch.arange(old, device=self.device).repeat_interleave(repeats))

@@ -1,0 +1,217 @@
+"""The NAtS cache in pages, as the attention layers and the Hugging Face models use it."""
+import numpy as np
+import pytest
+import torch
+
+from test_gpu_hf import tiny_llama
+from tests.paged_model import PagedModel
+
+pytestmark = pytest.mark.gpu
+DEV = 'cuda'
+
+
+def randn(g, *shape):
+    return torch.randn(*shape, generator=g, device=DEV).bfloat16()
+
+
+def onehot(roles):
+    return torch.nn.functional.one_hot(roles.long(), 3).to(torch.bfloat16)
+
+
+@pytest.mark.parametrize('calls', [[300, 1, 1, 1, 40, 7, 1, 130], [5, 1, 3, 1, 60], [64, 64, 1], [7] + [1] * 70])
+@pytest.mark.parametrize('D', [64, 128])
+def test_layer_cache_against_the_model_and_the_compacted_cache(calls, D):
+    from neuralattentionsearch_b200 import KVPagePool, NAtSChunkLayerCache, NAtSPagedLayerCache, check_status, prefill_attention
+    B, H, G, C, SW = 2, 2, 4, 32, 64
+    g = torch.Generator(device=DEV).manual_seed(len(calls) + D)
+    pool = KVPagePool(400, C, D)
+    lc = NAtSPagedLayerCache(B, H, SW, pool)
+    dense = NAtSChunkLayerCache(B, H, SW, chunk_size=C, device=torch.device(DEV))
+    model = PagedModel(B, H, C, D, 400, SW)
+    for i, n in enumerate(calls):
+        q, k, v = randn(g, B, H * G, n, D), randn(g, B, H, n, D), randn(g, B, H, n, D)
+        fill = lc.chunk_fill_size
+        roles = torch.randint(0, 3, (B, H, -(-(fill + n) // C)), generator=g, device=DEV).to(torch.uint8)
+        if i == 0:
+            roles[..., 0] = 0
+        if (fill + n) % C:
+            roles[..., -1] = 0
+        info = onehot(roles)
+        outs = []
+        for cache in (lc, dense):
+            keys, values = cache.update(k, v, info, fused=True)
+            if i == 0:
+                outs.append(prefill_attention(q, keys, values, roles, C, SW))
+            elif n == 1:
+                outs.append(cache.decode_attention(q))
+            else:
+                outs.append(cache.prefill_attention(q))
+            cache.post_update(n)
+        check_status()
+        model.append(k.double().cpu().numpy(), v.double().cpu().numpy(), roles.cpu().numpy(), [n] * B)
+        want, mag = model.attention(q.double().cpu().numpy(), [n] * B, D ** -0.5)
+        model.evict()
+        tol = (2.0 ** -8 + 2e-4) * mag + 2.0 ** -8 * np.abs(want)
+        for o in outs:                                            # both caches follow the same rule
+            assert (np.abs(o.double().cpu().numpy() - want) <= tol).all(), i
+        assert lc.get_seq_length() == dense.get_seq_length() and lc.chunk_fill_size == dense.chunk_fill_size
+        starts = [[[e[1] for e in model.rows[b][h]] for h in range(H)] for b in range(B)]
+        n_pages = lc.kv.n_pages.tolist()
+        assert [[lc.kv.entries[b, h, :n_pages[b][h], 1].tolist() for h in range(H)] for b in range(B)] == starts
+    used = sum(len(r) for rows in model.rows for r in rows)
+    assert pool.free_pages() == 400 - used
+    assert lc.kv_bytes() == sum(min(C, sum(calls) - e[1]) for rows in model.rows for r in rows for e in r) * D * 4
+    lc.reset_cache()
+    assert pool.free_pages() == 400 and lc.get_seq_length() == 0
+
+
+def test_replies_and_beams_of_a_layer_cache():
+    from neuralattentionsearch_b200 import KVPagePool, NAtSPagedLayerCache
+    H, G, C, SW, D = 2, 2, 16, 32, 64
+    g = torch.Generator(device=DEV).manual_seed(1)
+    pool = KVPagePool(200, C, D)
+    lc, model = NAtSPagedLayerCache(2, H, SW, pool), PagedModel(2, H, C, D, 200, SW)
+
+    def call(B, n, first=False):
+        k, v, q = randn(g, B, H, n, D), randn(g, B, H, n, D), randn(g, B, H * G, n, D)
+        fill = lc.chunk_fill_size
+        roles = torch.randint(0, 3, (B, H, -(-(fill + n) // C)), generator=g, device=DEV).to(torch.uint8)
+        lc.update(k, v, roles)
+        model.append(k.double().cpu().numpy(), v.double().cpu().numpy(), roles.cpu().numpy(), [n] * B)
+        if not first:
+            o = lc.decode_attention(q) if n == 1 else lc.prefill_attention(q)
+            want, mag = model.attention(q.double().cpu().numpy(), [n] * B, D ** -0.5)
+            assert (np.abs(o.double().cpu().numpy() - want) <= (2.0 ** -8 + 2e-4) * mag + 2.0 ** -8 * np.abs(want)).all()
+        lc.post_update(n)
+        model.evict()
+    call(2, 70, first=True)
+    lc.repeat_interleave(3)
+    model.S, model.rows, model.length = 6, model.rows + [[[] for _ in range(H)] for _ in range(4)], model.length + [0] * 4
+    model.reorder([0, 0, 0, 1, 1, 1])
+    for i in range(40):
+        call(6, 1)
+        if i % 5 == 2:
+            src = [0, 0, 2, 5, 3, 3] if i % 2 else [2, 1, 1, 4, 4, 4]
+            lc.reorder(torch.tensor(src, device=DEV))
+            model.reorder(src)
+    call(6, 33)
+    assert pool.free_pages() == model.refs.count(0)
+
+
+def test_tables_grow_and_the_pool_runs_out():
+    from neuralattentionsearch_b200 import KVPagePool, NAtSPagedLayerCache, _lib, check_status
+    g = torch.Generator(device=DEV).manual_seed(2)
+    pool = KVPagePool(70, 16, 64)
+    lc = NAtSPagedLayerCache(1, 1, 16, pool)
+    width = lc.kv.max_entries
+    k = randn(g, 1, 1, 16 * 20, 64)
+    for _ in range(3):
+        lc.update(k, k, torch.zeros(1, 1, 20, dtype=torch.uint8, device=DEV))
+        lc.post_update(320)
+    assert lc.kv.max_entries > width and lc.kv.n_pages.item() == 60
+    with pytest.raises(_lib.NatsB200Error, match='pages'):
+        lc.update(k, k, torch.zeros(1, 1, 20, dtype=torch.uint8, device=DEV))
+    assert lc.get_seq_length() == 960 and lc.chunk_fill_size == 0          # nothing has happened
+    lc.update(k[:, :, :17], k[:, :, :17], torch.zeros(1, 1, 2, dtype=torch.uint8, device=DEV))
+    o = lc.prefill_attention(k[:, :, :17])
+    lc.post_update(17)
+    check_status()
+    assert torch.isfinite(o).all() and lc.kv.length.item() == 977
+
+
+def _model():
+    from neuralattentionsearch_b200.hf import TransformerArgs, enable_llama_nats_chunk_eval
+    model = tiny_llama()
+    enable_llama_nats_chunk_eval(model, TransformerArgs(n_msks=2, chunk_size=16, local_seq_max_length=64))
+    torch.manual_seed(3)
+    for layer in model.model.layers:
+        layer.self_attn.proj_layer.weight.data.normal_(0, 0.5)
+    return model
+
+
+def _cache(pages):
+    from neuralattentionsearch_b200 import KVPagePool, NAtSCache
+    return NAtSCache(64, 16, pages=KVPagePool(2000, 16, 64) if pages else None)
+
+
+@torch.no_grad()
+def test_hugging_face_model_in_pages_is_the_same_model():
+    from neuralattentionsearch_b200 import check_status
+    model = _model()
+    ids = torch.randint(0, 512, (2, 420), device=DEV)
+    hs = []
+    for pages in (False, True):
+        cache, outs, pos = _cache(pages), [], 0
+        for n in [200, 150, 1, 1, 1, 30, 37]:
+            outs.append(model.model(input_ids=ids[:, pos:pos + n], past_key_values=cache, use_cache=True).last_hidden_state)
+            pos += n
+        hs.append(torch.cat(outs, 1).float())
+    check_status()
+    # the first call takes the same kernels; later ones differ by roundings of attention outputs, which two layers carry on
+    assert torch.equal(hs[0][:, :200], hs[1][:, :200])
+    assert (hs[0] - hs[1]).abs().mean() / hs[0].abs().mean() < 2e-2
+
+
+@torch.no_grad()
+def test_graphed_greedy_decoding_in_pages_equals_the_eager_loop():
+    from neuralattentionsearch_b200.hf import GraphedGreedyDecoder
+    model = _model()
+    ids = torch.randint(0, 512, (2, 150), device=DEV)
+    eager, graphed = _cache(True), _cache(True)
+    for cache in (eager, graphed):
+        out = model(input_ids=ids, past_key_values=cache, use_cache=True, logits_to_keep=1)
+    tok = out.logits[:, -1:].argmax(-1)
+    got = GraphedGreedyDecoder(model, graphed, 40).generate(tok, 40)
+    want = []
+    for _ in range(40):
+        out = model(input_ids=tok, past_key_values=eager, use_cache=True)
+        tok = out.logits[:, -1:].argmax(-1)
+        want.append(tok)
+    assert torch.equal(got, torch.cat(want, 1))
+    for a, b in zip(eager.cache_model, graphed.cache_model):
+        assert a.get_seq_length() == b.get_seq_length() == 190 and torch.equal(a.kv.n_pages, b.kv.n_pages)
+    more = model(input_ids=ids[:, :30], past_key_values=graphed, use_cache=True).logits      # the eager path goes on from there
+    same = model(input_ids=ids[:, :30], past_key_values=eager, use_cache=True).logits
+    assert torch.equal(more, same)
+
+
+@torch.no_grad()
+def test_replies_forked_off_a_prompt_equal_prompts_of_their_own():
+    model = _model()
+    prompt = torch.randint(0, 512, (1, 133), device=DEV)
+    reply = torch.randint(0, 512, (3, 60), device=DEV)
+    forked, apart = _cache(True), _cache(True)
+    model(input_ids=prompt, past_key_values=forked, use_cache=True, logits_to_keep=1)
+    forked.batch_repeat_interleave(3)
+    model(input_ids=prompt.expand(3, -1), past_key_values=apart, use_cache=True, logits_to_keep=1)
+    used = [c.pages.num_pages - c.pages.free_pages() for c in (forked, apart)]
+    assert used[0] < used[1] / 2
+    order = torch.tensor([2, 0, 2], device=DEV)
+    for pos in range(60):
+        a, b = (model(input_ids=reply[:, pos:pos + 1], past_key_values=c, use_cache=True).logits for c in (forked, apart))
+        assert torch.equal(a, b)
+        if pos == 30:
+            forked.reorder_cache(order)
+            apart.reorder_cache(order)
+            reply = reply[order]
+    forked.reset_cache()
+    assert forked.pages.free_pages() == forked.pages.num_pages and forked.get_seq_length() == 0
+
+
+@torch.no_grad()
+def test_attention_layer_on_a_cache_in_pages():
+    from neuralattentionsearch_b200 import KVPagePool, LlamaNAtSChunkAttentionLayer, NAtSCache
+    torch.manual_seed(0)
+    layer = LlamaNAtSChunkAttentionLayer(dim=512, n_heads=8, n_kv_heads=2, chunk_size=32, local_seq_max_length=64).to(DEV).to(torch.bfloat16).eval()
+    x = torch.randn(2, 300, 512, device=DEV).bfloat16()
+    ang = torch.arange(300, device=DEV)[:, None] * 10000.0 ** (-torch.arange(0, 64, 2, device=DEV) / 64)
+    ang = ang[None].repeat(1, 1, 2)
+    ys = []
+    for pages in (None, KVPagePool(300, 32, 64)):
+        cache, pos, out = NAtSCache(64, 32, pages=pages), 0, []
+        for n in (200, 1, 1, 60, 38):
+            out.append(layer(x[:, pos:pos + n], (ang[:, pos:pos + n].cos(), ang[:, pos:pos + n].sin()), None, start_pos=pos, cache=cache))
+            pos += n
+        ys.append(torch.cat(out, 1).float())
+    assert torch.equal(ys[0][:, :200], ys[1][:, :200])
+    assert (ys[0] - ys[1]).abs().mean() / ys[0].abs().mean() < 1e-2

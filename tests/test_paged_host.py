@@ -1,0 +1,101 @@
+"""The paged cache without a GPU: its model, its host-side checks, its C entry points' refusals."""
+import ctypes
+
+import numpy as np
+import pytest
+import torch
+
+from oracle import nats_oracle as orc
+from tests.paged_model import PagedModel
+
+
+@pytest.mark.parametrize('seed', range(4))
+def test_the_model_follows_the_one_call_rule(seed):
+    """Attention over the model's pages, call by call, is that of one call over the whole sequence under the oracle's mask."""
+    rng = np.random.default_rng(seed)
+    H, C, SW, D = 2, 8, 16, 4
+    calls = [40, 1, 1, 23, 8, 1, 50]
+    N = sum(calls)
+    roles = rng.choice(3, size=(1, H, -(-N // C)), p=(0.2, 0.3, 0.5)).astype(np.uint8)
+    roles[..., 0] = 0
+    if N % C:
+        roles[..., -1] = 0
+    q, k, v = (torch.from_numpy(rng.standard_normal((1, H, N, D)).astype(np.float32)) for _ in range(3))
+    want = orc.prefill_attention(q, k, v, roles, C, SW).numpy()
+    m, pos = PagedModel(1, H, C, D, 200, SW), 0
+    for n in calls:
+        sl = slice(pos, pos + n)
+        m.append(k[:, :, sl].double().numpy(), v[:, :, sl].double().numpy(), roles[:, :, pos // C:], [n])
+        got, _ = m.attention(q[:, :, sl].double().numpy(), [n], D ** -0.5)
+        assert np.abs(got - want[:, :, sl]).max() < 1e-5
+        m.evict()
+        pos += n
+    held = sum(len(r) for r in m.rows[0])
+    assert sum(m.refs) == held and held < H * N // C
+
+
+def test_host_side_refusals():
+    from neuralattentionsearch_b200 import KVPagePool, NAtSCache, NAtSPagedLayerCache, _lib
+    with pytest.raises(ValueError, match='page size'):
+        KVPagePool(10, 8, 64, device='cpu')
+    with pytest.raises(NotImplementedError, match='head_dim'):
+        KVPagePool(10, 16, 96, device='cpu')
+    with pytest.raises(ValueError):
+        KVPagePool(0, 16, 64, device='cpu')
+    pool = KVPagePool(45, 16, 64, device='cpu')
+    assert pool.free_pages() == 45 and pool.free_bits.tolist() == [-1, (1 << 13) - 1]
+    with pytest.raises(ValueError, match='one chunk per page'):
+        NAtSCache(64, 32, pages=pool)
+    with pytest.raises(ValueError, match='multiple'):
+        NAtSPagedLayerCache(1, 1, 40, pool)
+    with pytest.raises(_lib.NatsB200Error):
+        NAtSPagedLayerCache(1, 1, 64, pool)                     # no CPU path
+    with pytest.raises(_lib.NatsB200Error, match='46 pages'):
+        pool.take(46)
+    pool.take(45)
+    plain = NAtSCache(64, 16)
+    for call in (lambda: plain.reorder_cache(torch.zeros(1)), lambda: plain.batch_repeat_interleave(2)):
+        with pytest.raises(NotImplementedError, match='pages'):
+            call()
+
+
+def test_c_entry_points_refuse_bad_arguments():
+    from neuralattentionsearch_b200 import _lib, build
+    build.build()
+    lib = _lib.lib()
+    one = 256                                                   # never dereferenced: the checks fail first
+
+    def kv(**more):
+        a = dict(d_pages_k=one, d_pages_v=one, d_refs=one, d_free_bits=one, d_entries=one, d_n_pages=one, d_length=one, num_pages=10, page_size=16,
+                 head_dim=64, slots=2, n_kv_heads=2, max_entries=8)
+        a.update(more)
+        return _lib.NatsPagedKV(**a)
+    for more, rc, text in ((dict(d_refs=None), 1, b'null'), (dict(d_pages_k=264), 1, b'aligned'), (dict(num_pages=0), 1, b'pages'),
+                           (dict(num_pages=(1 << 24) + 1), 1, b'pages'), (dict(page_size=24), 1, b'page size'), (dict(head_dim=256), 2, b'head_dim'),
+                           (dict(slots=0), 1, b'table'), (dict(slots=5000), 1, b'table'), (dict(slots=4000, n_kv_heads=20), 1, b'rows'), (dict(max_entries=0), 1, b'table')):
+        for call in (lambda: lib.nats_b200_paged_evict(kv(**more), None), lambda: lib.nats_b200_paged_reorder(kv(**more), one, one, 1 << 30, one, None)):
+            assert call() == rc and text in lib.nats_b200_last_error(), more
+
+    def append(k=one, v=one, strides=(64,) * 6, f32=0, roles=one, n_roles=1, N=4, SW=16, ws=one, nbytes=1 << 30, status=one):
+        return lib.nats_b200_paged_append(kv(), k, v, *strides, f32, roles, n_roles, None, N, SW, 0, ws, nbytes, status, None)
+    for rc, text, call in ((1, b'null', lambda: append(k=None)), (1, b'null', lambda: append(roles=None)), (1, b'null', lambda: append(status=None)),
+                           (1, b'sizes', lambda: append(N=0)), (1, b'sizes', lambda: append(n_roles=-1)), (1, b'multiple', lambda: append(SW=24)),
+                           (1, b'multiple', lambda: append(SW=0)), (1, b'aligned', lambda: append(k=264)), (1, b'strides', lambda: append(strides=(64, 4, 64, 64, 64, 64))),
+                           (4, b'workspace', lambda: append(nbytes=100))):
+        assert call() == rc and text in lib.nats_b200_last_error()
+    assert lib.nats_b200_paged_append_count(kv(), None, 1, None, 4, 16, one, None) == 1
+
+    def attend(q=one, strides=(64,) * 6, heads=4, N=2, max_pages=8, scale=0.1, nbytes=1 << 40, status=one):
+        return lib.nats_b200_paged_attention(kv(), q, *strides[:3], one, *strides[3:], 0, None, heads, N, max_pages, scale, one, nbytes, status, None)
+    for rc, text, call in ((1, b'null', lambda: attend(q=None)), (1, b'query heads', lambda: attend(heads=3)), (1, b'sizes', lambda: attend(N=0)),
+                           (1, b'sizes', lambda: attend(max_pages=9)), (1, b'scale', lambda: attend(scale=0.0)), (1, b'scale', lambda: attend(scale=float('nan'))),
+                           (1, b'aligned', lambda: attend(q=264)), (1, b'strides', lambda: attend(strides=(64, 64, 64, 64, 64, 4))), (4, b'workspace', lambda: attend(nbytes=4096))):
+        assert call() == rc and text in lib.nats_b200_last_error()
+    assert lib.nats_b200_paged_reorder(kv(), None, one, 1 << 30, one, None) == 1
+    assert lib.nats_b200_paged_reorder(kv(), one, one, 64, one, None) == 4
+    for fn, args in ((lib.nats_b200_paged_append_workspace_bytes, (2, 2, 4, 16)), (lib.nats_b200_paged_reorder_workspace_bytes, (2, 2, 8)),
+                     (lib.nats_b200_paged_attention_workspace_bytes, (2, 4, 2, 4, 64, 16, 8, 8))):
+        assert fn(*args) > 0
+        assert fn(0, *args[1:]) == 0
+    assert lib.nats_b200_paged_attention_workspace_bytes(2, 3, 2, 4, 64, 16, 8, 8) == 0
+    assert ctypes.sizeof(_lib.NatsPagedKV) == 7 * 8 + 6 * 4
