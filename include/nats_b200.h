@@ -380,15 +380,14 @@ int nats_b200_paged_append_count(const NatsPagedKV* kv, const uint8_t* d_roles, 
 
 /* Attention of the last d_n_new[slot] (NULL: N) tokens of every slot, whose K and V are in the pages.  q bf16 and o (bf16, or fp32 with
  * o_f32 != 0) are [slots, n_heads, N, head_dim] with the strides given, the last axis dense.  Row i of a slot is the token at position
- * length - n_new + i; rows behind the slot's new tokens, and rows that see no key, are written as zero.  max_pages: a bound of d_n_pages (work is
- * split by it; where it is too low the result stays right).  A value that is not finite in a V row reaches the rows of the call that
- * share a 128-key tile with it from its own position on or not at all only where its page is hidden from all of them.
+ * length - n_new + i; rows behind the slot's new tokens, and rows that see no key, are written as zero.  What lies in pages
+ * behind a slot's last token, and in pages that no query of the call sees, is never used, whatever it holds; a V value of a visible token that is
+ * not finite reaches, besides the queries that see it, others of the same call.
  */
-size_t nats_b200_paged_attention_workspace_bytes(int slots, int n_heads, int n_kv_heads, int N, int head_dim, int page_size, int max_pages,
-                                                  int max_entries);
+size_t nats_b200_paged_attention_workspace_bytes(int slots, int n_heads, int n_kv_heads, int N, int head_dim, int page_size, int max_entries);
 int nats_b200_paged_attention(const NatsPagedKV* kv, const void* d_q, long long q_slot_stride, long long q_head_stride, long long q_token_stride,
                               void* d_o, long long o_slot_stride, long long o_head_stride, long long o_token_stride, int o_f32,
-                              const int32_t* d_n_new, int n_heads, int N, int max_pages, float sm_scale, void* d_workspace,
+                              const int32_t* d_n_new, int n_heads, int N, float sm_scale, void* d_workspace,
                               size_t workspace_bytes, int32_t* d_status, void* stream);
 
 /* Pages that the next query position (d_length) cannot see leave the rows; a page that loses its last holder is free again. */

@@ -59,8 +59,8 @@ SIGNATURES = {
     'nats_b200_paged_append_workspace_bytes': (_SZ, [_I, _I, _I, _I]),
     'nats_b200_paged_append': (_I, [_KV, _P, _P, _LL, _LL, _LL, _LL, _LL, _LL, _I, _P, _I, _P, _I, _I, _I, _P, _SZ, _P, _P]),
     'nats_b200_paged_append_count': (_I, [_KV, _P, _I, _P, _I, _I, _P, _P]),
-    'nats_b200_paged_attention_workspace_bytes': (_SZ, [_I, _I, _I, _I, _I, _I, _I, _I]),
-    'nats_b200_paged_attention': (_I, [_KV, _P, _LL, _LL, _LL, _P, _LL, _LL, _LL, _I, _P, _I, _I, _I, _F, _P, _SZ, _P, _P]),
+    'nats_b200_paged_attention_workspace_bytes': (_SZ, [_I, _I, _I, _I, _I, _I, _I]),
+    'nats_b200_paged_attention': (_I, [_KV, _P, _LL, _LL, _LL, _P, _LL, _LL, _LL, _I, _P, _I, _I, _F, _P, _SZ, _P, _P]),
     'nats_b200_paged_evict': (_I, [_KV, _P]),
     'nats_b200_paged_reorder_workspace_bytes': (_SZ, [_I, _I, _I]),
     'nats_b200_paged_reorder': (_I, [_KV, _P, _P, _SZ, _P, _P]),

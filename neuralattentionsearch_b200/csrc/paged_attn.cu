@@ -417,30 +417,25 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 && D == 64 ? 4 : 2) paged
 }
 
 // ---- host side ------------------------------------------------------------------------------------
-struct AttnPlan { bool tiles; long long line; int mt, row_tiles, split_pages, splits; size_t counter, partials, bytes; };
-// max_pages: bound of the pages of a row that the host knows; M: entries of a row
-static AttnPlan attn_plan(int S, int H, int G, int N, int D, int P, int max_pages, int M) {
+struct AttnPlan { bool tiles; int mt, row_tiles, split_pages; long long line; size_t counts, partials, bytes; };
+static AttnPlan attn_plan(int S, int H, int G, int N, int D, int P, int M) {
     AttnPlan a = {};
     // Query rows up to which paged_rows_kernel is faster.  us, rows / tiles: head_dim 64 32 rows (16 sequences of 4 heads, 2200 keys each) 24.6 / 29.1,
     // (16 of 8, 4700 keys) 41.7 / 48.7, 64 rows (one of 4, 1300 keys) 19.5 / 16.2; head_dim 128 32 rows (8 of 8, 2600 keys) 47.2 / 33.7.
     a.tiles = (long long)N * G > (D == 64 ? 2 : 1) * kRows && G <= kTile;
-    a.counter = kMaxTickets * 4;
-    a.partials = 4096;
-    static_assert(kMaxTickets * 4 + 4 <= 4096, "the front of the workspace holds the tickets and the counter");
+    a.counts = 4096;
+    static_assert(kMaxTickets * 4 <= 4096, "the front of the workspace holds the tickets");
     if (a.tiles) {
         a.row_tiles = cdiv(N, tile_tokens(G));
-        a.split_pages = 0;
-        // one item per SM as long as an item has four tiles of keys, and no more pages than an item can look at
-        const long long items = (long long)S * H * cdiv(a.row_tiles, 2);
-        const int wanted = (int)max(1ll, min(148 / items, (long long)max_pages * P / (4 * kTile)));
-        a.splits = max(wanted, cdiv(M, kTileMaxPages));
-        a.bytes = a.partials + paged_tile_partial_floats(S, H * G, N, D, a.splits) * 4;
+        a.line = (long long)S * H * cdiv(a.row_tiles, 2) * ((long long)M * P / kTile + 1);
+        a.partials = a.counts + paged_tile_count_bytes(S, H, a.row_tiles);
+        a.bytes = a.partials + paged_tile_result_bytes(D);
     } else {
         a.mt = D == 64 && (long long)N * G > kRows ? 2 : 1;
         a.row_tiles = (int)(((long long)N * G + 16 * a.mt - 1) / (16 * a.mt));
         a.split_pages = max(1, kMinStretch / P);
-        a.splits = 1;
         a.line = (long long)S * H * a.row_tiles * max(M, 1);
+        a.partials = a.counts;
         a.bytes = a.partials + (size_t)kMaxTickets * 2 * 16 * a.mt * (D + 2) * 4;
     }
     return a;
@@ -481,35 +476,34 @@ using namespace nats;
 
 #define NATS_EXPORT extern "C" __attribute__((visibility("default")))
 
-NATS_EXPORT size_t nats_b200_paged_attention_workspace_bytes(int slots, int n_heads, int n_kv_heads, int N, int head_dim, int page_size, int max_pages,
-                                                            int max_entries) {
-    if (slots <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || N <= 0 || head_dim <= 0 || page_size <= 0 || max_pages < 0 || max_entries <= 0) return 0;
-    return attn_plan(slots, n_kv_heads, n_heads / n_kv_heads, N, head_dim, page_size, max_pages, max_entries).bytes;
+NATS_EXPORT size_t nats_b200_paged_attention_workspace_bytes(int slots, int n_heads, int n_kv_heads, int N, int head_dim, int page_size, int max_entries) {
+    if (slots <= 0 || n_kv_heads <= 0 || n_heads <= 0 || n_heads % n_kv_heads || N <= 0 || head_dim <= 0 || page_size <= 0 || max_entries <= 0) return 0;
+    return attn_plan(slots, n_kv_heads, n_heads / n_kv_heads, N, head_dim, page_size, max_entries).bytes;
 }
 
 NATS_EXPORT int nats_b200_paged_attention(const NatsPagedKV* kv, const void* d_q, long long q_slot_stride, long long q_head_stride,
                                           long long q_token_stride, void* d_o, long long o_slot_stride, long long o_head_stride,
-                                          long long o_token_stride, int o_f32, const int32_t* d_n_new, int n_heads, int N, int max_pages,
+                                          long long o_token_stride, int o_f32, const int32_t* d_n_new, int n_heads, int N,
                                           float sm_scale, void* d_workspace, size_t workspace_bytes, int32_t* d_status, void* stream) {
     PagedAttnParams p;
     if (const int e = paged_kv(kv, p.kv)) return e;
     NATS_CHECK_ARG(d_q && d_o && d_workspace && d_status, "null pointer");
     NATS_CHECK_ARG(n_heads > 0 && n_heads % p.kv.H == 0, "%d query heads over %d kv-heads", n_heads, p.kv.H);
-    NATS_CHECK_ARG(N > 0 && N <= (1 << 24) && max_pages >= 0 && max_pages <= p.kv.M, "bad sizes N=%d max_pages=%d", N, max_pages);
+    NATS_CHECK_ARG(N > 0 && N <= (1 << 24), "bad size N=%d", N);
     NATS_CHECK_ARG(sm_scale > 0.f, "the scale must be positive");
     NATS_CHECK_ARG(((uintptr_t)d_q | (uintptr_t)d_o | (uintptr_t)d_workspace) % 16 == 0, "pointers must be 16-byte aligned");
     NATS_CHECK_ARG((q_slot_stride | q_head_stride | q_token_stride | o_slot_stride | o_head_stride | o_token_stride) % 8 == 0,
                    "strides must keep 16-byte alignment");
     const int G = n_heads / p.kv.H;
-    const AttnPlan a = attn_plan(p.kv.S, p.kv.H, G, N, p.kv.D, p.kv.P, max_pages, p.kv.M);
+    const AttnPlan a = attn_plan(p.kv.S, p.kv.H, G, N, p.kv.D, p.kv.P, p.kv.M);
     if (workspace_bytes < a.bytes) return fail(NATS_ERR_WORKSPACE, "paged attention workspace: %zu bytes given, %zu needed", workspace_bytes, a.bytes);
     NATS_CHECK_ARG(a.line < (1ll << 31), "%d new tokens of %d heads per kv-head are too many", N, G);
     p.q = (const __nv_bfloat16*)d_q; p.q_slot = q_slot_stride; p.q_head = q_head_stride; p.q_token = q_token_stride;
     p.o = d_o; p.o_slot = o_slot_stride; p.o_head = o_head_stride; p.o_token = o_token_stride; p.o_f32 = o_f32;
-    p.n_new = d_n_new; p.N = N; p.G = G; p.splits = a.splits; p.split_pages = a.split_pages; p.row_tiles = a.row_tiles;
+    p.n_new = d_n_new; p.N = N; p.G = G; p.split_pages = a.split_pages; p.row_tiles = a.row_tiles;
     p.scale_log2 = sm_scale * 1.4426950408889634f;
     p.tickets = (int32_t*)d_workspace;
-    p.counter = (int32_t*)((uint8_t*)d_workspace + a.counter);
+    p.counts = (int32_t*)((uint8_t*)d_workspace + a.counts);
     p.partials = (float*)((uint8_t*)d_workspace + a.partials);
     p.status = d_status;
     if (a.tiles) return launch_paged_tiles(p, (cudaStream_t)stream);

@@ -13,20 +13,19 @@ struct PagedAttnParams {
     int o_f32;
     const int32_t* n_new;                        // [S] or nullptr: N everywhere
     int N, G;
-    int splits;                                  // of the pages of a row
-    int split_pages;                             // pages per split (rows kernel)
+    int split_pages;                             // pages of a block's stretch at least (rows kernel)
     int row_tiles;                               // tiles of query rows per (slot, kv-head)
     float scale_log2;
     int32_t* tickets;
-    int32_t* counter;                            // next work item (tile kernel)
+    int32_t* counts;                             // K / V tiles of every unit (tile kernel)
     float* partials;
     int32_t* status;
 };
 
 // Tile kernel: query rows of a tile are 128 / G tokens with their G heads each
 inline int tile_tokens(int G) { return kTile / G; }
-constexpr int kTileMaxPages = 4096;              // pages that a work item looks at
 int launch_paged_tiles(const PagedAttnParams& p, cudaStream_t st);
-size_t paged_tile_partial_floats(int S, int Hq, int N, int D, int splits);
+size_t paged_tile_count_bytes(int S, int H, int row_tiles);
+size_t paged_tile_result_bytes(int D);
 
 }  // namespace nats

@@ -1,20 +1,24 @@
 // Attention of many new tokens over the paged cache: TMA-fed tcgen05.mma with TMEM accumulators.
 //
-// A work item = two tiles of query rows x one (slot, kv-head) x a split of its pages.  A query tile is 128 / G tokens with all G heads of the
-// group (row = G token + head), so that every page that is loaded serves all of them; the item's two tiles share its K / V tiles.  A K / V
-// tile holds 128 keys: the next 128 / P pages of the row that some query of the item sees, one TMA box of P rows x 64 columns each.  Pages
-// that no query of the item sees are neither loaded nor computed.
+// A unit = two tiles of query rows x one (slot, kv-head).  A query tile is 128 / G tokens with all G heads of the group (row = G token + head), so
+// that every page that is loaded serves all of them; the two tiles share the K / V tiles.  A K / V tile holds 128 keys: the next 128 / P
+// pages of the row that some query of the unit sees, one TMA box of P rows x 64 columns each.  Pages that no query of the unit sees are
+// neither loaded nor computed.
+//
+// The units with their K / V tiles form one line (paged_plan_kernel counts the tiles), of which every CTA, one per SM, takes a stretch of the
+// same length: a work item is a unit or the part of it that lies in the stretch.  Parts leave (O, maximum, sum) in the workspace and
+// paged_join_kernel joins them in order.  With whole units dealt out instead, 4001 new tokens over 22k keys (504 units, 3.4 per SM) took as long as
+// 4 per SM.
 //
 //   warp 0      TMA producer: K and V through one ring of tile-sized slots, and what the softmax warps have to know about a tile: the position and
 //               the limit of every 16 of its keys (pages are multiples of 16), and whether any query of the item must not see one of them
-//   warp 3      scheduler: takes the next item, finds the pages its queries see (a bitmap, while the item before runs), loads its Q tiles
+//   warp 3      scheduler: finds the next item of the stretch while the one before runs, loads its Q tiles
 //   warp 1      MMA issuer of S = Q.K^T, warp 2 of O += P.V (P from TMEM, as bf16: the tensor core takes both operands in one type)
 //   warps 4-7   softmax of query tile 0, warps 8-11 of query tile 1: one thread per row, the score row in registers, online, fp32
 //
 // Scores lie apart from P and are handed back as soon as they are in registers, so that the next tile's Q.K^T runs beside the softmax.
 // Keys behind a sequence's last one: the rows of an unfinished page may hold anything, and 0 * NaN is NaN, so the issuer of P.V writes zeros over
 // them in shared memory; pages that a part filled tile lacks are read as zero from behind the pool.
-// Few items: the pages of a row are split, partial results go to the workspace and a second kernel joins them in a fixed order.
 #include "paged_attn.cuh"
 #include "sm100.cuh"
 
@@ -30,13 +34,20 @@ struct PtHeader {
     int valid;                                   // 0: no more work
     int row, tile;                               // slot * H + kv-head; first query tile
     int ntiles;                                  // query tiles with a real token: 1 or 2 (0: only padding)
-    int n_kv;                                    // K / V tiles
-    int first;                                   // first entry of the item
-    int n_vis;                                   // visible pages
+    int n_kv;                                    // K / V tiles of the item
+    int skip;                                    // visible pages of the unit in front of them
     int q0, n;                                   // position of the slot's first new token, number of new tokens
-    int split;
-    int pad[2];
+    int part;                                    // -1: the whole unit; else where its partial result goes, see PtPart
+    int pad[3];
 };
+
+// A CTA shares at most two units with others: one that began before its stretch (part 0), one that goes on behind it (part 1).
+// In the workspace: [CTA][2] results of 256 rows, then what the join has to know about the unit that a CTA is the first to share.
+struct PtPart { int split, row, tile, last; int begin, chunk, pad[2]; };
+constexpr int kPtRows = 256;
+template <int D>
+struct PtResult { float4 o[D / 4][kPtRows]; float2 ml[kPtRows]; };
+constexpr int kPtMaxCtas = 160;
 
 struct PtMeta {
     int start[8], limit[8];                      // of every 16 keys: position of the first one, last query position that may see them
@@ -53,7 +64,6 @@ struct PtSmem {
     uint8_t q[2][kTileBytes];
     uint8_t ring[kSlots][kTileBytes];
     PtMeta meta[kMetas];
-    uint32_t seen[2][kTileMaxPages / 32];          // bit i: entry first + i is seen by some query of the item
     PtHeader item[2];
     unsigned long long bar_q_full[2], bar_q_empty[2];
     unsigned long long bar_full[kSlots], bar_empty[kSlots];
@@ -79,16 +89,60 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "l"(policy) : "memory");
 }
 
-// Work item w: query tile pairs fastest (they share pages), the last ones, which see most, first
-struct PtWork { int row, tile, split; };
-__device__ __forceinline__ PtWork pt_work(const PagedAttnParams& p, int w) {
-    const int pairs = (p.row_tiles + 1) / 2;
-    PtWork k;
-    k.tile = 2 * (pairs - 1 - w % pairs);
-    w /= pairs;
-    k.split = w % p.splits;
-    k.row = w / p.splits;
-    return k;
+// Position of the n-th set bit of a word (n = 0: the lowest), some position below 32 if there are not so many
+__device__ __forceinline__ int nth_set(uint32_t word, int n) {
+    int at = 0;
+#pragma unroll
+    for (int width = 16; width > 0; width >>= 1) {
+        const int low = __popc(word & ((1u << width) - 1u));
+        if (n >= low) { n -= low; word >>= width; at += width; }
+    }
+    return at;
+}
+
+// What a unit's queries see: positions of its first and last real token
+struct PtUnit { int s, n, q0, t0, t1; };
+__device__ __forceinline__ PtUnit pt_unit(const PagedAttnParams& p, int row, int tile) {
+    PtUnit u;
+    u.s = row / p.kv.H;
+    u.n = p.n_new == nullptr ? p.N : min(max(p.n_new[u.s], 0), p.N);
+    u.q0 = p.kv.length[u.s] - u.n;
+    const int TT = kTile / p.G;
+    u.t0 = tile * TT;
+    u.t1 = min(u.t0 + 2 * TT, u.n);
+    return u;
+}
+__device__ __forceinline__ bool pt_sees(const PagedKv& kv, const int4& e, int q_lo, int q_hi) {
+    return (unsigned)e.x < (unsigned)kv.num_pages && e.z >= q_lo && e.y <= q_hi;
+}
+
+// K / V tiles of every unit, in the order (row, pair of query tiles); -1 where all its tokens are padding.  `warps` warps per unit: eight while that
+// does not make more blocks than run at once, since a warp waits for its entries most of the time.
+__global__ void __launch_bounds__(256) paged_plan_kernel(const PagedAttnParams p, int warps) {
+    __shared__ int s_seen[8];
+    const int pairs = (p.row_tiles + 1) / 2, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const int unit = blockIdx.x * (8 / warps) + warp / warps, part = warp % warps;
+    wait_for_launch_before();
+    int n_vis = 0;
+    bool live = false;
+    if (unit < p.kv.S * p.kv.H * pairs) {
+        const int row = unit / pairs;
+        const PtUnit u = pt_unit(p, row, 2 * (unit - row * pairs));
+        live = u.t1 > u.t0;
+        if (live) {
+            const int q_lo = u.q0 + u.t0, q_hi = u.q0 + u.t1 - 1, n = min(max(p.kv.n_pages[row], 0), p.kv.M);
+            const int4* entries = p.kv.entries + (size_t)row * p.kv.M;
+#pragma unroll 4
+            for (int i = part * 32 + lane; i < n; i += warps * 32) n_vis += pt_sees(p.kv, entries[i], q_lo, q_hi);
+        }
+    }
+    n_vis = __reduce_add_sync(0xffffffffu, n_vis);
+    if (lane == 0) s_seen[warp] = n_vis;
+    __syncthreads();
+    if (part == 0 && lane == 0 && unit < p.kv.S * p.kv.H * pairs) {
+        for (int w = 1; w < warps; ++w) n_vis += s_seen[warp + w];
+        p.counts[unit] = live ? (n_vis * p.kv.P + kTile - 1) / kTile : -1;
+    }
 }
 
 template <int D>
@@ -148,11 +202,38 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     tc_fence_after();
     const uint32_t tmem = sm.tmem_base;
     const int G = p.G, TT = kTile / G;           // tokens per query tile
+    PtResult<D>* const results = reinterpret_cast<PtResult<D>*>(p.partials);
+    PtPart* const parts_info = reinterpret_cast<PtPart*>(results + 2 * (size_t)gridDim.x);
     if (warp < 4) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kPtRegsLow));
 
     if (warp == 3) {
         // =============================== scheduler ===============================
-        const int total = kv.S * kv.H * p.splits * ((p.row_tiles + 1) / 2);
+        const int pairs = (p.row_tiles + 1) / 2, units = kv.S * kv.H * pairs;
+        auto length_of = [&](int u) {                    // a unit that sees nothing has zeros to write, one of padding has not
+            const int c = u < units ? p.counts[u] : -1;
+            return c < 0 ? 0 : max(c, 1);
+        };
+        int sum = 0;
+#pragma unroll 4
+        for (int u = lane; u < units; u += 32) sum += length_of(u);
+        sum = __reduce_add_sync(0xffffffffu, sum);
+        const int chunk = (sum + (int)gridDim.x - 1) / (int)gridDim.x;
+        const int begin = min((int)blockIdx.x * chunk, sum), end = min(begin + chunk, sum);
+        // the unit at the beginning of the stretch, and where it begins
+        int unit = 0, unit_begin = 0;
+        for (; begin < end; unit += 32) {
+            const int incl = warp_incl_scan(length_of(unit + lane), lane);
+            const unsigned behind = __ballot_sync(0xffffffffu, unit_begin + incl > begin);
+            if (behind != 0u) {
+                const int i = __ffs(behind) - 1, at = __shfl_sync(0xffffffffu, incl, max(i - 1, 0));
+                unit += i;
+                if (i > 0) unit_begin += at;
+                break;
+            }
+            unit_begin += __shfl_sync(0xffffffffu, incl, 31);
+        }
+        PtPart shared = {};
+        int line = begin;
         bool ok = true;
         int q_loads[2] = {0, 0};
         const uint64_t pol_q = l2_policy_evict_first();
@@ -160,46 +241,26 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             const int slot = ic & 1, use = ic >> 1;
             if (use > 0) ok = util_wait<kRelaxNs>(smem_u32(&sm.bar_list_empty[slot]), (use - 1) & 1, abort_flag, p.status, kPtErr + kErrList);
             if (!ok) break;
-            int w = blockIdx.x;                          // the first item is the CTA's own, others come from the counter
-            if (ic > 0) {
-                if (total > (int)gridDim.x && lane == 0) w = atomicAdd(p.counter, 1);
-                w = (int)gridDim.x + __shfl_sync(0xffffffffu, w, 0);
-            }
-            const bool have = w < total;
+            const bool have = line < end;
             PtHeader hd;
             hd.valid = have;
             if (have) {
-                const PtWork k = pt_work(p, w);
-                const int s = k.row / kv.H;
-                hd.row = k.row; hd.tile = k.tile; hd.split = k.split;
-                hd.n = p.n_new == nullptr ? p.N : min(max(p.n_new[s], 0), p.N);
-                hd.q0 = kv.length[s] - hd.n;
-                const int t0 = k.tile * TT, t1 = min(t0 + 2 * TT, hd.n);       // the item's tokens
-                hd.ntiles = t1 <= t0 ? 0 : t1 - t0 > TT ? 2 : 1;
-                const int n_pages = min(max(kv.n_pages[k.row], 0), kv.M);
-                const int per = (n_pages + p.splits - 1) / p.splits, e0 = min(k.split * per, n_pages), e1 = min(e0 + per, n_pages);
-                hd.first = e0;
-                int n_vis = 0;
-                if (hd.ntiles > 0) {
-                    const int q_lo = hd.q0 + t0, q_hi = hd.q0 + t1 - 1;
-                    const int4* entries = kv.entries + (size_t)k.row * kv.M;
-                    for (int i = e0; i < e1; i += 128) {
-                        int4 e[4];
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const int at = i + 32 * x + lane;
-                            e[x] = at < e1 ? entries[at] : make_int4(-1, 0, 0, 0);
-                        }
-#pragma unroll
-                        for (int x = 0; x < 4; ++x) {
-                            const unsigned m = __ballot_sync(0xffffffffu, (unsigned)e[x].x < (unsigned)kv.num_pages && e[x].z >= q_lo && e[x].y <= q_hi);
-                            if (lane == 0 && i + 32 * x < e1) sm.seen[slot][(i - e0) / 32 + x] = m;
-                            n_vis += __popc(m);
-                        }
-                    }
-                }
-                hd.n_vis = n_vis;
-                hd.n_kv = (n_vis * kv.P + kTile - 1) / kTile;
+                for (unsigned m; (m = __ballot_sync(0xffffffffu, length_of(unit + lane) > 0)) == 0u || (unit += __ffs(m) - 1, false);) unit += 32;
+                hd.row = unit / pairs;
+                hd.tile = 2 * (unit - hd.row * pairs);
+                const PtUnit u = pt_unit(p, hd.row, hd.tile);
+                hd.n = u.n;
+                hd.q0 = u.q0;
+                hd.ntiles = u.t1 <= u.t0 ? 0 : u.t1 - u.t0 > TT ? 2 : 1;
+                const int tiles = p.counts[unit], unit_end = unit_begin + max(tiles, 1), to = min(end, unit_end);
+                const int first = unit_begin / chunk, last = (unit_end - 1) / chunk;
+                hd.n_kv = tiles > 0 ? to - line : 0;
+                hd.skip = (line - unit_begin) * (kTile / kv.P);
+                hd.part = first == last ? -1 : unit_begin < begin ? 0 : 1;
+                if (hd.part == 1) { shared.split = 1; shared.row = hd.row; shared.tile = hd.tile; shared.last = last; shared.begin = unit_begin; shared.chunk = chunk; }
+                line = to;
+                unit_begin = unit_end;
+                ++unit;
             }
             if (lane == 0) sm.item[slot] = hd;
             __syncwarp();
@@ -223,6 +284,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                 __syncwarp();
             }
         }
+        if (lane == 0) parts_info[blockIdx.x] = shared;
         if (!ok) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
@@ -242,21 +304,52 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             if (!ok) break;
             const PtHeader hd = sm.item[slot];
             if (!hd.valid) break;
-            const int4* entries = kv.entries + (size_t)hd.row * kv.M + hd.first;
+            const int4* entries = kv.entries + (size_t)hd.row * kv.M;
+            const int n_entries = hd.n_kv > 0 ? min(max(kv.n_pages[hd.row], 0), kv.M) : 0;
             const int q_lo = hd.q0 + hd.tile * TT, q_hi = hd.q0 + min(hd.tile * TT + 2 * TT, hd.n) - 1, end = hd.q0 + hd.n;
+            // a window of 32 entries, one per lane, the next one on its way; seen: those of the window that are visible and not used up
+            int base = 0;
+            auto window = [&](int at) { return at + lane < n_entries ? entries[at + lane] : make_int4(-1, 0, 0, 0); };
+            int skip = hd.skip;
+            while (skip > 0 && base < n_entries) {               // four windows at a time
+                int4 w[4];
+                unsigned m[4];
+#pragma unroll
+                for (int i = 0; i < 4; ++i) w[i] = window(base + 32 * i);
+                int c = 0;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) { m[i] = __ballot_sync(0xffffffffu, pt_sees(kv, w[i], q_lo, q_hi)); c += __popc(m[i]); }
+                if (c > skip) {
+#pragma unroll
+                    for (int i = 0; i < 3; ++i)
+                        if (c > skip && __popc(m[i]) <= skip) { skip -= __popc(m[i]); base += 32; c = skip + 1; } else break;
+                    break;
+                }
+                skip -= c;
+                base += 128;
+            }
+            int4 win = window(base), win_next = window(base + 32);
+            unsigned seen = __ballot_sync(0xffffffffu, pt_sees(kv, win, q_lo, q_hi));
+            auto next_window = [&]() {
+                base += 32;
+                win = win_next;
+                win_next = window(base + 32);
+                seen = __ballot_sync(0xffffffffu, pt_sees(kv, win, q_lo, q_hi));
+            };
+            for (; skip > 0; --skip) seen &= seen - 1u;
             // the pages of the next tile, looked up a tile ahead: lane j holds the entry of its j-th page (page num_pages: none, read as zero)
-            int word = 0, left = hd.n_vis;
-            uint32_t cur = hd.n_kv > 0 ? sm.seen[slot][0] : 0u;
             int4 e;
             auto look_up = [&]() {
-                int at = -1;
-                for (int j = 0; j < ppt && left > 0; ++j, --left) {
-                    while (cur == 0u) cur = sm.seen[slot][++word];
-                    const int b = __ffs(cur) - 1;
-                    cur &= cur - 1u;
-                    if (lane == j) at = word * 32 + b;
+                e = make_int4(kv.num_pages, kNoLimit, -1, 0);
+                for (int got = 0; got < ppt && base < n_entries;) {
+                    const int c = min(__popc(seen), ppt - got);
+                    const int from = nth_set(seen, lane - got);
+                    const int x = __shfl_sync(0xffffffffu, win.x, from), y = __shfl_sync(0xffffffffu, win.y, from), z = __shfl_sync(0xffffffffu, win.z, from);
+                    if (lane >= got && lane < got + c) e = make_int4(x, y, z, 0);
+                    got += c;
+                    if (c == __popc(seen)) next_window();
+                    else for (int i = 0; i < c; ++i) seen &= seen - 1u;
                 }
-                e = at >= 0 ? entries[at] : make_int4(kv.num_pages, kNoLimit, -1, 0);
             };
             if (hd.n_kv > 0) look_up();
             for (int j = 0; j < hd.n_kv && ok; ++j) {
@@ -412,6 +505,17 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         const int tok = row / G, head = row - tok * G;   // token in the tile, head in the group
         uint32_t gt = 0;                                 // tiles of this query tile so far
         int metas = 0;
+        if (p.n_new != nullptr) {
+            // padding: zeros, while the first tiles are on their way.  A CTA takes every gridDim.x-th eighth of a head's tokens.
+            const int vecs = D / (p.o_f32 ? 4 : 8), per = (p.N + 7) / 8, size = p.o_f32 ? 4 : 2;
+            for (int w = blockIdx.x; w < kv.S * kv.H * G * 8; w += gridDim.x) {
+                const int hq = w / 8 % (kv.H * G), s = w / 8 / (kv.H * G), t0 = max(min(max(p.n_new[s], 0), p.N), w % 8 * per), t1 = min(p.N, (w % 8 + 1) * per);
+                uint8_t* base = (uint8_t*)p.o + (s * p.o_slot + hq * p.o_head) * size;
+                for (int i = (warp - 4) * 32 + lane; i < (t1 - t0) * vecs; i += 256)
+                    st16(base + (t0 + i / vecs) * p.o_token * size + i % vecs * 16, make_uint4(0, 0, 0, 0));
+            }
+            __syncwarp();
+        }
         bool ok = true;
         for (int ic = 0; ok; ++ic) {
             const int slot = ic & 1;
@@ -524,19 +628,14 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                 tc_fence_after();
             }
             if (ok) {
-                // O / l, or with splits O, the maximum and l; a token without a visible key, and padding, give zeros
+                // O / l, or of a part O, the maximum and l; a token without a visible key gives zeros
                 const int s = hd.row / kv.H, hq = (hd.row - s * kv.H) * G + head;
-                const bool has_o = h < hd.ntiles && n > 0, mine = tok < TT && t < p.N;
-                const bool whole = p.splits == 1;
-                const size_t lin = ((size_t)s * (kv.H * G) + hq) * p.N + t, rows = (size_t)kv.S * kv.H * G * p.N;
-                float* part = p.partials + ((size_t)hd.split * rows + lin) * D;
-                if (!whole && mine) {
-                    float* ml = p.partials + (size_t)p.splits * rows * D + ((size_t)hd.split * rows + lin) * 2;
-                    *reinterpret_cast<float2*>(ml) = make_float2(has_o && real ? m_ref : -INFINITY, has_o && real ? l_sum : 0.f);
-                }
-                const float inv = whole ? (l_sum != 0.f && real ? 1.f / l_sum : 0.f) : 1.f;
-                const bool zero = !has_o || !real || l_sum == 0.f;
+                const bool has_o = h < hd.ntiles && n > 0, whole = hd.part < 0;
+                const float inv = whole ? 1.f / l_sum : 1.f;
+                const bool zero = !has_o || l_sum == 0.f;
                 const long long o_at = s * p.o_slot + hq * p.o_head + t * p.o_token;
+                PtResult<D>& result = results[2 * (size_t)blockIdx.x + (whole ? 0 : hd.part)];
+                if (!whole && real) result.ml[h * kTile + row] = make_float2(m_ref, l_sum);
 #pragma unroll 1
                 for (int c0 = 0; c0 < D; c0 += 32) {
                     uint32_t r[32];
@@ -552,18 +651,23 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                     }
 #pragma unroll
                     for (int i = 0; i < 32; ++i) r[i] = zero ? 0u : __float_as_uint(__uint_as_float(r[i]) * inv);
-                    float* to = whole ? (float*)p.o + o_at + c0 : part + c0;
-                    if (mine && (whole ? p.o_f32 != 0 : !zero)) {
+                    if (!whole) {
+                        if (real) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 4) st16(&result.o[(c0 + i) / 4][h * kTile + row], make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]));
+                        }
+                    } else if (real && p.o_f32) {
+                        float* to = (float*)p.o + o_at + c0;
 #pragma unroll
                         for (int i = 0; i < 32; i += 4) st16(to + i, make_uint4(r[i], r[i + 1], r[i + 2], r[i + 3]));
-                    } else if (mine && whole) {
-                        __nv_bfloat16* to16 = (__nv_bfloat16*)p.o + o_at + c0;
+                    } else if (real) {
+                        __nv_bfloat16* to = (__nv_bfloat16*)p.o + o_at + c0;
 #pragma unroll
                         for (int i = 0; i < 32; i += 8) {
                             uint32_t w[4];
 #pragma unroll
                             for (int x = 0; x < 4; ++x) w[x] = pack_bf16(__uint_as_float(r[i + 2 * x]), __uint_as_float(r[i + 2 * x + 1]));
-                            st16(to16 + i, make_uint4(w[0], w[1], w[2], w[3]));
+                            st16(to + i, make_uint4(w[0], w[1], w[2], w[3]));
                         }
                     }
                 }
@@ -585,58 +689,71 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     }
 }
 
-// Joins the splits of a query row: a warp per row, D / 32 columns per lane.  The splits' maxima and sums are read by as many lanes, their columns
-// eight splits at a time.
+// Joins the parts of the units that lie in several stretches: blockIdx.x is the first CTA of such a unit, blockIdx.y 32 of its rows.  A lane
+// per row, 16 columns per warp and pass.
 template <int D>
-__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p) {
-    constexpr int W = D / 32;
-    const size_t rows = (size_t)p.kv.S * p.kv.H * p.G * p.N, lin = (size_t)blockIdx.x * 8 + threadIdx.x / 32;
+__global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p, int n_ctas) {
     wait_for_launch_before();
-    if (lin >= rows) return;
-    const int lane = threadIdx.x & 31;
-    const float2* ml = reinterpret_cast<const float2*>(p.partials + (size_t)p.splits * rows * D);
-    float m = -INFINITY;
-    for (int x = lane; x < p.splits; x += 32) m = fmaxf(m, ml[x * rows + lin].x);
+    if (*p.status != 0) return;                  // the CTAs may have left nothing
+    const PtResult<D>* results = reinterpret_cast<const PtResult<D>*>(p.partials);
+    const PtPart part = reinterpret_cast<const PtPart*>(results + 2 * (size_t)n_ctas)[blockIdx.x];
+    if (!part.split) return;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.y * 32 + lane;
+    const int TT = kTile / p.G, row = r & (kTile - 1), tok = row / p.G, head = row - tok * p.G;
+    const int s = part.row / p.kv.H, n = p.n_new == nullptr ? p.N : min(max(p.n_new[s], 0), p.N);
+    const int t = (part.tile + r / kTile) * TT + tok, first = blockIdx.x;
+    if (tok >= TT || t >= p.N) return;
+    const bool real = t < n;
+    auto result_of = [&](int x) -> const PtResult<D>& { return results[2 * (size_t)x + (part.begin < x * part.chunk ? 0 : 1)]; };
+    const int hq = (part.row - s * p.kv.H) * p.G + head;
+    const long long at = s * p.o_slot + hq * p.o_head + t * p.o_token;
+    for (int c = warp * 4; c < D / 4; c += 32) {           // four groups of four columns
+        float4 a[4] = {};
+        float m = -INFINITY, l = 0.f;
+        constexpr int AT_ONCE = 4;                         // parts on their way at a time
+        for (int x0 = real ? first : part.last + 1; x0 <= part.last; x0 += AT_ONCE) {
+            float2 ml[AT_ONCE];
+            float4 o[AT_ONCE][4];
 #pragma unroll
-    for (int o = 16; o > 0; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
-    const float mu = m == -INFINITY ? 0.f : m;
-    float a[W] = {}, l = 0.f;
-    for (int x0 = 0; x0 < p.splits; x0 += 8) {
-        float2 v[8];
-        float o[8][W];
+            for (int k = 0; k < AT_ONCE; ++k) {
+                const PtResult<D>& res = result_of(min(x0 + k, part.last));
+                ml[k] = __ldcg(&res.ml[r]);
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-            v[x] = x0 + x < p.splits ? ml[(x0 + x) * rows + lin] : make_float2(0.f, 0.f);
-            if (x0 + x < p.splits) {
-                const float* from = p.partials + ((x0 + x) * rows + lin) * D + lane * W;
-#pragma unroll
-                for (int i = 0; i < W; ++i) o[x][i] = from[i];
+                for (int i = 0; i < 4; ++i) o[k][i] = __ldcg(&res.o[c + i][r]);
             }
+            float m_new = m;
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) m_new = fmaxf(m_new, ml[k].x);
+            const float mu = m_new == -INFINITY ? 0.f : m_new, old = ex2(m - mu);
+            l *= old;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) { a[i].x *= old; a[i].y *= old; a[i].z *= old; a[i].w *= old; }
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) {
+                if (x0 + k > part.last) break;
+                const float f = ex2(ml[k].x - mu);
+                l = fmaf(ml[k].y, f, l);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    a[i].x = fmaf(o[k][i].x, f, a[i].x); a[i].y = fmaf(o[k][i].y, f, a[i].y);
+                    a[i].z = fmaf(o[k][i].z, f, a[i].z); a[i].w = fmaf(o[k][i].w, f, a[i].w);
+                }
+            }
+            m = m_new;
         }
+        const float inv = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
-        for (int x = 0; x < 8; ++x) {
-            if (v[x].y == 0.f) continue;                 // nothing visible in this split: no O was written
-            const float f = ex2(v[x].x - mu);
-            l = fmaf(v[x].y, f, l);
-#pragma unroll
-            for (int i = 0; i < W; ++i) a[i] = fmaf(o[x][i], f, a[i]);
+        for (int i = 0; i < 4; ++i) {
+            if (p.o_f32) *reinterpret_cast<float4*>((float*)p.o + at + (c + i) * 4) = make_float4(a[i].x * inv, a[i].y * inv, a[i].z * inv, a[i].w * inv);
+            else *reinterpret_cast<uint2*>((__nv_bfloat16*)p.o + at + (c + i) * 4) = make_uint2(pack_bf16(a[i].x * inv, a[i].y * inv), pack_bf16(a[i].z * inv, a[i].w * inv));
         }
-    }
-    const float inv = l != 0.f ? 1.f / l : 0.f;
-    const int t = (int)(lin % p.N);
-    const size_t sh = lin / p.N;
-    const int Hq = p.kv.H * p.G, hq = (int)(sh % Hq), s = (int)(sh / Hq);
-    const long long at = s * p.o_slot + hq * p.o_head + t * p.o_token + lane * W;
-    if (p.o_f32) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) ((float*)p.o)[at + i] = a[i] * inv;
-    } else {
-#pragma unroll
-        for (int i = 0; i < W; i += 2) *reinterpret_cast<uint32_t*>((__nv_bfloat16*)p.o + at + i) = pack_bf16(a[i] * inv, a[i + 1] * inv);
     }
 }
 
-size_t paged_tile_partial_floats(int S, int Hq, int N, int D, int splits) { return splits == 1 ? 0 : (size_t)splits * S * Hq * N * (D + 2); }
+size_t paged_tile_count_bytes(int S, int H, int row_tiles) { return align_up((size_t)S * H * ((row_tiles + 1) / 2) * 4, 256); }
+size_t paged_tile_result_bytes(int D) {
+    return (size_t)kPtMaxCtas * (2 * (D == 64 ? sizeof(PtResult<64>) : sizeof(PtResult<128>)) + sizeof(PtPart));
+}
 
 static int pool_map(CUtensorMap* map, const void* base, const PagedKv& kv) {
     EncodeTiledFn fn = get_encode_fn();
@@ -675,26 +792,26 @@ static int launch_tiles(const PagedAttnParams& p, cudaStream_t st) {
         NATS_CHECK_CUDA(cudaDeviceGetAttribute(&n_sm, cudaDevAttrMultiProcessorCount, dev));
         if (dev < 64) sms[dev] = n_sm;
     }
-    const long long items = (long long)p.kv.S * p.kv.H * p.splits * ((p.row_tiles + 1) / 2);
-    if (items > n_sm) NATS_CHECK_CUDA(cudaMemsetAsync(p.counter, 0, 4, st));
+    const int units = p.kv.S * p.kv.H * ((p.row_tiles + 1) / 2), ctas = min(n_sm, kPtMaxCtas);
     cudaLaunchAttribute attr = {};
     attr.id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr.val.programmaticStreamSerializationAllowed = 1;
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)min(items, (long long)n_sm));
-    cfg.blockDim = dim3(kPtThreads);
-    cfg.dynamicSmemBytes = sizeof(PtSmem<D>);
+    const int warps = units <= 8 * n_sm ? 8 : 1;
+    cfg.gridDim = dim3(cdiv(units, 8 / warps));
+    cfg.blockDim = dim3(256);
     cfg.stream = st;
     cfg.attrs = &attr;
     cfg.numAttrs = 1;
+    NATS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_plan_kernel, p, warps));
+    cfg.gridDim = dim3(ctas);
+    cfg.blockDim = dim3(kPtThreads);
+    cfg.dynamicSmemBytes = sizeof(PtSmem<D>);
     NATS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_tile_kernel<D>, map_q, map_k, map_v, p));
-    if (p.splits > 1) {
-        const size_t rows = (size_t)p.kv.S * p.kv.H * p.G * p.N;
-        cfg.gridDim = dim3((unsigned)((rows + 7) / 8));
-        cfg.blockDim = dim3(256);
-        cfg.dynamicSmemBytes = 0;
-        NATS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<D>, p));
-    }
+    cfg.gridDim = dim3(ctas, kPtRows / 32);
+    cfg.blockDim = dim3(256);
+    cfg.dynamicSmemBytes = 0;
+    NATS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<D>, p, ctas));
     return NATS_OK;
 }
 

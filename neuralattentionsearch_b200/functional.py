@@ -802,12 +802,11 @@ def _paged_append(kv, k, v, roles, lens, N, sliding_window, skip_hidden):
 
 
 def paged_attention(kv: PagedKV, q: torch.Tensor, sm_scale: float | None = None, n_new: torch.Tensor | None = None,
-                    max_pages: int | None = None, token_major: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
+                    token_major: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of the newest tokens of every slot over its pages, which hold their K and V already.  q [S,Hq,N,D] (cast to bf16 if needed;
     any strides that keep rows dense and 16-byte aligned); row i of slot s is the token at position ``length[s] - n_new[s] + i``
     (``n_new`` int32 [S]; None: N everywhere).  A key is seen from its own position on up to the limit of its page.  Rows behind a slot's
-    new tokens and rows that see nothing are zero.  ``max_pages``: a bound of ``n_pages`` the host knows (the work is split by it; the
-    result does not depend on its being right).  Returns o [S,Hq,N,D] in q's dtype; ``token_major``: a view of a [S,N,Hq,D] tensor;
+    new tokens and rows that see nothing are zero.  Returns o [S,Hq,N,D] in q's dtype; ``token_major``: a view of a [S,N,Hq,D] tensor;
     ``out``: written and returned, of q's shape and type (bf16 or fp32)."""
     kv._check(q)
     S, Hq, N, D = q.shape
@@ -817,15 +816,14 @@ def paged_attention(kv: PagedKV, q: torch.Tensor, sm_scale: float | None = None,
     scale = D ** -0.5 if sm_scale is None else float(sm_scale)
     if not scale > 0.0:
         raise ValueError('sm_scale must be positive')
-    bound = kv.max_entries if max_pages is None else max(0, min(int(max_pages), kv.max_entries))
     if out is not None:
         kv._check(out)
         if out.shape != q.shape or out.dtype is not q.dtype or out.dtype not in (torch.bfloat16, torch.float32) or not _strided_ok(out) or 0 in out.stride():
             raise ValueError('out must be bf16 or fp32, shaped and typed like q, with dense rows and 16-byte alignment')
-    return _on(kv.index, _paged_attention, kv, q, scale, lens, bound, token_major, out)
+    return _on(kv.index, _paged_attention, kv, q, scale, lens, token_major, out)
 
 
-def _paged_attention(kv, q, scale, lens, bound, token_major, o):
+def _paged_attention(kv, q, scale, lens, token_major, o):
     S, Hq, N, D = q.shape
     f32 = q.dtype is torch.float32                       # fp32 callers: the kernel writes fp32 itself
     dtype = torch.float32 if f32 else torch.bfloat16
@@ -838,10 +836,10 @@ def _paged_attention(kv, q, scale, lens, bound, token_major, o):
         if not _strided_ok(qb) or 0 in qb.stride():
             qb = qb.contiguous()
         stream = torch._C._cuda_getCurrentRawStream(kv.index)
-        ws = _paged_scratch(kv, 'attention', stream, S, Hq, kv.n_kv_heads, N, D, kv.page_size, bound, kv.max_entries)
+        ws = _paged_scratch(kv, 'attention', stream, S, Hq, kv.n_kv_heads, N, D, kv.page_size, kv.max_entries)
         qs, qh, qt, _ = qb.stride()
         os, oh, ot, _ = o.stride()
-        _lib.call('nats_b200_paged_attention', kv._c, qb.data_ptr(), qs, qh, qt, o.data_ptr(), os, oh, ot, f32, lens, Hq, N, bound, scale,
+        _lib.call('nats_b200_paged_attention', kv._c, qb.data_ptr(), qs, qh, qt, o.data_ptr(), os, oh, ot, f32, lens, Hq, N, scale,
                   ws.data_ptr(), ws.numel(), _status_ptr(kv.index), stream)
     return o if o.dtype is q.dtype else o.to(q.dtype)
 

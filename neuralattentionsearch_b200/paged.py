@@ -156,10 +156,10 @@ class NAtSPagedLayerCache:
     def prefill_attention(self, xq: torch.Tensor, sm_scale: float | None = None) -> torch.Tensor:
         """Attention of several new tokens over the cache, which holds them since ``update``: [B,Hq,n,D] -> [B,Hq,n,D], the outputs that one
         call over the whole sequence would give."""
-        return F_.paged_attention(self.kv, xq, sm_scale, max_pages=self._bound, token_major=True)
+        return F_.paged_attention(self.kv, xq, sm_scale, token_major=True)
 
     def decode_attention(self, xq: torch.Tensor, sm_scale: float | None = None) -> torch.Tensor:
-        return F_.paged_attention(self.kv, xq, sm_scale, max_pages=self._bound)
+        return F_.paged_attention(self.kv, xq, sm_scale)
 
     def post_update(self, x_len: int) -> None:
         if x_len == 0:
@@ -180,7 +180,7 @@ class NAtSPagedLayerCache:
         self._room((self.chunk_fill_size + n_steps) // self.chunk_size + 1)
         kv, stream = self.kv, torch.cuda.current_stream(self.device).cuda_stream
         F_._paged_scratch(kv, 'append', stream, kv.slots, kv.n_kv_heads, 1, kv.page_size)
-        F_._paged_scratch(kv, 'attention', stream, kv.slots, n_heads, kv.n_kv_heads, 1, head_dim, kv.page_size, self._bound, kv.max_entries)
+        F_._paged_scratch(kv, 'attention', stream, kv.slots, n_heads, kv.n_kv_heads, 1, head_dim, kv.page_size, kv.max_entries)
         self._static_steps_left = n_steps
 
     def decode_step_static(self, xq: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, roles: torch.Tensor, out: torch.Tensor,
@@ -189,7 +189,7 @@ class NAtSPagedLayerCache:
         [B,Hq,1,D], k_new / v_new [B,Hkv,1,D]; roles uint8 [B,Hkv] = role of the chunk this token completes (read on the device only
         if it does).  While a graph is being recorded pass ``recording=True``; after replaying the step n times call ``note_static_steps(n)``."""
         F_.paged_append(self.kv, k_new, v_new, roles.view(self.bsz, self.n_msks, 1), self.sliding_window_size)
-        F_.paged_attention(self.kv, xq, sm_scale, max_pages=self._bound, out=out)
+        F_.paged_attention(self.kv, xq, sm_scale, out=out)
         F_.paged_evict(self.kv)
         if not recording:
             self.note_static_steps(1)

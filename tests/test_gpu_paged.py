@@ -275,12 +275,12 @@ def test_bad_page_numbers_are_pages_that_are_not_there():
         assert torch.equal(got, t.F.paged_attention(t.kv, q))
 
 
-def test_any_bound_of_the_pages_gives_the_same():
+def test_many_pages_per_row():
     t = Pair(S=2, Hkv=2, G=4, P=16, D=64, SW=64, num_pages=1200, M=260, seed=4)
-    t.append(4000, roles=None)
-    for n in (1, 40, 300):
-        for bound in (None, 250, 260, 1, 0, 100):
-            t.attend(n, n_new=None, max_pages=bound)
+    t.append(4000, n_new=[4000, 1700], roles=None)
+    for n in (1, 8, 40, 300):
+        t.attend(n)
+        t.attend(n, n_new=[n, n // 2])
 
 
 def test_other_streams_and_a_recorded_step():

@@ -85,17 +85,17 @@ def test_c_entry_points_refuse_bad_arguments():
         assert call() == rc and text in lib.nats_b200_last_error()
     assert lib.nats_b200_paged_append_count(kv(), None, 1, None, 4, 16, one, None) == 1
 
-    def attend(q=one, strides=(64,) * 6, heads=4, N=2, max_pages=8, scale=0.1, nbytes=1 << 40, status=one):
-        return lib.nats_b200_paged_attention(kv(), q, *strides[:3], one, *strides[3:], 0, None, heads, N, max_pages, scale, one, nbytes, status, None)
-    for rc, text, call in ((1, b'null', lambda: attend(q=None)), (1, b'query heads', lambda: attend(heads=3)), (1, b'sizes', lambda: attend(N=0)),
-                           (1, b'sizes', lambda: attend(max_pages=9)), (1, b'scale', lambda: attend(scale=0.0)), (1, b'scale', lambda: attend(scale=float('nan'))),
+    def attend(q=one, strides=(64,) * 6, heads=4, N=2, scale=0.1, nbytes=1 << 40, status=one):
+        return lib.nats_b200_paged_attention(kv(), q, *strides[:3], one, *strides[3:], 0, None, heads, N, scale, one, nbytes, status, None)
+    for rc, text, call in ((1, b'null', lambda: attend(q=None)), (1, b'query heads', lambda: attend(heads=3)), (1, b'size', lambda: attend(N=0)),
+                           (1, b'scale', lambda: attend(scale=0.0)), (1, b'scale', lambda: attend(scale=float('nan'))),
                            (1, b'aligned', lambda: attend(q=264)), (1, b'strides', lambda: attend(strides=(64, 64, 64, 64, 64, 4))), (4, b'workspace', lambda: attend(nbytes=4096))):
         assert call() == rc and text in lib.nats_b200_last_error()
     assert lib.nats_b200_paged_reorder(kv(), None, one, 1 << 30, one, None) == 1
     assert lib.nats_b200_paged_reorder(kv(), one, one, 64, one, None) == 4
     for fn, args in ((lib.nats_b200_paged_append_workspace_bytes, (2, 2, 4, 16)), (lib.nats_b200_paged_reorder_workspace_bytes, (2, 2, 8)),
-                     (lib.nats_b200_paged_attention_workspace_bytes, (2, 4, 2, 4, 64, 16, 8, 8))):
+                     (lib.nats_b200_paged_attention_workspace_bytes, (2, 4, 2, 4, 64, 16, 8))):
         assert fn(*args) > 0
         assert fn(0, *args[1:]) == 0
-    assert lib.nats_b200_paged_attention_workspace_bytes(2, 3, 2, 4, 64, 16, 8, 8) == 0
+    assert lib.nats_b200_paged_attention_workspace_bytes(2, 3, 2, 4, 64, 16, 8) == 0
     assert ctypes.sizeof(_lib.NatsPagedKV) == 7 * 8 + 6 * 4
