@@ -368,11 +368,15 @@ typedef struct NatsPagedKV {
  * Free pages are taken from the lowest on in the order (slot, kv-head, chunk).  skip_hidden != 0: whole chunks that no query behind this call
  * sees are not stored (a prompt whose attention does not read the pages).
  */
+typedef struct NatsPagedAppend {
+    const void* d_k; const void* d_v;
+    long long k_slot_stride, k_head_stride, k_token_stride, v_slot_stride, v_head_stride, v_token_stride;
+    const uint8_t* d_roles; const int32_t* d_n_new;
+    void* d_workspace; size_t workspace_bytes; int32_t* d_status;
+    int f32, n_roles, N, SW, skip_hidden;
+} NatsPagedAppend;
 size_t nats_b200_paged_append_workspace_bytes(int slots, int n_kv_heads, int N, int page_size);
-int nats_b200_paged_append(const NatsPagedKV* kv, const void* d_k, const void* d_v, long long k_slot_stride, long long k_head_stride,
-                           long long k_token_stride, long long v_slot_stride, long long v_head_stride, long long v_token_stride,
-                           int f32, const uint8_t* d_roles, int n_roles, const int32_t* d_n_new, int N, int SW, int skip_hidden,
-                           void* d_workspace, size_t workspace_bytes, int32_t* d_status, void* stream);
+int nats_b200_paged_append(const NatsPagedKV* kv, const NatsPagedAppend* args, void* stream);
 
 /* d_counts int32 [slots, n_kv_heads]: pages that nats_b200_paged_append with skip_hidden would take for a row.  Changes nothing. */
 int nats_b200_paged_append_count(const NatsPagedKV* kv, const uint8_t* d_roles, int n_roles, const int32_t* d_n_new, int N, int SW,
@@ -384,11 +388,16 @@ int nats_b200_paged_append_count(const NatsPagedKV* kv, const uint8_t* d_roles, 
  * behind a slot's last token, and in pages that no query of the call sees, is never used, whatever it holds; a V value of a visible token that is
  * not finite reaches, besides the queries that see it, others of the same call.
  */
+typedef struct NatsPagedAttention {
+    const void* d_q; void* d_o;
+    long long q_slot_stride, q_head_stride, q_token_stride, o_slot_stride, o_head_stride, o_token_stride;
+    const int32_t* d_n_new;
+    void* d_workspace; size_t workspace_bytes; int32_t* d_status;
+    float sm_scale;
+    int o_f32, n_heads, N;
+} NatsPagedAttention;
 size_t nats_b200_paged_attention_workspace_bytes(int slots, int n_heads, int n_kv_heads, int N, int head_dim, int page_size, int max_entries);
-int nats_b200_paged_attention(const NatsPagedKV* kv, const void* d_q, long long q_slot_stride, long long q_head_stride, long long q_token_stride,
-                              void* d_o, long long o_slot_stride, long long o_head_stride, long long o_token_stride, int o_f32,
-                              const int32_t* d_n_new, int n_heads, int N, float sm_scale, void* d_workspace,
-                              size_t workspace_bytes, int32_t* d_status, void* stream);
+int nats_b200_paged_attention(const NatsPagedKV* kv, const NatsPagedAttention* args, void* stream);
 
 /* Pages that the next query position (d_length) cannot see leave the rows; a page that loses its last holder is free again. */
 int nats_b200_paged_evict(const NatsPagedKV* kv, void* stream);

@@ -4,6 +4,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -12,15 +13,11 @@ LIB_PATH = os.environ.get('NATS_B200_LIB') or os.path.join(_HERE, 'libnats_b200.
 _c = ctypes
 _P, _I, _F, _SZ = _c.c_void_p, _c.c_int, _c.c_float, _c.c_size_t
 
-_LL = _c.c_longlong
-
-
-class NatsPagedKV(_c.Structure):
-    _fields_ = [(n, _P) for n in ('d_pages_k', 'd_pages_v', 'd_refs', 'd_free_bits', 'd_entries', 'd_n_pages', 'd_length')] + \
-               [(n, _I) for n in ('num_pages', 'page_size', 'head_dim', 'slots', 'n_kv_heads', 'max_entries')]
-
-
-_KV = _c.POINTER(NatsPagedKV)
+# The structs of the paged entry points as packed bytes (NatsPagedKV, NatsPagedAppend, NatsPagedAttention): packing is several times cheaper
+# than a ctypes.Structure, and a decode step makes three such calls per layer
+PAGED_KV = struct.Struct('7Q6i').pack
+PAGED_APPEND = struct.Struct('2Q6q5Q5i').pack
+PAGED_ATTENTION = struct.Struct('2Q6q4Qf3i').pack
 
 # name -> (restype, argtypes); mirrors include/nats_b200.h
 SIGNATURES = {
@@ -57,13 +54,13 @@ SIGNATURES = {
     'nats_b200_decode_step_place': (_I, [_P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _P]),
     'nats_b200_decode_step': (_I, [_P, _P, _P, _P, _P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _F, _P, _SZ, _P]),
     'nats_b200_paged_append_workspace_bytes': (_SZ, [_I, _I, _I, _I]),
-    'nats_b200_paged_append': (_I, [_KV, _P, _P, _LL, _LL, _LL, _LL, _LL, _LL, _I, _P, _I, _P, _I, _I, _I, _P, _SZ, _P, _P]),
-    'nats_b200_paged_append_count': (_I, [_KV, _P, _I, _P, _I, _I, _P, _P]),
+    'nats_b200_paged_append': (_I, [_P, _P, _P]),
+    'nats_b200_paged_append_count': (_I, [_P, _P, _I, _P, _I, _I, _P, _P]),
     'nats_b200_paged_attention_workspace_bytes': (_SZ, [_I, _I, _I, _I, _I, _I, _I]),
-    'nats_b200_paged_attention': (_I, [_KV, _P, _LL, _LL, _LL, _P, _LL, _LL, _LL, _I, _P, _I, _I, _F, _P, _SZ, _P, _P]),
-    'nats_b200_paged_evict': (_I, [_KV, _P]),
+    'nats_b200_paged_attention': (_I, [_P, _P, _P]),
+    'nats_b200_paged_evict': (_I, [_P, _P]),
     'nats_b200_paged_reorder_workspace_bytes': (_SZ, [_I, _I, _I]),
-    'nats_b200_paged_reorder': (_I, [_KV, _P, _P, _SZ, _P, _P]),
+    'nats_b200_paged_reorder': (_I, [_P, _P, _P, _SZ, _P, _P]),
     'nats_b200_decode_place': (_I, [_P, _P, _P, _P, _I, _P, _P, _P, _I, _I, _I, _I, _I, _I, _P]),
 }
 

@@ -18,10 +18,10 @@ constexpr int kRowTile = 16;                     // keys per warp tile
 constexpr int kRowStages = 3;
 constexpr int kRows = 16;                        // query rows of an A fragment
 constexpr int kMaxTickets = 640;                 // blocks of a launch; the workspace begins with as many words, which are zero between calls
-#ifndef NATS_MIN_STRETCH
-#define NATS_MIN_STRETCH 64
-#endif
-constexpr int kMinStretch = NATS_MIN_STRETCH;    // keys of a block's stretch at least
+constexpr int kMinStretch = 64;                  // keys of a block's stretch at least
+// What a unit costs a block besides its keys (draining and filling the ring, joining the warps, partial results), in keys.  us with 0 / 64 / 128 /
+// 256 / 512: 64 sequences of 8 heads 164 / 161 / 161 / 162 / 166, a step of 16 46.1 / 45.8 / 44.9 / 44.3 / 46.8, 4 of 8 23.4 / 22.8 / 21.5 / 21.5 / 22.2.
+constexpr int kUnitCost = 128;
 
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
@@ -80,34 +80,49 @@ __device__ __forceinline__ void join_parts(const PagedAttnParams& p, int s, int 
         if (mr < live) mx = fmaxf(mx, __ldcg(part_of(x) + R * D + 2 * mr));
     s_max[tid] = mx;
     __syncthreads();
-    for (int i = tid; i < n_rows * (D / 4); i += kRowThreads) {
-        const int r = i / (D / 4), d = i % (D / 4) * 4;
-        float4 a = make_float4(0.f, 0.f, 0.f, 0.f);
-        float l = 0.f, mu = -INFINITY;
-        if (r < live) {
+    // four columns of ITEMS rows per thread, AT_ONCE parts of each on their way at a time
+    constexpr int ITEMS = R * D / 4 / kRowThreads, STEP = kRowThreads / (D / 4), AT_ONCE = 4;
+    const int r_first = tid / (D / 4), d = tid % (D / 4) * 4;
+    float4 a[ITEMS];
+    float l[ITEMS], mu[ITEMS];
 #pragma unroll
-            for (int k = 0; k < kRowThreads / R; ++k) mu = fmaxf(mu, s_max[k * R + r]);
-            mu = mu == -INFINITY ? 0.f : mu;
-            constexpr int AT_ONCE = 8;             // parts on their way at a time
-            for (int x0 = first; x0 <= last; x0 += AT_ONCE) {
-                float4 o[AT_ONCE];
-                float2 ml[AT_ONCE];
+    for (int j = 0; j < ITEMS; ++j) {
+        a[j] = make_float4(0.f, 0.f, 0.f, 0.f);
+        l[j] = 0.f;
+        mu[j] = -INFINITY;
 #pragma unroll
-                for (int k = 0; k < AT_ONCE; ++k) {
-                    const float* part = part_of(min(x0 + k, last));
-                    o[k] = __ldcg(reinterpret_cast<const float4*>(part + r * D + d));
-                    ml[k] = __ldcg(reinterpret_cast<const float2*>(part + R * D + 2 * r));
-                }
+        for (int k = 0; k < kRowThreads / R; ++k) mu[j] = fmaxf(mu[j], s_max[k * R + r_first + j * STEP]);
+        if (mu[j] == -INFINITY) mu[j] = 0.f;
+    }
+    for (int x0 = first; x0 <= last; x0 += AT_ONCE) {
+        float4 o[ITEMS][AT_ONCE];
+        float2 ml[ITEMS][AT_ONCE];
 #pragma unroll
-                for (int k = 0; k < AT_ONCE; ++k) {
-                    if (x0 + k > last) break;
-                    const float f = exp2_approx(ml[k].x - mu);
-                    add_scaled(a, o[k], f);
-                    l = fmaf(ml[k].y, f, l);
-                }
+        for (int k = 0; k < AT_ONCE; ++k) {
+            const float* part = part_of(min(x0 + k, last));
+#pragma unroll
+            for (int j = 0; j < ITEMS; ++j) {
+                const int r = r_first + j * STEP;
+                ml[j][k] = make_float2(-INFINITY, 0.f);
+                if (r >= live || x0 + k > last) continue;
+                o[j][k] = __ldcg(reinterpret_cast<const float4*>(part + r * D + d));
+                ml[j][k] = __ldcg(reinterpret_cast<const float2*>(part + R * D + 2 * r));
             }
         }
-        store_o(p, s, h, r0 + r, d, divided(a, l));
+#pragma unroll
+        for (int j = 0; j < ITEMS; ++j)
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) {
+                if (r_first + j * STEP >= live || x0 + k > last) continue;
+                const float f = exp2_approx(ml[j][k].x - mu[j]);
+                add_scaled(a[j], o[j][k], f);
+                l[j] = fmaf(ml[j][k].y, f, l[j]);
+            }
+    }
+#pragma unroll
+    for (int j = 0; j < ITEMS; ++j) {
+        const int r = r_first + j * STEP;
+        if (r < n_rows) store_o(p, s, h, r0 + r, d, divided(a[j], l[j]));
     }
 }
 
@@ -146,7 +161,7 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 && D == 64 ? 4 : 2) paged
     const int per = (n_rows_all + kRowThreads - 1) / kRowThreads;
     auto row_pages = [&](int row) {
         const int n = row_tokens(p, row / kv.H), live = min((n * p.G + R - 1) / R, p.row_tiles);
-        return live * unit_pages(kv, row, true) + p.row_tiles - live;
+        return live * (unit_pages(kv, row, true) + p.front_pages) + p.row_tiles - live;
     };
     int sum = 0;
     for (int i = 0; i < per; ++i) {
@@ -184,10 +199,10 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 && D == 64 ? 4 : 2) paged
         int unit_begin = row_begin;
         for (int rt = 0; rt < p.row_tiles && line < end; ++rt) {
             const int r0 = rt * R, n_rows = min(R, p.N * p.G - r0), live = min(n_rows, n * p.G - r0);   // rows of the unit, those of real tokens
-            const int pages = live > 0 ? max(n_pages, 1) : 1, unit_end = unit_begin + pages;
+            const int front = live > 0 ? p.front_pages : 0, pages = live > 0 ? max(n_pages, 1) : 1, unit_end = unit_begin + front + pages;
             if (unit_end <= line) { unit_begin = unit_end; continue; }
             const int first_block = unit_begin / chunk, last_block = (unit_end - 1) / chunk;
-            const int e_first = line - unit_begin, e_end = min(min(end, unit_end) - unit_begin, n_pages);
+            const int e_first = max(line - unit_begin - front, 0), e_end = min(min(end, unit_end) - unit_begin - front, n_pages);
             if (live <= 0) {
                 for (int i = tid; i < n_rows * (D / 4); i += kRowThreads) store_o(p, s, h, r0 + i / (D / 4), i % (D / 4) * 4, make_float4(0.f, 0.f, 0.f, 0.f));
                 line = unit_end;
@@ -401,9 +416,12 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 && D == 64 ? 4 : 2) paged
             if (!alone) {
                 if (tid == 0) {
                     __threadfence();
-                    sh.last = atomicAdd(&p.tickets[first_block], 1) == last_block - first_block;
-                    if (sh.last) p.tickets[first_block] = 0;
-                    __threadfence();
+                    const bool last = atomicAdd(&p.tickets[first_block], 1) == last_block - first_block;
+                    if (last) {
+                        p.tickets[first_block] = 0;
+                        __threadfence();
+                    }
+                    sh.last = last;
                 }
                 __syncthreads();
                 if (sh.last) join_parts<D, R>(p, s, h, r0, n_rows, live, unit_begin, chunk, first_block, last_block, &s_m[0][0]);
@@ -417,7 +435,7 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 && D == 64 ? 4 : 2) paged
 }
 
 // ---- host side ------------------------------------------------------------------------------------
-struct AttnPlan { bool tiles; int mt, row_tiles, split_pages; long long line; size_t counts, partials, bytes; };
+struct AttnPlan { bool tiles; int mt, row_tiles, split_pages, front_pages; long long line; size_t counts, partials, bytes; };
 static AttnPlan attn_plan(int S, int H, int G, int N, int D, int P, int M) {
     AttnPlan a = {};
     // Query rows up to which paged_rows_kernel is faster.  us, rows / tiles: head_dim 64 32 rows (16 sequences of 4 heads, 2200 keys each) 24.6 / 29.1,
@@ -434,7 +452,8 @@ static AttnPlan attn_plan(int S, int H, int G, int N, int D, int P, int M) {
         a.mt = D == 64 && (long long)N * G > kRows ? 2 : 1;
         a.row_tiles = (int)(((long long)N * G + 16 * a.mt - 1) / (16 * a.mt));
         a.split_pages = max(1, kMinStretch / P);
-        a.line = (long long)S * H * a.row_tiles * max(M, 1);
+        a.front_pages = cdiv(kUnitCost, P);
+        a.line = (long long)S * H * a.row_tiles * (max(M, 1) + a.front_pages);
         a.partials = a.counts;
         a.bytes = a.partials + (size_t)kMaxTickets * 2 * 16 * a.mt * (D + 2) * 4;
     }
@@ -481,32 +500,32 @@ NATS_EXPORT size_t nats_b200_paged_attention_workspace_bytes(int slots, int n_he
     return attn_plan(slots, n_kv_heads, n_heads / n_kv_heads, N, head_dim, page_size, max_entries).bytes;
 }
 
-NATS_EXPORT int nats_b200_paged_attention(const NatsPagedKV* kv, const void* d_q, long long q_slot_stride, long long q_head_stride,
-                                          long long q_token_stride, void* d_o, long long o_slot_stride, long long o_head_stride,
-                                          long long o_token_stride, int o_f32, const int32_t* d_n_new, int n_heads, int N,
-                                          float sm_scale, void* d_workspace, size_t workspace_bytes, int32_t* d_status, void* stream) {
-    PagedAttnParams p;
+NATS_EXPORT int nats_b200_paged_attention(const NatsPagedKV* kv, const NatsPagedAttention* args, void* stream) {
+    PagedAttnParams p = {};
     if (const int e = paged_kv(kv, p.kv)) return e;
-    NATS_CHECK_ARG(d_q && d_o && d_workspace && d_status, "null pointer");
+    NATS_CHECK_ARG(args && args->d_q && args->d_o && args->d_workspace && args->d_status, "null pointer");
+    const int N = args->N, n_heads = args->n_heads;
     NATS_CHECK_ARG(n_heads > 0 && n_heads % p.kv.H == 0, "%d query heads over %d kv-heads", n_heads, p.kv.H);
     NATS_CHECK_ARG(N > 0 && N <= (1 << 24), "bad size N=%d", N);
-    NATS_CHECK_ARG(sm_scale > 0.f, "the scale must be positive");
-    NATS_CHECK_ARG(((uintptr_t)d_q | (uintptr_t)d_o | (uintptr_t)d_workspace) % 16 == 0, "pointers must be 16-byte aligned");
-    NATS_CHECK_ARG((q_slot_stride | q_head_stride | q_token_stride | o_slot_stride | o_head_stride | o_token_stride) % 8 == 0,
-                   "strides must keep 16-byte alignment");
-    const int G = n_heads / p.kv.H;
-    const AttnPlan a = attn_plan(p.kv.S, p.kv.H, G, N, p.kv.D, p.kv.P, p.kv.M);
-    if (workspace_bytes < a.bytes) return fail(NATS_ERR_WORKSPACE, "paged attention workspace: %zu bytes given, %zu needed", workspace_bytes, a.bytes);
-    NATS_CHECK_ARG(a.line < (1ll << 31), "%d new tokens of %d heads per kv-head are too many", N, G);
-    p.q = (const __nv_bfloat16*)d_q; p.q_slot = q_slot_stride; p.q_head = q_head_stride; p.q_token = q_token_stride;
-    p.o = d_o; p.o_slot = o_slot_stride; p.o_head = o_head_stride; p.o_token = o_token_stride; p.o_f32 = o_f32;
-    p.n_new = d_n_new; p.N = N; p.G = G; p.split_pages = a.split_pages; p.row_tiles = a.row_tiles;
-    p.scale_log2 = sm_scale * 1.4426950408889634f;
-    p.tickets = (int32_t*)d_workspace;
-    p.counts = (int32_t*)((uint8_t*)d_workspace + a.counts);
-    p.partials = (float*)((uint8_t*)d_workspace + a.partials);
-    p.status = d_status;
-    if (a.tiles) return launch_paged_tiles(p, (cudaStream_t)stream);
-    if (p.kv.D == 64) return a.mt == 1 ? launch_rows<64, 1>(p, (cudaStream_t)stream) : launch_rows<64, 2>(p, (cudaStream_t)stream);
-    return launch_rows<128, 1>(p, (cudaStream_t)stream);
+    NATS_CHECK_ARG(args->sm_scale > 0.f, "the scale must be positive");
+    NATS_CHECK_ARG(((uintptr_t)args->d_q | (uintptr_t)args->d_o | (uintptr_t)args->d_workspace) % 16 == 0, "pointers must be 16-byte aligned");
+    NATS_CHECK_ARG((args->q_slot_stride | args->q_head_stride | args->q_token_stride | args->o_slot_stride | args->o_head_stride |
+                    args->o_token_stride) % 8 == 0, "strides must keep 16-byte alignment");
+    p.G = n_heads / p.kv.H;
+    const AttnPlan a = attn_plan(p.kv.S, p.kv.H, p.G, N, p.kv.D, p.kv.P, p.kv.M);
+    if (args->workspace_bytes < a.bytes) return fail(NATS_ERR_WORKSPACE, "paged attention workspace: %zu bytes given, %zu needed", args->workspace_bytes, a.bytes);
+    NATS_CHECK_ARG(a.line < (1ll << 31), "%d new tokens of %d heads per kv-head are too many", N, p.G);
+    p.q = (const __nv_bfloat16*)args->d_q; p.q_slot = args->q_slot_stride; p.q_head = args->q_head_stride; p.q_token = args->q_token_stride;
+    p.o = args->d_o; p.o_slot = args->o_slot_stride; p.o_head = args->o_head_stride; p.o_token = args->o_token_stride; p.o_f32 = args->o_f32;
+    p.n_new = args->d_n_new; p.N = N; p.split_pages = a.split_pages; p.front_pages = a.front_pages; p.row_tiles = a.row_tiles;
+    p.scale_log2 = args->sm_scale * 1.4426950408889634f;
+    uint8_t* ws = (uint8_t*)args->d_workspace;
+    p.tickets = (int32_t*)ws;
+    p.counts = (int32_t*)(ws + a.counts);
+    p.partials = (float*)(ws + a.partials);
+    p.status = args->d_status;
+    const cudaStream_t st = (cudaStream_t)stream;
+    if (a.tiles) return launch_paged_tiles(p, st);
+    if (p.kv.D == 64) return a.mt == 1 ? launch_rows<64, 1>(p, st) : launch_rows<64, 2>(p, st);
+    return launch_rows<128, 1>(p, st);
 }

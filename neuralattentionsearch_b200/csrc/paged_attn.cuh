@@ -14,6 +14,7 @@ struct PagedAttnParams {
     const int32_t* n_new;                        // [S] or nullptr: N everywhere
     int N, G;
     int split_pages;                             // pages of a block's stretch at least (rows kernel)
+    int front_pages;                             // what a unit costs besides its pages, in pages (rows kernel)
     int row_tiles;                               // tiles of query rows per (slot, kv-head)
     float scale_log2;
     int32_t* tickets;

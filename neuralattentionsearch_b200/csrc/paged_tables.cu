@@ -529,34 +529,31 @@ NATS_EXPORT size_t nats_b200_paged_append_workspace_bytes(int slots, int n_kv_he
     return 256 + align_up(rows * 4, 256) + align_up(rows * append_chunks(N, page_size) * 4, 256);
 }
 
-NATS_EXPORT int nats_b200_paged_append(const NatsPagedKV* kv, const void* d_k, const void* d_v, long long k_slot_stride, long long k_head_stride,
-                                       long long k_token_stride, long long v_slot_stride, long long v_head_stride, long long v_token_stride,
-                                       int f32, const uint8_t* d_roles, int n_roles, const int32_t* d_n_new, int N, int SW, int skip_hidden,
-                                       void* d_workspace, size_t workspace_bytes, int32_t* d_status, void* stream) {
+NATS_EXPORT int nats_b200_paged_append(const NatsPagedKV* kv, const NatsPagedAppend* a, void* stream) {
     AppendParams p;
     if (const int e = paged_kv(kv, p.kv)) return e;
-    NATS_CHECK_ARG(d_k && d_v && d_workspace && d_status && (d_roles || n_roles == 0), "null pointer");
-    NATS_CHECK_ARG(N > 0 && N <= (1 << 24) && n_roles >= 0, "bad sizes N=%d n_roles=%d", N, n_roles);
+    NATS_CHECK_ARG(a && a->d_k && a->d_v && a->d_workspace && a->d_status && (a->d_roles || a->n_roles == 0), "null pointer");
+    const int N = a->N, SW = a->SW, step = a->f32 ? 4 : 8;                 // step: elements of 16 bytes
+    NATS_CHECK_ARG(N > 0 && N <= (1 << 24) && a->n_roles >= 0, "bad sizes N=%d n_roles=%d", N, a->n_roles);
     NATS_CHECK_ARG(SW > 0 && SW % p.kv.P == 0, "sliding window %d must be a positive multiple of the page size %d", SW, p.kv.P);
-    NATS_CHECK_ARG(((uintptr_t)d_k | (uintptr_t)d_v) % 16 == 0, "K and V must be 16-byte aligned");
-    const int step = f32 ? 4 : 8;                // elements of 16 bytes
-    NATS_CHECK_ARG((k_slot_stride | k_head_stride | k_token_stride | v_slot_stride | v_head_stride | v_token_stride) % step == 0,
+    NATS_CHECK_ARG(((uintptr_t)a->d_k | (uintptr_t)a->d_v) % 16 == 0, "K and V must be 16-byte aligned");
+    NATS_CHECK_ARG((a->k_slot_stride | a->k_head_stride | a->k_token_stride | a->v_slot_stride | a->v_head_stride | a->v_token_stride) % step == 0,
                    "strides of K and V must keep 16-byte alignment");
     const size_t need = nats_b200_paged_append_workspace_bytes(p.kv.S, p.kv.H, N, p.kv.P), rows = (size_t)p.kv.S * p.kv.H;
-    if (workspace_bytes < need) return fail(NATS_ERR_WORKSPACE, "paged append workspace: %zu bytes given, %zu needed", workspace_bytes, need);
-    p.k = (const uint8_t*)d_k; p.v = (const uint8_t*)d_v; p.f32 = f32;
-    p.k_slot = k_slot_stride; p.k_head = k_head_stride; p.k_token = k_token_stride;
-    p.v_slot = v_slot_stride; p.v_head = v_head_stride; p.v_token = v_token_stride;
-    p.roles = d_roles; p.n_roles = n_roles; p.n_new = d_n_new; p.N = N; p.SW = SW; p.n_chunks = append_chunks(N, p.kv.P);
+    if (a->workspace_bytes < need) return fail(NATS_ERR_WORKSPACE, "paged append workspace: %zu bytes given, %zu needed", a->workspace_bytes, need);
+    p.k = (const uint8_t*)a->d_k; p.v = (const uint8_t*)a->d_v; p.f32 = a->f32;
+    p.k_slot = a->k_slot_stride; p.k_head = a->k_head_stride; p.k_token = a->k_token_stride;
+    p.v_slot = a->v_slot_stride; p.v_head = a->v_head_stride; p.v_token = a->v_token_stride;
+    p.roles = a->d_roles; p.n_roles = a->n_roles; p.n_new = a->d_n_new; p.N = N; p.SW = SW; p.n_chunks = append_chunks(N, p.kv.P);
     p.copy_here = N <= kCopyTokens;
-    uint8_t* ws = (uint8_t*)d_workspace;
+    uint8_t* ws = (uint8_t*)a->d_workspace;
     p.ticket = (int32_t*)ws;
     p.counts = (int32_t*)(ws + 256);
     p.map = (int32_t*)(ws + 256 + align_up(rows * 4, 256));
-    p.status = d_status;
+    p.status = a->d_status;
     const cudaStream_t st = (cudaStream_t)stream;
-    if (skip_hidden) NATS_CHECK_CUDA(launch_behind(paged_count_kernel, (unsigned)rows, 0, st, p));
-    NATS_CHECK_CUDA(launch_behind(skip_hidden ? paged_append_kernel<true> : paged_append_kernel<false>, (unsigned)rows, 0, st, p));
+    if (a->skip_hidden) NATS_CHECK_CUDA(launch_behind(paged_count_kernel, (unsigned)rows, 0, st, p));
+    NATS_CHECK_CUDA(launch_behind(a->skip_hidden ? paged_append_kernel<true> : paged_append_kernel<false>, (unsigned)rows, 0, st, p));
     if (!p.copy_here) NATS_CHECK_CUDA(launch_behind(paged_copy_kernel, dim3(cdiv(N, kCopyTokens), (unsigned)rows), 0, st, p));
     return NATS_OK;
 }

@@ -667,10 +667,11 @@ class PagedKV:
         S, H, M, four = entries.shape
         if pages_k.dtype is not torch.bfloat16 or pages_v.dtype is not torch.bfloat16 or pages_v.shape != pages_k.shape:
             raise ValueError('pages_k and pages_v must be bf16 [pages, page_size, head_dim]')
-        for t, shape, name in ((refs, (n,), 'refs'), (free_bits, ((n + 31) // 32,), 'free_bits'), (entries, (S, H, M, 4), 'entries'),
-                               (n_pages, (S, H), 'n_pages'), (length, (S,), 'length')):
-            if t.dtype is not torch.int32 or t.shape != shape:
-                raise ValueError(f'{name} must be int32 {list(shape)}, got {t.dtype} {list(t.shape)}')
+        i32 = torch.int32
+        if refs.dtype is not i32 or free_bits.dtype is not i32 or entries.dtype is not i32 or n_pages.dtype is not i32 or length.dtype is not i32 or \
+                refs.shape != (n,) or free_bits.shape != ((n + 31) // 32,) or four != 4 or n_pages.shape != (S, H) or length.shape != (S,):
+            raise ValueError(f'refs, free_bits, entries, n_pages and length must be int32 [{n}], [{(n + 31) // 32}], [S,Hkv,M,4], [{S},{H}] and [{S}], got ' +
+                             ', '.join(f'{t.dtype} {list(t.shape)}' for t in tensors[2:]))
         self.index = index = pages_k.get_device()
         for t in tensors:
             if t.get_device() != index or index < 0:
@@ -684,8 +685,8 @@ class PagedKV:
         self.pages_k, self.pages_v, self.refs, self.free_bits, self.entries, self.n_pages, self.length = tensors
         self.num_pages, self.page_size, self.head_dim, self.slots, self.n_kv_heads, self.max_entries = n, P, D, S, H, M
         self.scratch: dict | None = None
-        self._c = _lib.NatsPagedKV(pages_k.data_ptr(), pages_v.data_ptr(), refs.data_ptr(), free_bits.data_ptr(), entries.data_ptr(),
-                                   n_pages.data_ptr(), length.data_ptr(), n, P, D, S, H, M)
+        self._c = _lib.PAGED_KV(pages_k.data_ptr(), pages_v.data_ptr(), refs.data_ptr(), free_bits.data_ptr(), entries.data_ptr(),
+                                n_pages.data_ptr(), length.data_ptr(), n, P, D, S, H, M)
 
     @property
     def device(self) -> torch.device:
@@ -740,9 +741,9 @@ def _strided_ok(t: torch.Tensor) -> bool:
     return d == 1 and t.data_ptr() % 16 == 0 and a % step == 0 and b % step == 0 and c % step == 0
 
 
-def _check_n_new(kv: PagedKV, n_new: torch.Tensor | None) -> int | None:
+def _check_n_new(kv: PagedKV, n_new: torch.Tensor | None) -> int:
     if n_new is None:
-        return None
+        return 0
     if n_new.dtype is not torch.int32 or n_new.shape != (kv.slots,) or n_new.get_device() != kv.index or not n_new.is_contiguous():
         raise ValueError(f'n_new must be int32 [{kv.slots}] on {kv.device}')
     return n_new.data_ptr()
@@ -786,7 +787,7 @@ def _check_roles(kv: PagedKV, roles: torch.Tensor | None) -> torch.Tensor | None
 
 
 def _paged_append(kv, k, v, roles, lens, N, sliding_window, skip_hidden):
-    n_roles, roles_ptr = (0, None) if roles is None else (roles.shape[2], roles.data_ptr())
+    n_roles, roles_ptr = (0, 0) if roles is None else (roles.shape[2], roles.data_ptr())
     if k.dtype is not v.dtype or (k.dtype is not torch.bfloat16 and k.dtype is not torch.float32):
         k, v = k.to(torch.bfloat16), v.to(torch.bfloat16)
     if not _strided_ok(k):
@@ -797,8 +798,9 @@ def _paged_append(kv, k, v, roles, lens, N, sliding_window, skip_hidden):
     ws = _paged_scratch(kv, 'append', stream, kv.slots, kv.n_kv_heads, N, kv.page_size)
     ka, kb, kc, _ = k.stride()
     va, vb, vc, _ = v.stride()
-    _lib.call('nats_b200_paged_append', kv._c, k.data_ptr(), v.data_ptr(), ka, kb, kc, va, vb, vc, k.dtype is torch.float32, roles_ptr, n_roles,
-              lens, N, sliding_window, skip_hidden, ws.data_ptr(), ws.numel(), _status_ptr(kv.index), stream)
+    _lib.call('nats_b200_paged_append', kv._c,
+              _lib.PAGED_APPEND(k.data_ptr(), v.data_ptr(), ka, kb, kc, va, vb, vc, roles_ptr, lens, ws.data_ptr(), ws.numel(), _status_ptr(kv.index),
+                                k.dtype is torch.float32, n_roles, N, sliding_window, skip_hidden), stream)
 
 
 def paged_attention(kv: PagedKV, q: torch.Tensor, sm_scale: float | None = None, n_new: torch.Tensor | None = None,
@@ -828,9 +830,10 @@ def _paged_attention(kv, q, scale, lens, token_major, o):
     f32 = q.dtype is torch.float32                       # fp32 callers: the kernel writes fp32 itself
     dtype = torch.float32 if f32 else torch.bfloat16
     if o is None:
-        o = torch.empty((S, N, Hq, D) if token_major else (S, Hq, N, D), dtype=dtype, device=kv.device)
         if token_major:
-            o = o.transpose(1, 2)
+            o = torch.empty(S, N, Hq, D, dtype=dtype, device=kv.device).transpose(1, 2)
+        else:
+            o = torch.empty_like(q, dtype=dtype, memory_format=torch.contiguous_format)
     if N > 0:
         qb = q if q.dtype is torch.bfloat16 else q.to(torch.bfloat16)
         if not _strided_ok(qb) or 0 in qb.stride():
@@ -839,8 +842,9 @@ def _paged_attention(kv, q, scale, lens, token_major, o):
         ws = _paged_scratch(kv, 'attention', stream, S, Hq, kv.n_kv_heads, N, D, kv.page_size, kv.max_entries)
         qs, qh, qt, _ = qb.stride()
         os, oh, ot, _ = o.stride()
-        _lib.call('nats_b200_paged_attention', kv._c, qb.data_ptr(), qs, qh, qt, o.data_ptr(), os, oh, ot, f32, lens, Hq, N, scale,
-                  ws.data_ptr(), ws.numel(), _status_ptr(kv.index), stream)
+        _lib.call('nats_b200_paged_attention', kv._c,
+                  _lib.PAGED_ATTENTION(qb.data_ptr(), o.data_ptr(), qs, qh, qt, os, oh, ot, lens, ws.data_ptr(), ws.numel(), _status_ptr(kv.index),
+                                       scale, f32, Hq, N), stream)
     return o if o.dtype is q.dtype else o.to(q.dtype)
 
 

@@ -1,6 +1,4 @@
 """The paged cache without a GPU: its model, its host-side checks, its C entry points' refusals."""
-import ctypes
-
 import numpy as np
 import pytest
 import torch
@@ -69,16 +67,17 @@ def test_c_entry_points_refuse_bad_arguments():
         a = dict(d_pages_k=one, d_pages_v=one, d_refs=one, d_free_bits=one, d_entries=one, d_n_pages=one, d_length=one, num_pages=10, page_size=16,
                  head_dim=64, slots=2, n_kv_heads=2, max_entries=8)
         a.update(more)
-        return _lib.NatsPagedKV(**a)
-    for more, rc, text in ((dict(d_refs=None), 1, b'null'), (dict(d_pages_k=264), 1, b'aligned'), (dict(num_pages=0), 1, b'pages'),
+        return _lib.PAGED_KV(*a.values())
+    for more, rc, text in ((dict(d_refs=0), 1, b'null'), (dict(d_pages_k=264), 1, b'aligned'), (dict(num_pages=0), 1, b'pages'),
                            (dict(num_pages=(1 << 24) + 1), 1, b'pages'), (dict(page_size=24), 1, b'page size'), (dict(head_dim=256), 2, b'head_dim'),
                            (dict(slots=0), 1, b'table'), (dict(slots=5000), 1, b'table'), (dict(slots=4000, n_kv_heads=20), 1, b'rows'), (dict(max_entries=0), 1, b'table')):
         for call in (lambda: lib.nats_b200_paged_evict(kv(**more), None), lambda: lib.nats_b200_paged_reorder(kv(**more), one, one, 1 << 30, one, None)):
             assert call() == rc and text in lib.nats_b200_last_error(), more
 
     def append(k=one, v=one, strides=(64,) * 6, f32=0, roles=one, n_roles=1, N=4, SW=16, ws=one, nbytes=1 << 30, status=one):
-        return lib.nats_b200_paged_append(kv(), k, v, *strides, f32, roles, n_roles, None, N, SW, 0, ws, nbytes, status, None)
-    for rc, text, call in ((1, b'null', lambda: append(k=None)), (1, b'null', lambda: append(roles=None)), (1, b'null', lambda: append(status=None)),
+        return lib.nats_b200_paged_append(kv(), _lib.PAGED_APPEND(k, v, *strides, roles, 0, ws, nbytes, status, f32, n_roles, N, SW, 0), None)
+    assert lib.nats_b200_paged_append(kv(), None, None) == 1 and lib.nats_b200_paged_attention(kv(), None, None) == 1
+    for rc, text, call in ((1, b'null', lambda: append(k=0)), (1, b'null', lambda: append(roles=0)), (1, b'null', lambda: append(status=0)),
                            (1, b'sizes', lambda: append(N=0)), (1, b'sizes', lambda: append(n_roles=-1)), (1, b'multiple', lambda: append(SW=24)),
                            (1, b'multiple', lambda: append(SW=0)), (1, b'aligned', lambda: append(k=264)), (1, b'strides', lambda: append(strides=(64, 4, 64, 64, 64, 64))),
                            (4, b'workspace', lambda: append(nbytes=100))):
@@ -86,8 +85,8 @@ def test_c_entry_points_refuse_bad_arguments():
     assert lib.nats_b200_paged_append_count(kv(), None, 1, None, 4, 16, one, None) == 1
 
     def attend(q=one, strides=(64,) * 6, heads=4, N=2, scale=0.1, nbytes=1 << 40, status=one):
-        return lib.nats_b200_paged_attention(kv(), q, *strides[:3], one, *strides[3:], 0, None, heads, N, scale, one, nbytes, status, None)
-    for rc, text, call in ((1, b'null', lambda: attend(q=None)), (1, b'query heads', lambda: attend(heads=3)), (1, b'size', lambda: attend(N=0)),
+        return lib.nats_b200_paged_attention(kv(), _lib.PAGED_ATTENTION(q, one, *strides, 0, one, nbytes, status, scale, 0, heads, N), None)
+    for rc, text, call in ((1, b'null', lambda: attend(q=0)), (1, b'query heads', lambda: attend(heads=3)), (1, b'size', lambda: attend(N=0)),
                            (1, b'scale', lambda: attend(scale=0.0)), (1, b'scale', lambda: attend(scale=float('nan'))),
                            (1, b'aligned', lambda: attend(q=264)), (1, b'strides', lambda: attend(strides=(64, 64, 64, 64, 64, 4))), (4, b'workspace', lambda: attend(nbytes=4096))):
         assert call() == rc and text in lib.nats_b200_last_error()
@@ -98,4 +97,3 @@ def test_c_entry_points_refuse_bad_arguments():
         assert fn(*args) > 0
         assert fn(0, *args[1:]) == 0
     assert lib.nats_b200_paged_attention_workspace_bytes(2, 3, 2, 4, 64, 16, 8) == 0
-    assert ctypes.sizeof(_lib.NatsPagedKV) == 7 * 8 + 6 * 4
