@@ -67,32 +67,20 @@ __device__ __forceinline__ float4 divided(const float4& a, float l) {      // a 
     return l != 0.f ? make_float4(a.x / l, a.y / l, a.z / l, a.w / l) : make_float4(0.f, 0.f, 0.f, 0.f);
 }
 
-// Joins the parts of a unit: s_max has room for kRowThreads floats
+// Joins the parts of a unit: four columns of ITEMS rows per thread, AT_ONCE parts of each on their way at a time
 template <int D, int R>
 __device__ __forceinline__ void join_parts(const PagedAttnParams& p, int s, int h, int r0, int n_rows, int live, int unit_begin, int chunk,
-                                           int first, int last, float* s_max) {
-    const int tid = threadIdx.x;
-    auto part_of = [&](int x) { return p.partials + ((size_t)x * 2 + (unit_begin < x * chunk ? 0 : 1)) * R * (D + 2); };
-    // maxima of the rows over the parts: kRowThreads / R threads per row
-    const int mr = tid % R;
-    float mx = -INFINITY;
-    for (int x = first + tid / R; x <= last; x += kRowThreads / R)
-        if (mr < live) mx = fmaxf(mx, __ldcg(part_of(x) + R * D + 2 * mr));
-    s_max[tid] = mx;
-    __syncthreads();
-    // four columns of ITEMS rows per thread, AT_ONCE parts of each on their way at a time
+                                           int first, int last) {
     constexpr int ITEMS = R * D / 4 / kRowThreads, STEP = kRowThreads / (D / 4), AT_ONCE = 4;
-    const int r_first = tid / (D / 4), d = tid % (D / 4) * 4;
+    const int r_first = threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+    auto part_of = [&](int x) { return p.partials + ((size_t)x * 2 + (unit_begin < x * chunk ? 0 : 1)) * R * (D + 2); };
     float4 a[ITEMS];
-    float l[ITEMS], mu[ITEMS];
+    float l[ITEMS], m[ITEMS];
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j) {
         a[j] = make_float4(0.f, 0.f, 0.f, 0.f);
         l[j] = 0.f;
-        mu[j] = -INFINITY;
-#pragma unroll
-        for (int k = 0; k < kRowThreads / R; ++k) mu[j] = fmaxf(mu[j], s_max[k * R + r_first + j * STEP]);
-        if (mu[j] == -INFINITY) mu[j] = 0.f;
+        m[j] = -INFINITY;
     }
     for (int x0 = first; x0 <= last; x0 += AT_ONCE) {
         float4 o[ITEMS][AT_ONCE];
@@ -110,14 +98,23 @@ __device__ __forceinline__ void join_parts(const PagedAttnParams& p, int s, int 
             }
         }
 #pragma unroll
-        for (int j = 0; j < ITEMS; ++j)
+        for (int j = 0; j < ITEMS; ++j) {
+            if (r_first + j * STEP >= live) continue;
+            float m_new = m[j];
+#pragma unroll
+            for (int k = 0; k < AT_ONCE; ++k) m_new = fmaxf(m_new, ml[j][k].x);
+            const float mu = m_new == -INFINITY ? 0.f : m_new, old = exp2_approx(m[j] - mu);
+            a[j] = make_float4(a[j].x * old, a[j].y * old, a[j].z * old, a[j].w * old);
+            l[j] *= old;
+            m[j] = m_new;
 #pragma unroll
             for (int k = 0; k < AT_ONCE; ++k) {
-                if (r_first + j * STEP >= live || x0 + k > last) continue;
-                const float f = exp2_approx(ml[j][k].x - mu[j]);
+                if (x0 + k > last) break;
+                const float f = exp2_approx(ml[j][k].x - mu);
                 add_scaled(a[j], o[j][k], f);
                 l[j] = fmaf(ml[j][k].y, f, l[j]);
             }
+        }
     }
 #pragma unroll
     for (int j = 0; j < ITEMS; ++j) {
@@ -424,8 +421,8 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 && D == 64 ? 4 : 2) paged
                     sh.last = last;
                 }
                 __syncthreads();
-                if (sh.last) join_parts<D, R>(p, s, h, r0, n_rows, live, unit_begin, chunk, first_block, last_block, &s_m[0][0]);
-                __syncthreads();                                                    // sh.last and the scratch have been read
+                if (sh.last) join_parts<D, R>(p, s, h, r0, n_rows, live, unit_begin, chunk, first_block, last_block);
+                __syncthreads();                                                    // sh.last has been read
             }
             line = min(end, unit_end);
             unit_begin = unit_end;
