@@ -38,7 +38,8 @@ struct PtHeader {
     int skip;                                    // visible pages of the unit in front of them
     int q0, n;                                   // position of the slot's first new token, number of new tokens
     int part;                                    // -1: the whole unit; else where its partial result goes, see PtPart
-    int pad[3];
+    int n_pages;                                 // of the row
+    int pad[2];
 };
 
 // A CTA shares at most two units with others: one that began before its stretch (part 0), one that goes on behind it (part 1).
@@ -241,13 +242,18 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             const int slot = ic & 1, use = ic >> 1;
             if (use > 0) ok = util_wait<kRelaxNs>(smem_u32(&sm.bar_list_empty[slot]), (use - 1) & 1, abort_flag, p.status, kPtErr + kErrList);
             if (!ok) break;
-            const bool have = line < end;
+            unsigned m = 0u;                             // the next unit with a length
+            if (line < end) {
+                while (unit < units && (m = __ballot_sync(0xffffffffu, length_of(unit + lane) > 0)) == 0u) unit += 32;
+            }
+            const bool have = m != 0u;
             PtHeader hd;
             hd.valid = have;
             if (have) {
-                for (unsigned m; (m = __ballot_sync(0xffffffffu, length_of(unit + lane) > 0)) == 0u || (unit += __ffs(m) - 1, false);) unit += 32;
+                unit += __ffs(m) - 1;
                 hd.row = unit / pairs;
                 hd.tile = 2 * (unit - hd.row * pairs);
+                hd.n_pages = min(max(kv.n_pages[hd.row], 0), kv.M);
                 const PtUnit u = pt_unit(p, hd.row, hd.tile);
                 hd.n = u.n;
                 hd.q0 = u.q0;
@@ -305,7 +311,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
             const PtHeader hd = sm.item[slot];
             if (!hd.valid) break;
             const int4* entries = kv.entries + (size_t)hd.row * kv.M;
-            const int n_entries = hd.n_kv > 0 ? min(max(kv.n_pages[hd.row], 0), kv.M) : 0;
+            const int n_entries = hd.n_kv > 0 ? hd.n_pages : 0;
             const int q_lo = hd.q0 + hd.tile * TT, q_hi = hd.q0 + min(hd.tile * TT + 2 * TT, hd.n) - 1, end = hd.q0 + hd.n;
             // a window of 32 entries, one per lane, the next one on its way; seen: those of the window that are visible and not used up
             int base = 0;
