@@ -444,7 +444,7 @@ static AttnPlan attn_plan(int S, int H, int G, int N, int D, int P, int M) {
     static_assert(kMaxTickets * 4 <= 4096, "the front of the workspace holds the tickets");
     if (a.tiles) {
         a.row_tiles = cdiv(N, tile_tokens(G));
-        a.line = (long long)S * H * cdiv(a.row_tiles, 2) * ((long long)M * P / kTile + 1);
+        a.line = (long long)S * H * cdiv(a.row_tiles, 2) * ((long long)M * P / kTile + 8);
         a.partials = a.counts + paged_tile_count_bytes(S, H, a.row_tiles);
         a.bytes = a.partials + paged_tile_result_bytes(D);
     } else {

@@ -49,6 +49,9 @@ constexpr int kPtRows = 256;
 template <int D>
 struct PtResult { float4 o[D / 4][kPtRows]; float2 ml[kPtRows]; };
 constexpr int kPtMaxCtas = 160;
+// What a unit costs a CTA besides its tiles (Q, the way to its first page, O written out), in tiles: CTAs of three units took 154 us, of eight 177.  us
+// with 0 / 1 / 2 / 3 / 4: 1500 tokens of 4 sequences 193 / 188 / 183 / 183 / 183, 64 tokens over 26k keys 48.5 / 47.3 / 45.9 / 46.0 / 47.0.
+constexpr int kPtUnitTiles = 2;
 
 struct PtMeta {
     int start[8], limit[8];                      // of every 16 keys: position of the first one, last query position that may see them
@@ -210,29 +213,26 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     if (warp == 3) {
         // =============================== scheduler ===============================
         const int pairs = (p.row_tiles + 1) / 2, units = kv.S * kv.H * pairs;
-        auto length_of = [&](int u) {                    // a unit that sees nothing has zeros to write, one of padding has not
+        // a unit that sees nothing has zeros to write, one of padding has no length
+        auto length_of = [&](int u) {
             const int c = u < units ? p.counts[u] : -1;
-            return c < 0 ? 0 : max(c, 1);
+            return c < 0 ? 0 : c + kPtUnitTiles;
         };
+        // every lane sums up its share of the units; the one whose share holds the beginning of the stretch looks for the unit there
+        const int per = (units + 31) / 32;
         int sum = 0;
 #pragma unroll 4
-        for (int u = lane; u < units; u += 32) sum += length_of(u);
-        sum = __reduce_add_sync(0xffffffffu, sum);
-        const int chunk = (sum + (int)gridDim.x - 1) / (int)gridDim.x;
-        const int begin = min((int)blockIdx.x * chunk, sum), end = min(begin + chunk, sum);
-        // the unit at the beginning of the stretch, and where it begins
-        int unit = 0, unit_begin = 0;
-        for (; begin < end; unit += 32) {
-            const int incl = warp_incl_scan(length_of(unit + lane), lane);
-            const unsigned behind = __ballot_sync(0xffffffffu, unit_begin + incl > begin);
-            if (behind != 0u) {
-                const int i = __ffs(behind) - 1, at = __shfl_sync(0xffffffffu, incl, max(i - 1, 0));
-                unit += i;
-                if (i > 0) unit_begin += at;
-                break;
-            }
-            unit_begin += __shfl_sync(0xffffffffu, incl, 31);
-        }
+        for (int i = 0; i < per; ++i) sum += length_of(lane * per + i);
+        const int incl = warp_incl_scan(sum, lane), total = __shfl_sync(0xffffffffu, incl, 31);
+        const int chunk = max((total + (int)gridDim.x - 1) / (int)gridDim.x, 1);
+        const int begin = min((int)blockIdx.x * chunk, total), end = min(begin + chunk, total);
+        int unit = lane * per, unit_begin = incl - sum;
+        const unsigned holds = __ballot_sync(0xffffffffu, unit_begin <= begin && begin < incl);
+        if (unit_begin <= begin && begin < incl)
+            for (int x; unit_begin + (x = length_of(unit)) <= begin; ++unit) unit_begin += x;
+        const int who = holds ? __ffs(holds) - 1 : 0;
+        unit = __shfl_sync(0xffffffffu, unit, who);
+        unit_begin = __shfl_sync(0xffffffffu, unit_begin, who);
         PtPart shared = {};
         int line = begin;
         bool ok = true;
@@ -258,10 +258,11 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                 hd.n = u.n;
                 hd.q0 = u.q0;
                 hd.ntiles = u.t1 <= u.t0 ? 0 : u.t1 - u.t0 > TT ? 2 : 1;
-                const int tiles = p.counts[unit], unit_end = unit_begin + max(tiles, 1), to = min(end, unit_end);
+                const int unit_end = unit_begin + length_of(unit), to = min(end, unit_end);
+                const int t0 = max(line - unit_begin - kPtUnitTiles, 0);
                 const int first = unit_begin / chunk, last = (unit_end - 1) / chunk;
-                hd.n_kv = tiles > 0 ? to - line : 0;
-                hd.skip = (line - unit_begin) * (kTile / kv.P);
+                hd.n_kv = max(to - unit_begin - kPtUnitTiles - t0, 0);
+                hd.skip = t0 * (kTile / kv.P);
                 hd.part = first == last ? -1 : unit_begin < begin ? 0 : 1;
                 if (hd.part == 1) { shared.split = 1; shared.row = hd.row; shared.tile = hd.tile; shared.last = last; shared.begin = unit_begin; shared.chunk = chunk; }
                 line = to;
@@ -327,8 +328,11 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                 for (int i = 0; i < 4; ++i) { m[i] = __ballot_sync(0xffffffffu, pt_sees(kv, w[i], q_lo, q_hi)); c += __popc(m[i]); }
                 if (c > skip) {
 #pragma unroll
-                    for (int i = 0; i < 3; ++i)
-                        if (c > skip && __popc(m[i]) <= skip) { skip -= __popc(m[i]); base += 32; c = skip + 1; } else break;
+                    for (int i = 0; i < 3; ++i) {
+                        if (__popc(m[i]) > skip) break;
+                        skip -= __popc(m[i]);
+                        base += 32;
+                    }
                     break;
                 }
                 skip -= c;
@@ -696,7 +700,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
 }
 
 // Joins the parts of the units that lie in several stretches: blockIdx.x is the first CTA of such a unit, blockIdx.y 32 of its rows.  A lane
-// per row, 16 columns per warp and pass.
+// per row, eight columns per warp and pass.
 template <int D>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p, int n_ctas) {
     wait_for_launch_before();
@@ -713,19 +717,19 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
     auto result_of = [&](int x) -> const PtResult<D>& { return results[2 * (size_t)x + (part.begin < x * part.chunk ? 0 : 1)]; };
     const int hq = (part.row - s * p.kv.H) * p.G + head;
     const long long at = s * p.o_slot + hq * p.o_head + t * p.o_token;
-    for (int c = warp * 4; c < D / 4; c += 32) {           // four groups of four columns
-        float4 a[4] = {};
+    for (int c = (blockIdx.z * 8 + warp) * 2; c < D / 4; c += 16 * gridDim.z) {     // two groups of four columns
+        float4 a[2] = {};
         float m = -INFINITY, l = 0.f;
-        constexpr int AT_ONCE = 4;                         // parts on their way at a time
+        constexpr int AT_ONCE = 8;                         // parts on their way at a time
         for (int x0 = real ? first : part.last + 1; x0 <= part.last; x0 += AT_ONCE) {
             float2 ml[AT_ONCE];
-            float4 o[AT_ONCE][4];
+            float4 o[AT_ONCE][2];
 #pragma unroll
             for (int k = 0; k < AT_ONCE; ++k) {
                 const PtResult<D>& res = result_of(min(x0 + k, part.last));
                 ml[k] = __ldcg(&res.ml[r]);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) o[k][i] = __ldcg(&res.o[c + i][r]);
+                for (int i = 0; i < 2; ++i) o[k][i] = __ldcg(&res.o[c + i][r]);
             }
             float m_new = m;
 #pragma unroll
@@ -733,14 +737,14 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
             const float mu = m_new == -INFINITY ? 0.f : m_new, old = ex2(m - mu);
             l *= old;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) { a[i].x *= old; a[i].y *= old; a[i].z *= old; a[i].w *= old; }
+            for (int i = 0; i < 2; ++i) { a[i].x *= old; a[i].y *= old; a[i].z *= old; a[i].w *= old; }
 #pragma unroll
             for (int k = 0; k < AT_ONCE; ++k) {
                 if (x0 + k > part.last) break;
                 const float f = ex2(ml[k].x - mu);
                 l = fmaf(ml[k].y, f, l);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
+                for (int i = 0; i < 2; ++i) {
                     a[i].x = fmaf(o[k][i].x, f, a[i].x); a[i].y = fmaf(o[k][i].y, f, a[i].y);
                     a[i].z = fmaf(o[k][i].z, f, a[i].z); a[i].w = fmaf(o[k][i].w, f, a[i].w);
                 }
@@ -749,7 +753,7 @@ __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p
         }
         const float inv = l != 0.f ? 1.f / l : 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
+        for (int i = 0; i < 2; ++i) {
             if (p.o_f32) *reinterpret_cast<float4*>((float*)p.o + at + (c + i) * 4) = make_float4(a[i].x * inv, a[i].y * inv, a[i].z * inv, a[i].w * inv);
             else *reinterpret_cast<uint2*>((__nv_bfloat16*)p.o + at + (c + i) * 4) = make_uint2(pack_bf16(a[i].x * inv, a[i].y * inv), pack_bf16(a[i].z * inv, a[i].w * inv));
         }
@@ -814,7 +818,7 @@ static int launch_tiles(const PagedAttnParams& p, cudaStream_t st) {
     cfg.blockDim = dim3(kPtThreads);
     cfg.dynamicSmemBytes = sizeof(PtSmem<D>);
     NATS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_tile_kernel<D>, map_q, map_k, map_v, p));
-    cfg.gridDim = dim3(ctas, kPtRows / 32);
+    cfg.gridDim = dim3(ctas, kPtRows / 32, D / 64);
     cfg.blockDim = dim3(256);
     cfg.dynamicSmemBytes = 0;
     NATS_CHECK_CUDA(cudaLaunchKernelEx(&cfg, paged_join_kernel<D>, p, ctas));
