@@ -326,6 +326,54 @@ def test_other_streams_and_a_recorded_step():
         t.compare()
 
 
+def test_a_recorded_call_of_many_tokens():
+    t = Pair(S=2, Hkv=2, G=4, P=32, D=64, SW=64, num_pages=300, M=60, seed=7)
+    t.append(500, n_new=[500, 230])
+    k, v, q = t.randn(2, 2, 70, 64), t.randn(2, 2, 70, 64), t.randn(2, 8, 70, 64)
+    n_new = torch.tensor([70, 3], dtype=torch.int32, device=DEV)
+    roles = torch.zeros(2, 2, 4, dtype=torch.uint8, device=DEV)
+    out = torch.empty_like(q)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        t.F.paged_append(t.kv, k, v, roles, 64, n_new=n_new)
+        assert t.F.paged_attention(t.kv, q, n_new=n_new, out=out) is out
+        t.F.paged_evict(t.kv)
+    for lens in ([70, 3], [0, 70], [33, 33]):
+        k.copy_(t.randn(2, 2, 70, 64)); v.copy_(t.randn(2, 2, 70, 64)); q.copy_(t.randn(2, 8, 70, 64))
+        r = t.roles(4)
+        roles.copy_(torch.from_numpy(r)); n_new.copy_(torch.tensor(lens))
+        g.replay()
+        t.model.append(k.double().cpu().numpy(), v.double().cpu().numpy(), r, lens)
+        want, mag = t.model.attention(q.double().cpu().numpy(), lens, 64 ** -0.5)
+        assert (np.abs(out.double().cpu().numpy() - want) <= (2.0 ** -8 + 2e-4) * mag + 2.0 ** -8 * np.abs(want)).all()
+        t.model.evict()
+        t.compare()
+
+
+def test_hundreds_of_slots():
+    t = Pair(S=300, Hkv=2, G=2, P=16, D=64, SW=16, num_pages=5000, M=12, seed=11)
+    n_new = t.rng.integers(0, 60, 300).tolist()
+    t.append(60, n_new=n_new)
+    for n in (1, 20):
+        t.append(n)
+        t.attend(n)
+        t.evict()
+    src = t.rng.integers(-1, 300, 300).tolist()
+    t.reorder(src)
+    t.append(1)
+    t.attend(1)
+
+
+def test_pages_that_an_append_would_take():
+    t = Pair(S=3, Hkv=2, G=1, P=16, D=64, SW=48, num_pages=700, M=200, seed=12)
+    roles, n_new = t.roles(70, (0.1, 0.3, 0.6)), [16 * 30, 16 * 60 + 5, 7]
+    dev = torch.from_numpy(roles).to(DEV), torch.tensor(n_new, dtype=torch.int32, device=DEV)
+    counts = t.F.paged_append_count(t.kv, 1000, dev[0], 48, n_new=dev[1])
+    t.append(1000, n_new=n_new, roles=roles, skip_hidden=True)
+    assert torch.equal(counts, t.kv.n_pages)
+    assert not t.F.paged_append_count(t.kv, 0, None, 48).any()
+
+
 def test_pages_behind_32_bits():
     """Page numbers whose byte and element offsets need more than 32 bits"""
     from neuralattentionsearch_b200 import functional as F
@@ -406,7 +454,7 @@ def test_refusals_of_the_python_entry_points():
     def with_(i, x):
         return parts[:i] + [x] + parts[i + 1:]
     for bad in (with_(0, kv.pages_k.float()), with_(1, kv.pages_v[:5]), with_(2, kv.refs[:-1]), with_(3, kv.free_bits.long()), with_(5, kv.n_pages.T.contiguous().T),
-                with_(4, kv.entries[..., :3].contiguous() if False else kv.entries.float())):
+                with_(4, kv.entries.float()), with_(4, kv.entries[..., :3].contiguous()), with_(6, kv.length[:1])):
         with pytest.raises(ValueError):
             F.PagedKV(*bad)
     with pytest.raises(NotImplementedError):
@@ -418,7 +466,7 @@ def test_refusals_of_the_python_entry_points():
                  lambda: F.paged_append(kv, k, k, torch.zeros(2, 2, 1, device=DEV), 32),
                  lambda: F.paged_append(kv, k, k, None, 32, n_new=torch.zeros(2, device=DEV)),
                  lambda: F.paged_attention(kv, t.randn(2, 3, 1, 64)), lambda: F.paged_attention(kv, t.randn(2, 4, 1, 128)),
-                 lambda: F.paged_attention(kv, k, sm_scale=0.0), lambda: F.paged_attention(kv, k, sm_scale=float('nan')),
+                 lambda: F.paged_attention(kv, k, sm_scale=0.0), lambda: F.paged_attention(kv, k, out=k.float()), lambda: F.paged_attention(kv, k, out=k[:, :, :2]), lambda: F.paged_attention(kv, k, sm_scale=float('nan')),
                  lambda: F.paged_reorder(kv, torch.zeros(2, dtype=torch.long, device=DEV)), lambda: F.paged_reorder(kv, torch.zeros(3, dtype=torch.int32, device=DEV))):
         with pytest.raises(ValueError):
             call()
