@@ -438,6 +438,7 @@ class NAtSCache:
         if pages is not None and pages.page_size != chunk_size:
             raise ValueError(f'a cache in pages has one chunk per page: chunk size {chunk_size}, page size {pages.page_size}')
         self.pages = pages
+        self.moves = 0                          # how often sequences have been moved or repeated
         self.cache_model: list[NAtSChunkLayerCache | NAtSPagedLayerCache] = []
         self.sliding_window_size = sliding_window_size
         self.chunk_size = chunk_size
@@ -454,6 +455,7 @@ class NAtSCache:
     def reorder_cache(self, beam_idx: torch.Tensor):
         """Sequence b of every layer becomes a copy of what sequence ``beam_idx[b]`` was.  Only with ``pages``."""
         self._need_pages()
+        self.moves += 1
         for layer in self.cache_model:
             layer.reorder(beam_idx)
         self.cached_x = [None if x is None else x.index_select(0, beam_idx.to(x.device)) for x in self.cached_x]
@@ -461,6 +463,7 @@ class NAtSCache:
     def batch_repeat_interleave(self, repeats: int):
         """Every sequence ``repeats`` times, one after the other.  Only with ``pages``."""
         self._need_pages()
+        self.moves += 1
         for layer in self.cache_model:
             layer.repeat_interleave(repeats)
         self.cached_x = [None if x is None else x.repeat_interleave(repeats, 0) for x in self.cached_x]

@@ -15,6 +15,7 @@ with PyTorch ops: if the CUDA library is missing the import of ``_lib`` raises.
 from __future__ import annotations
 
 import math
+import threading
 
 import torch
 
@@ -703,14 +704,15 @@ PAGED_HEADER = 4096                        # bytes at the front of a workspace t
 
 
 def _paged_scratch(kv: PagedKV, name: str, stream: int, *sizes: int) -> torch.Tensor:
-    """Scratch for the entry point ``nats_b200_paged_<name>``: the cache's own where it has some, else one per stream.  While a graph is
-    recorded scratch that is not the cache's own is the graph's, so that two recorded graphs never share it."""
+    """Scratch for the entry point ``nats_b200_paged_<name>``: the cache's own where it has some, else one per stream and host thread (a call is
+    several launches, between which another thread's may come).  While a graph is recorded scratch that is not the cache's own is the
+    graph's, so that two recorded graphs never share it."""
     key = (name, *sizes)
     nbytes = _paged_bytes.get(key)
     if nbytes is None:
         nbytes = _paged_bytes[key] = getattr(_lib.lib(), f'nats_b200_paged_{name}_workspace_bytes')(*sizes)
     own = kv.scratch
-    kept, key = (_workspaces, ('paged', name, kv.index, stream)) if own is None else (own, name)
+    kept, key = (_workspaces, ('paged', name, kv.index, stream, threading.get_ident())) if own is None else (own, name)
     ws = kept.get(key)
     recording = torch.cuda.is_current_stream_capturing()
     if ws is None or ws.numel() < nbytes or (recording and own is None):

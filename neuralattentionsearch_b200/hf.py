@@ -206,6 +206,7 @@ class GraphedGreedyDecoder:
         self.steps_left = max_steps
         self.graph = None
         self._seen = start                  # tokens the cache must hold when generate() is called
+        self._moves = cache.moves
 
     def _step(self, recording: bool) -> None:
         core, C, B = self.model.model, self.C, self.B
@@ -238,7 +239,7 @@ class GraphedGreedyDecoder:
         holds the logits of the last step."""
         if n_steps < 1 or n_steps > self.steps_left:
             raise ValueError(f'{n_steps} steps asked for, room for {self.steps_left}')
-        if self.cache.get_seq_length(0) != self._seen:
+        if self.cache.get_seq_length(0) != self._seen or self.cache.moves != self._moves:
             # token position, chunk fill and pooled hidden states live on the device: they are only right if nobody else
             # has moved the cache since this object last did
             raise RuntimeError('the cache has been used by another path since this decoder was built: build a new GraphedGreedyDecoder')

@@ -11,6 +11,8 @@ There is no dense view of the cache: ``update`` returns the new K and V, and ``c
 """
 from __future__ import annotations
 
+import threading
+
 import torch
 
 from . import _lib
@@ -35,6 +37,7 @@ class KVPagePool:
         if num_pages % 32:
             self.free_bits[-1:].fill_((1 << num_pages % 32) - 1)
         self._free_bound = num_pages                  # pages that are free at least; the exact number is on the device
+        self._lock = threading.Lock()                 # a layer's post_update may run on a thread of its own
 
     def free_pages(self) -> int:
         """Pages that nobody holds (waits for the device)."""
@@ -43,9 +46,10 @@ class KVPagePool:
 
     def take(self, n: int) -> None:
         """Accounts for at most ``n`` pages that the next kernels take; raises before anything is launched if there may be fewer."""
-        if n > self._free_bound and n > self.free_pages():
-            raise _lib.NatsB200Error(f'a paged cache may need {n} pages, {self._free_bound} of {self.num_pages} are free')
-        self._free_bound -= n
+        with self._lock:
+            if n > self._free_bound and n > self.free_pages():
+                raise _lib.NatsB200Error(f'a paged cache may need {n} pages, {self._free_bound} of {self.num_pages} are free')
+            self._free_bound -= n
 
 
 class NAtSPagedLayerCache:

@@ -436,6 +436,36 @@ def test_long_rows_against_dense_attention():
                 assert ((o[s, h * G:(h + 1) * G] - want).abs() <= tol).all()
 
 
+@pytest.mark.parametrize('G', [40, 64, 128, 130])
+@pytest.mark.parametrize('N', [1, 3])
+def test_many_heads_per_kv_head(G, N):
+    t = Pair(S=2, Hkv=1, G=G, P=16, D=128, SW=32, num_pages=60, M=20, seed=G)
+    t.append(70, n_new=[70, 20])
+    t.append(N)
+    t.attend(N)
+
+
+def test_two_threads_on_one_stream():
+    import threading
+    pairs = [Pair(S=2, Hkv=2, G=2, P=16, D=64, SW=32, num_pages=900, M=100, seed=20 + i) for i in range(2)]
+    failed = []
+
+    def work(t):
+        try:
+            for _ in range(6):
+                t.append(100)                       # more than a block copies by itself: two launches with a workspace between them
+                t.attend(100)
+                t.evict()
+        except BaseException as e:
+            failed.append(e)
+    threads = [threading.Thread(target=work, args=(t,)) for t in pairs]
+    for th in threads:
+        th.start()
+    for th in threads:
+        th.join()
+    assert not failed, failed
+
+
 def test_two_runs_give_the_same_bits():
     outs = []
     for _ in range(2):

@@ -170,6 +170,10 @@ def test_graphed_greedy_decoding_in_pages_equals_the_eager_loop():
     assert torch.equal(got, torch.cat(want, 1))
     for a, b in zip(eager.cache_model, graphed.cache_model):
         assert a.get_seq_length() == b.get_seq_length() == 190 and torch.equal(a.kv.n_pages, b.kv.n_pages)
+    decoder = GraphedGreedyDecoder(model, graphed, 8)
+    graphed.reorder_cache(torch.tensor([0, 1], device=DEV))
+    with pytest.raises(RuntimeError, match='another path'):       # its pooled hidden states are those of the order before
+        decoder.generate(tok, 2)
     more = model(input_ids=ids[:, :30], past_key_values=graphed, use_cache=True).logits      # the eager path goes on from there
     same = model(input_ids=ids[:, :30], past_key_values=eager, use_cache=True).logits
     assert torch.equal(more, same)
