@@ -92,7 +92,7 @@ def lib() -> ctypes.CDLL:
 
 def call(name: str, *args) -> None:
     """Calls an int-returning entry point and raises NatsB200Error with the library's message on failure."""
-    rc = getattr(lib(), name)(*args)
+    rc = getattr(_lib or lib(), name)(*args)
     if rc != 0:
         msg = lib().nats_b200_last_error().decode()
         raise NatsB200Error(f'{name} failed (code {rc}): {msg}')

@@ -663,7 +663,6 @@ class PagedKV:
 
     def __init__(self, pages_k: torch.Tensor, pages_v: torch.Tensor, refs: torch.Tensor, free_bits: torch.Tensor, entries: torch.Tensor,
                  n_pages: torch.Tensor, length: torch.Tensor):
-        tensors = (pages_k, pages_v, refs, free_bits, entries, n_pages, length)
         n, P, D = pages_k.shape
         S, H, M, four = entries.shape
         if pages_k.dtype is not torch.bfloat16 or pages_v.dtype is not torch.bfloat16 or pages_v.shape != pages_k.shape:
@@ -672,18 +671,21 @@ class PagedKV:
         if refs.dtype is not i32 or free_bits.dtype is not i32 or entries.dtype is not i32 or n_pages.dtype is not i32 or length.dtype is not i32 or \
                 refs.shape != (n,) or free_bits.shape != ((n + 31) // 32,) or four != 4 or n_pages.shape != (S, H) or length.shape != (S,):
             raise ValueError(f'refs, free_bits, entries, n_pages and length must be int32 [{n}], [{(n + 31) // 32}], [S,Hkv,M,4], [{S},{H}] and [{S}], got ' +
-                             ', '.join(f'{t.dtype} {list(t.shape)}' for t in tensors[2:]))
-        self.index = index = pages_k.get_device()
-        for t in tensors:
-            if t.get_device() != index or index < 0:
-                _need_cuda(*tensors)
-            if not t.is_contiguous():
-                raise ValueError('the tensors of a paged cache must be contiguous')
+                             ', '.join(f'{t.dtype} {list(t.shape)}' for t in (refs, free_bits, entries, n_pages, length)))
+        index = pages_k.get_device()
+        if index < 0 or not index == pages_v.get_device() == refs.get_device() == free_bits.get_device() == entries.get_device() == \
+                n_pages.get_device() == length.get_device():
+            _need_cuda(pages_k, pages_v, refs, free_bits, entries, n_pages, length)
+        if not (pages_k.is_contiguous() and pages_v.is_contiguous() and refs.is_contiguous() and free_bits.is_contiguous() and
+                entries.is_contiguous() and n_pages.is_contiguous() and length.is_contiguous()):
+            raise ValueError('the tensors of a paged cache must be contiguous')
         if P not in PAGE_SIZES:
             raise ValueError(f'page size {P}: {PAGE_SIZES} are supported')
         if D not in PAGED_HEAD_DIMS:
             raise NotImplementedError(f'head_dim {D}: the paged cache is built for {PAGED_HEAD_DIMS}')
-        self.pages_k, self.pages_v, self.refs, self.free_bits, self.entries, self.n_pages, self.length = tensors
+        self.index = index
+        self.pages_k, self.pages_v, self.refs, self.free_bits, self.entries, self.n_pages, self.length = \
+            pages_k, pages_v, refs, free_bits, entries, n_pages, length
         self.num_pages, self.page_size, self.head_dim, self.slots, self.n_kv_heads, self.max_entries = n, P, D, S, H, M
         self.scratch: dict | None = None
         self._c = _lib.PAGED_KV(pages_k.data_ptr(), pages_v.data_ptr(), refs.data_ptr(), free_bits.data_ptr(), entries.data_ptr(),
@@ -714,7 +716,7 @@ def _paged_scratch(kv: PagedKV, name: str, stream: int, *sizes: int) -> torch.Te
     own = kv.scratch
     kept, key = (_workspaces, ('paged', name, kv.index, stream, threading.get_ident())) if own is None else (own, name)
     ws = kept.get(key)
-    recording = torch.cuda.is_current_stream_capturing()
+    recording = torch._C._cuda_isCurrentStreamCapturing()
     if ws is None or ws.numel() < nbytes or (recording and own is None):
         ws = torch.empty(nbytes, dtype=torch.uint8, device=kv.device)
         ws[:PAGED_HEADER].zero_()
@@ -725,7 +727,7 @@ def _paged_scratch(kv: PagedKV, name: str, stream: int, *sizes: int) -> torch.Te
 
 def _on(index: int, fn, *args):
     """``fn(*args)`` with the device of the cache current."""
-    if index == torch.cuda.current_device():
+    if index == torch._C._cuda_getDevice():
         return fn(*args)
     with torch.cuda.device(index):
         return fn(*args)
@@ -733,11 +735,15 @@ def _on(index: int, fn, *args):
 
 def _status_ptr(index: int) -> int:
     t = _status.get(index)
-    return (t if t is not None else status_word(torch.device('cuda', index))).data_ptr()
+    if t is None:
+        t = status_word(torch.device('cuda', index))
+    return t.data_ptr()
 
 
 def _strided_ok(t: torch.Tensor) -> bool:
     """Rows dense, everything 16-byte aligned: what the kernels read without a copy."""
+    if t.is_contiguous():                                # head dims are multiples of 16 bytes
+        return t.data_ptr() % 16 == 0
     step = 16 // t.element_size()
     a, b, c, d = t.stride()
     return d == 1 and t.data_ptr() % 16 == 0 and a % step == 0 and b % step == 0 and c % step == 0
