@@ -15,7 +15,7 @@ with PyTorch ops: if the CUDA library is missing the import of ``_lib`` raises.
 from __future__ import annotations
 
 import math
-import threading
+from threading import get_ident as _get_ident
 
 import torch
 
@@ -695,26 +695,20 @@ class PagedKV:
     def device(self) -> torch.device:
         return self.pages_k.device
 
-    def _check(self, *tensors: torch.Tensor) -> None:
-        for t in tensors:
-            if t.get_device() != self.index:
-                _need_cuda(self.pages_k, t)
-
 
 _paged_bytes: dict[tuple, int] = {}
 PAGED_HEADER = 4096                        # bytes at the front of a workspace that have to be zero before its first use
 
 
-def _paged_scratch(kv: PagedKV, name: str, stream: int, *sizes: int) -> torch.Tensor:
-    """Scratch for the entry point ``nats_b200_paged_<name>``: the cache's own where it has some, else one per stream and host thread (a call is
+def _paged_scratch(kv: PagedKV, stream: int, sizes: tuple) -> tuple[int, int]:
+    """Scratch for the entry point ``nats_b200_paged_<sizes[0]>``, its address and size: the cache's own where it has some, else one per stream and host thread (a call is
     several launches, between which another thread's may come).  While a graph is recorded scratch that is not the cache's own is the
     graph's, so that two recorded graphs never share it."""
-    key = (name, *sizes)
-    nbytes = _paged_bytes.get(key)
+    nbytes = _paged_bytes.get(sizes)
     if nbytes is None:
-        nbytes = _paged_bytes[key] = getattr(_lib.lib(), f'nats_b200_paged_{name}_workspace_bytes')(*sizes)
+        nbytes = _paged_bytes[sizes] = getattr(_lib.lib(), f'nats_b200_paged_{sizes[0]}_workspace_bytes')(*sizes[1:])
     own = kv.scratch
-    kept, key = (_workspaces, ('paged', name, kv.index, stream, threading.get_ident())) if own is None else (own, name)
+    kept, key = (_workspaces, (sizes[0], kv.index, stream, _get_ident())) if own is None else (own, sizes[0])
     ws = kept.get(key)
     recording = torch._C._cuda_isCurrentStreamCapturing()
     if ws is None or ws.numel() < nbytes or (recording and own is None):
@@ -722,15 +716,7 @@ def _paged_scratch(kv: PagedKV, name: str, stream: int, *sizes: int) -> torch.Te
         ws[:PAGED_HEADER].zero_()
         if not recording:
             kept[key] = ws
-    return ws
-
-
-def _on(index: int, fn, *args):
-    """``fn(*args)`` with the device of the cache current."""
-    if index == torch._C._cuda_getDevice():
-        return fn(*args)
-    with torch.cuda.device(index):
-        return fn(*args)
+    return ws.data_ptr(), nbytes
 
 
 def _status_ptr(index: int) -> int:
@@ -765,14 +751,34 @@ def paged_append(kv: PagedKV, k_new: torch.Tensor, v_new: torch.Tensor, roles: t
     global.  A chunk that a call completes gets its limit from its role; a completed global one closes the local ones in front.
     ``skip_hidden``: whole chunks that no query behind this call sees are not stored -- for a prompt whose attention does not
     read the pages.  Running out of pages or of entries raises the device's status word (``check_status``)."""
-    kv._check(k_new, v_new)
+    index = kv.index
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return paged_append(kv, k_new, v_new, roles, sliding_window, n_new, skip_hidden)
+    if k_new.get_device() != index or v_new.get_device() != index:
+        _need_cuda(kv.pages_k, k_new, v_new)
     S, H, N, D = shape = k_new.shape
     if S != kv.slots or H != kv.n_kv_heads or D != kv.head_dim or v_new.shape != shape:
         raise ValueError(f'k_new / v_new must be [{kv.slots},{kv.n_kv_heads},N,{kv.head_dim}], got {tuple(k_new.shape)} / {tuple(v_new.shape)}')
     roles = _check_roles(kv, roles)
     lens = _check_n_new(kv, n_new)
-    if N > 0:
-        _on(kv.index, _paged_append, kv, k_new, v_new, roles, lens, N, sliding_window, skip_hidden)
+    if N == 0:
+        return
+    f32 = k_new.dtype is torch.float32
+    if k_new.dtype is not v_new.dtype or not (f32 or k_new.dtype is torch.bfloat16):
+        f32 = False
+        k_new, v_new = k_new.to(torch.bfloat16), v_new.to(torch.bfloat16)
+    if not _strided_ok(k_new):
+        k_new = k_new.contiguous()
+    if not _strided_ok(v_new):
+        v_new = v_new.contiguous()
+    n_roles, roles_ptr = (0, 0) if roles is None else (roles.shape[2], roles.data_ptr())
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    ws, ws_bytes = _paged_scratch(kv, stream, ('append', S, H, N, kv.page_size))
+    ka, kb, kc, _ = k_new.stride()
+    va, vb, vc, _ = v_new.stride()
+    _lib.call('nats_b200_paged_append', kv._c, _lib.PAGED_APPEND(k_new.data_ptr(), v_new.data_ptr(), ka, kb, kc, va, vb, vc, roles_ptr, lens, ws, ws_bytes,
+                                                                 _status_ptr(index), f32, n_roles, N, sliding_window, skip_hidden), stream)
 
 
 def paged_append_count(kv: PagedKV, N: int, roles: torch.Tensor | None, sliding_window: int, n_new: torch.Tensor | None = None) -> torch.Tensor:
@@ -781,8 +787,8 @@ def paged_append_count(kv: PagedKV, N: int, roles: torch.Tensor | None, sliding_
     counts = torch.zeros(kv.slots, kv.n_kv_heads, dtype=torch.int32, device=kv.device)
     if N > 0:
         n_roles, roles_ptr = (0, None) if roles is None else (roles.shape[2], roles.data_ptr())
-        _on(kv.index, _lib.call, 'nats_b200_paged_append_count', kv._c, roles_ptr, n_roles, _check_n_new(kv, n_new), N, sliding_window, counts.data_ptr(),
-            torch._C._cuda_getCurrentRawStream(kv.index))
+        _call(kv.device, 'nats_b200_paged_append_count', kv._c, roles_ptr, n_roles, _check_n_new(kv, n_new), N, sliding_window, counts.data_ptr(),
+              _stream(kv.device))
     return counts
 
 
@@ -794,23 +800,6 @@ def _check_roles(kv: PagedKV, roles: torch.Tensor | None) -> torch.Tensor | None
     return roles.contiguous()
 
 
-def _paged_append(kv, k, v, roles, lens, N, sliding_window, skip_hidden):
-    n_roles, roles_ptr = (0, 0) if roles is None else (roles.shape[2], roles.data_ptr())
-    if k.dtype is not v.dtype or (k.dtype is not torch.bfloat16 and k.dtype is not torch.float32):
-        k, v = k.to(torch.bfloat16), v.to(torch.bfloat16)
-    if not _strided_ok(k):
-        k = k.contiguous()
-    if not _strided_ok(v):
-        v = v.contiguous()
-    stream = torch._C._cuda_getCurrentRawStream(kv.index)
-    ws = _paged_scratch(kv, 'append', stream, kv.slots, kv.n_kv_heads, N, kv.page_size)
-    ka, kb, kc, _ = k.stride()
-    va, vb, vc, _ = v.stride()
-    _lib.call('nats_b200_paged_append', kv._c,
-              _lib.PAGED_APPEND(k.data_ptr(), v.data_ptr(), ka, kb, kc, va, vb, vc, roles_ptr, lens, ws.data_ptr(), ws.numel(), _status_ptr(kv.index),
-                                k.dtype is torch.float32, n_roles, N, sliding_window, skip_hidden), stream)
-
-
 def paged_attention(kv: PagedKV, q: torch.Tensor, sm_scale: float | None = None, n_new: torch.Tensor | None = None,
                     token_major: bool = False, out: torch.Tensor | None = None) -> torch.Tensor:
     """Attention of the newest tokens of every slot over its pages, which hold their K and V already.  q [S,Hq,N,D] (cast to bf16 if needed;
@@ -818,7 +807,12 @@ def paged_attention(kv: PagedKV, q: torch.Tensor, sm_scale: float | None = None,
     (``n_new`` int32 [S]; None: N everywhere).  A key is seen from its own position on up to the limit of its page.  Rows behind a slot's
     new tokens and rows that see nothing are zero.  Returns o [S,Hq,N,D] in q's dtype; ``token_major``: a view of a [S,N,Hq,D] tensor;
     ``out``: written and returned, of q's shape and type (bf16 or fp32)."""
-    kv._check(q)
+    index = kv.index
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return paged_attention(kv, q, sm_scale, n_new, token_major, out)
+    if q.get_device() != index:
+        _need_cuda(kv.pages_k, q)
     S, Hq, N, D = q.shape
     if S != kv.slots or D != kv.head_dim or Hq == 0 or Hq % kv.n_kv_heads:
         raise ValueError(f'q must be [{kv.slots},multiple of {kv.n_kv_heads},N,{kv.head_dim}], got {tuple(q.shape)}')
@@ -826,43 +820,37 @@ def paged_attention(kv: PagedKV, q: torch.Tensor, sm_scale: float | None = None,
     scale = D ** -0.5 if sm_scale is None else float(sm_scale)
     if not scale > 0.0:
         raise ValueError('sm_scale must be positive')
+    dtype = q.dtype
+    f32 = dtype is torch.float32                         # fp32 callers: the kernel writes fp32 itself
     if out is not None:
-        kv._check(out)
-        if out.shape != q.shape or out.dtype is not q.dtype or out.dtype not in (torch.bfloat16, torch.float32) or not _strided_ok(out) or 0 in out.stride():
-            raise ValueError('out must be bf16 or fp32, shaped and typed like q, with dense rows and 16-byte alignment')
-    return _on(kv.index, _paged_attention, kv, q, scale, lens, token_major, out)
-
-
-def _paged_attention(kv, q, scale, lens, token_major, o):
-    S, Hq, N, D = q.shape
-    f32 = q.dtype is torch.float32                       # fp32 callers: the kernel writes fp32 itself
-    dtype = torch.float32 if f32 else torch.bfloat16
-    if o is None:
-        if token_major:
-            o = torch.empty(S, N, Hq, D, dtype=dtype, device=kv.device).transpose(1, 2)
-        else:
-            o = torch.empty_like(q, dtype=dtype, memory_format=torch.contiguous_format)
+        if out.get_device() != index or out.shape != q.shape or out.dtype is not dtype or not (f32 or dtype is torch.bfloat16) or \
+                not _strided_ok(out) or 0 in out.stride():
+            raise ValueError('out must be bf16 or fp32, shaped and typed like q on its device, with dense rows and 16-byte alignment')
+    elif token_major:
+        out = torch.empty(S, N, Hq, D, dtype=dtype if f32 else torch.bfloat16, device=kv.device).transpose(1, 2)
+    else:
+        out = torch.empty_like(q, dtype=dtype if f32 else torch.bfloat16, memory_format=torch.contiguous_format)
     if N > 0:
-        qb = q if q.dtype is torch.bfloat16 else q.to(torch.bfloat16)
-        if not _strided_ok(qb) or 0 in qb.stride():
-            qb = qb.contiguous()
-        stream = torch._C._cuda_getCurrentRawStream(kv.index)
-        ws = _paged_scratch(kv, 'attention', stream, S, Hq, kv.n_kv_heads, N, D, kv.page_size, kv.max_entries)
-        qs, qh, qt, _ = qb.stride()
-        os, oh, ot, _ = o.stride()
-        _lib.call('nats_b200_paged_attention', kv._c,
-                  _lib.PAGED_ATTENTION(qb.data_ptr(), o.data_ptr(), qs, qh, qt, os, oh, ot, lens, ws.data_ptr(), ws.numel(), _status_ptr(kv.index),
-                                       scale, f32, Hq, N), stream)
-    return o if o.dtype is q.dtype else o.to(q.dtype)
+        if dtype is not torch.bfloat16:
+            q = q.to(torch.bfloat16)
+        if not _strided_ok(q) or 0 in q.stride():
+            q = q.contiguous()
+        stream = torch._C._cuda_getCurrentRawStream(index)
+        ws, ws_bytes = _paged_scratch(kv, stream, ('attention', S, Hq, kv.n_kv_heads, N, D, kv.page_size, kv.max_entries))
+        qs, qh, qt, _ = q.stride()
+        os, oh, ot, _ = out.stride()
+        _lib.call('nats_b200_paged_attention', kv._c, _lib.PAGED_ATTENTION(q.data_ptr(), out.data_ptr(), qs, qh, qt, os, oh, ot, lens, ws, ws_bytes,
+                                                                           _status_ptr(index), scale, f32, Hq, N), stream)
+    return out if out.dtype is dtype else out.to(dtype)
 
 
 def paged_evict(kv: PagedKV) -> None:
     """Pages that the next query position (``length``) cannot see leave the rows; those that lose their last holder are free again."""
-    _on(kv.index, _paged_evict, kv)
-
-
-def _paged_evict(kv):
-    _lib.call('nats_b200_paged_evict', kv._c, torch._C._cuda_getCurrentRawStream(kv.index))
+    index = kv.index
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return paged_evict(kv)
+    _lib.call('nats_b200_paged_evict', kv._c, torch._C._cuda_getCurrentRawStream(index))
 
 
 def paged_reorder(kv: PagedKV, src: torch.Tensor) -> None:
@@ -872,10 +860,10 @@ def paged_reorder(kv: PagedKV, src: torch.Tensor) -> None:
     word (``check_status``) and leaves the slot empty."""
     if src.dtype is not torch.int32 or src.shape != (kv.slots,) or src.get_device() != kv.index or not src.is_contiguous():
         raise ValueError(f'src must be int32 [{kv.slots}] on {kv.device}')
-    _on(kv.index, _paged_reorder, kv, src)
-
-
-def _paged_reorder(kv, src):
-    stream = torch._C._cuda_getCurrentRawStream(kv.index)
-    ws = _paged_scratch(kv, 'reorder', stream, kv.slots, kv.n_kv_heads, kv.max_entries)
-    _lib.call('nats_b200_paged_reorder', kv._c, src.data_ptr(), ws.data_ptr(), ws.numel(), _status_ptr(kv.index), stream)
+    index = kv.index
+    if index != torch._C._cuda_getDevice():
+        with torch.cuda.device(index):
+            return paged_reorder(kv, src)
+    stream = torch._C._cuda_getCurrentRawStream(index)
+    ws, ws_bytes = _paged_scratch(kv, stream, ('reorder', kv.slots, kv.n_kv_heads, kv.max_entries))
+    _lib.call('nats_b200_paged_reorder', kv._c, src.data_ptr(), ws, ws_bytes, _status_ptr(index), stream)

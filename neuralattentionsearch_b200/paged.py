@@ -183,8 +183,8 @@ class NAtSPagedLayerCache:
         """Gets the cache ready for ``n_steps`` calls of ``decode_step_static`` that neither allocate nor read anything back."""
         self._room((self.chunk_fill_size + n_steps) // self.chunk_size + 1)
         kv, stream = self.kv, torch.cuda.current_stream(self.device).cuda_stream
-        F_._paged_scratch(kv, 'append', stream, kv.slots, kv.n_kv_heads, 1, kv.page_size)
-        F_._paged_scratch(kv, 'attention', stream, kv.slots, n_heads, kv.n_kv_heads, 1, head_dim, kv.page_size, kv.max_entries)
+        F_._paged_scratch(kv, stream, ('append', kv.slots, kv.n_kv_heads, 1, kv.page_size))
+        F_._paged_scratch(kv, stream, ('attention', kv.slots, n_heads, kv.n_kv_heads, 1, head_dim, kv.page_size, kv.max_entries))
         self._static_steps_left = n_steps
 
     def decode_step_static(self, xq: torch.Tensor, k_new: torch.Tensor, v_new: torch.Tensor, roles: torch.Tensor, out: torch.Tensor,
