@@ -177,6 +177,30 @@ def test_rows_whose_pages_are_all_hidden():
     assert o[:, :, :3].abs().amax() > 0 and not o[:, :, 3:].any()
 
 
+@pytest.mark.parametrize('G,N', [(2, 1), (2, 5), (4, 12), (4, 90)])
+def test_what_nobody_sees_is_never_used(G, N):
+    """Expired pages that are still in the rows, pages of other slots and the rest of unfinished pages hold NaN and infinities"""
+    t = Pair(S=2, Hkv=2, G=G, P=16, D=64, SW=32, num_pages=200, M=60, seed=N)
+    t.append(300, n_new=[300, 211], mix=(0.1, 0.2, 0.7))
+    t.append(N)
+    first = [n - N for n in t.model.length]
+    used = {e[0] for s in range(2) for row in t.model.rows[s] for e in row if e[2] >= first[s]}
+    hidden = torch.tensor([p for p in range(200) if p not in used], dtype=torch.long, device=DEV)
+    assert len(hidden) > 80
+    for pages in (t.kv.pages_k, t.kv.pages_v):
+        pages[hidden] = torch.tensor([float('nan'), float('inf'), -float('inf'), 3e38], device=DEV).bfloat16().repeat(16)
+    t.attend(N)
+
+
+def test_a_call_without_new_tokens():
+    t = Pair(S=2, Hkv=2, G=4, P=16, D=128, SW=32, num_pages=60, M=20, seed=1)
+    t.append(70, n_new=[70, 9])
+    for n in (3, 100):
+        o = t.attend(n, n_new=[0, 0])
+        assert not o.any()
+    t.append(5, n_new=[0, 0])
+
+
 @pytest.mark.parametrize('skip', [False, True])
 def test_a_prompt_without_its_hidden_chunks(skip):
     a = Pair(S=3, Hkv=2, G=2, P=16, D=64, SW=48, num_pages=700, M=100, seed=5)
