@@ -35,4 +35,15 @@ __device__ __forceinline__ void wait_for_launch_before() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// Position of the n-th set bit of a word (n = 0: the lowest), some position below 32 if there are not so many
+__device__ __forceinline__ int nth_set(uint32_t word, int n) {
+    int at = 0;
+#pragma unroll
+    for (int width = 16; width > 0; width >>= 1) {
+        const int low = __popc(word & ((1u << width) - 1u));
+        if (n >= low) { n -= low; word >>= width; at += width; }
+    }
+    return at;
+}
+
 }  // namespace nats

@@ -22,6 +22,7 @@ constexpr int kMinStretch = 64;                  // keys of a block's stretch at
 // What a unit costs a block besides its keys (draining and filling the ring, joining the warps, partial results), in keys.  us with 0 / 64 / 128 /
 // 256 / 512: 64 sequences of 8 heads 164 / 161 / 161 / 162 / 166, a step of 16 46.1 / 45.8 / 44.9 / 44.3 / 46.8, 4 of 8 23.4 / 22.8 / 21.5 / 21.5 / 22.2.
 constexpr int kUnitCost = 128;
+constexpr long long kFewKeys = 128 * 1024;       // keys times row tiles, see attn_plan
 
 __device__ __forceinline__ float exp2_approx(float x) {
     float y;
@@ -134,8 +135,6 @@ struct RowShared {
 };
 
 __device__ __forceinline__ int row_tokens(const PagedAttnParams& p, int s) { return p.n_new == nullptr ? p.N : min(max(p.n_new[s], 0), p.N); }
-// pages of a unit on the line
-__device__ __forceinline__ int unit_pages(const PagedKv& kv, int row, bool live) { return live ? max(min(kv.n_pages[row], kv.M), 1) : 1; }
 
 // Blocks per SM: what registers allow without spilling (head_dim 64 and sixteen rows: 3 or, with 70 bytes spilled, 4 blocks: 96 sequences of 1000
 // keys 47.0 / 50.2 us, 32 of 4000 keys 46.8 / 51.0).
@@ -160,7 +159,7 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 && D == 64 ? 3 : 2) paged
     const int per = (n_rows_all + kRowThreads - 1) / kRowThreads;
     auto row_pages = [&](int row) {
         const int n = row_tokens(p, row / kv.H), live = min((n * p.G + R - 1) / R, p.row_tiles);
-        return live * (unit_pages(kv, row, true) + p.front_pages) + p.row_tiles - live;
+        return live * (max(min(kv.n_pages[row], kv.M), 1) + p.front_pages) + p.row_tiles - live;
     };
     int sum = 0;
     for (int i = 0; i < per; ++i) {
@@ -437,9 +436,14 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 && D == 64 ? 3 : 2) paged
 struct AttnPlan { bool tiles; int mt, row_tiles, split_pages, front_pages; long long line; size_t counts, partials, bytes; };
 static AttnPlan attn_plan(int S, int H, int G, int N, int D, int P, int M) {
     AttnPlan a = {};
-    // Query rows up to which paged_rows_kernel is faster.  us, rows / tiles: head_dim 64 32 rows (16 sequences of 4 heads, 2200 keys each) 24.6 / 29.1,
-    // (16 of 8, 4700 keys) 41.7 / 48.7, 64 rows (one of 4, 1300 keys) 19.5 / 16.2; head_dim 128 32 rows (8 of 8, 2600 keys) 47.2 / 33.7.
-    a.tiles = (long long)N * G > (D == 64 ? 2 : 1) * kRows && G <= kTile;
+    // Where paged_rows_kernel is faster: up to one of its row tiles (sixteen query rows, 32 at head_dim 64), and beyond as long as all of the row
+    // tiles together look at few keys, which the host bounds by the tables' widths.  us, rows / tiles: head_dim 64 32 rows (16 sequences of 4
+    // heads, 2200 keys each) 24.6 / 29.1, (16 of 8, 4700 keys) 41.7 / 48.7; head_dim 128 32 rows (8 of 8, 2700 keys) 39.3 / 32.3.  Few keys, 8 kv-heads
+    // of one sequence, 1500 keys: 32 rows 17.8 / 22.8, 64 rows 18.0 / 23.0, 128 rows 21.6 / 24.2; 6000 keys, 32 rows 21.0 / 23.6; 500 keys, 256 rows 20.5 /
+    // 21.4.  3 sequences of 2700 keys, 32 rows 22.5 / 22.9; head_dim 64, 8 sequences of 1300 keys, 64 rows 28 / 23.
+    a.mt = D == 64 && (long long)N * G > kRows ? 2 : 1;
+    const long long tiles = ((long long)N * G + 16 * a.mt - 1) / (16 * a.mt);
+    a.tiles = G <= kTile && tiles > 1 && (long long)S * H * tiles * M * P > kFewKeys;
     a.counts = 4096;
     static_assert(kMaxTickets * 4 <= 4096, "the front of the workspace holds the tickets");
     if (a.tiles) {
@@ -448,8 +452,7 @@ static AttnPlan attn_plan(int S, int H, int G, int N, int D, int P, int M) {
         a.partials = a.counts + paged_tile_count_bytes(S, H, a.row_tiles);
         a.bytes = a.partials + paged_tile_result_bytes(D);
     } else {
-        a.mt = D == 64 && (long long)N * G > kRows ? 2 : 1;
-        a.row_tiles = (int)(((long long)N * G + 16 * a.mt - 1) / (16 * a.mt));
+        a.row_tiles = (int)tiles;
         a.split_pages = max(1, kMinStretch / P);
         a.front_pages = cdiv(kUnitCost, P);
         a.line = (long long)S * H * a.row_tiles * (max(M, 1) + a.front_pages);
@@ -511,6 +514,7 @@ NATS_EXPORT int nats_b200_paged_attention(const NatsPagedKV* kv, const NatsPaged
     NATS_CHECK_ARG((args->q_slot_stride | args->q_head_stride | args->q_token_stride | args->o_slot_stride | args->o_head_stride |
                     args->o_token_stride) % 8 == 0, "strides must keep 16-byte alignment");
     p.G = n_heads / p.kv.H;
+    NATS_CHECK_ARG((long long)N * p.G < (1 << 30), "%d new tokens of %d heads per kv-head are too many", N, p.G);
     const AttnPlan a = attn_plan(p.kv.S, p.kv.H, p.G, N, p.kv.D, p.kv.P, p.kv.M);
     if (args->workspace_bytes < a.bytes) return fail(NATS_ERR_WORKSPACE, "paged attention workspace: %zu bytes given, %zu needed", args->workspace_bytes, a.bytes);
     NATS_CHECK_ARG(a.line < (1ll << 31), "%d new tokens of %d heads per kv-head are too many", N, p.G);

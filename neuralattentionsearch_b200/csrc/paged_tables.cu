@@ -61,17 +61,6 @@ __device__ __forceinline__ FreeBits load_free(const PagedKv& kv, int w0) {
 }
 __device__ __forceinline__ int count_free(const FreeBits& f) { return __popc(f.w[0]) + __popc(f.w[1]) + __popc(f.w[2]) + __popc(f.w[3]); }
 
-// position of the n-th set bit (n = 0: the lowest) of a word with more than n of them
-__device__ __forceinline__ int nth_bit(uint32_t word, int n) {
-    int at = 0;
-#pragma unroll
-    for (int width = 16; width > 0; width >>= 1) {
-        const int low = __popc(word & ((1u << width) - 1u));
-        if (n >= low) { n -= low; word >>= width; at += width; }
-    }
-    return at;
-}
-
 struct PickScratch { int part[kTabWarps]; int rank[kTabThreads]; uint32_t words[kFreeWords]; };
 // The page of the calling thread's rank among the free ones (the lowest has rank 0), -1 if there are not so many or the rank is below 0.
 // Every thread of the block calls it; a thread looks its rank up in the prefix sums of the threads' words.
@@ -94,7 +83,7 @@ __device__ __forceinline__ int pick_free(const PagedKv& kv, const FreeBits& firs
             n -= sc.rank[t];
             int j = 0;
             for (int c; n >= (c = __popc(sc.words[4 * t + j])); ++j) n -= c;
-            page = (w0 + 4 * t + j) * 32 + nth_bit(sc.words[4 * t + j], n);
+            page = (w0 + 4 * t + j) * 32 + nth_set(sc.words[4 * t + j], n);
         }
         base += total;
     }

@@ -93,17 +93,6 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const CUtensorMap* map
         ::"r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(bar), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "l"(policy) : "memory");
 }
 
-// Position of the n-th set bit of a word (n = 0: the lowest), some position below 32 if there are not so many
-__device__ __forceinline__ int nth_set(uint32_t word, int n) {
-    int at = 0;
-#pragma unroll
-    for (int width = 16; width > 0; width >>= 1) {
-        const int low = __popc(word & ((1u << width) - 1u));
-        if (n >= low) { n -= low; word >>= width; at += width; }
-    }
-    return at;
-}
-
 // What a unit's queries see: positions of its first and last real token
 struct PtUnit { int s, n, q0, t0, t1; };
 __device__ __forceinline__ PtUnit pt_unit(const PagedAttnParams& p, int row, int tile) {

@@ -104,7 +104,7 @@ class Pair:
 @pytest.mark.parametrize('D', [64, 128])
 @pytest.mark.parametrize('P', [16, 32, 64, 128])
 def test_prompt_then_tokens(D, P):
-    t = Pair(S=2, Hkv=2, G=4, P=P, D=D, SW=2 * P, num_pages=200, M=40)
+    t = Pair(S=2, Hkv=2, G=4, P=P, D=D, SW=2 * P, num_pages=200, M=4000)
     t.append(5 * P + 3)
     t.attend(5 * P + 3)
     t.evict()
@@ -117,8 +117,9 @@ def test_prompt_then_tokens(D, P):
 
 @pytest.mark.parametrize('G', [1, 2, 3, 4, 5, 8, 16, 20])
 @pytest.mark.parametrize('N', [1, 2, 7, 33, 129])
-def test_group_sizes_and_lengths(G, N):
-    t = Pair(S=2, Hkv=2, G=G, P=16, D=64, SW=64, num_pages=400, M=80, seed=G * 1000 + N)
+@pytest.mark.parametrize('M', [80, 4000])             # the width of the tables has a say in which kernel runs
+def test_group_sizes_and_lengths(G, N, M):
+    t = Pair(S=2, Hkv=2, G=G, P=16, D=64, SW=64, num_pages=400, M=M, seed=G * 1000 + N)
     t.append(150)
     t.evict()
     t.append(N)
@@ -126,17 +127,19 @@ def test_group_sizes_and_lengths(G, N):
     t.attend(N, token_major=True)
 
 
+@pytest.mark.parametrize('M', [50, 3000])
 @pytest.mark.parametrize('mix', [(1, 0, 0), (0, 1, 0), (0, 0, 1), (0.05, 0.15, 0.8)])
-def test_roles_of_one_kind(mix):
-    t = Pair(S=1, Hkv=2, G=2, P=32, D=128, SW=64, num_pages=120, M=50)
+def test_roles_of_one_kind(mix, M):
+    t = Pair(S=1, Hkv=2, G=2, P=32, D=128, SW=64, num_pages=120, M=M)
     for n in (100, 1, 300, 27, 64, 200):
         t.append(n, mix=mix)
         t.attend(n)
         t.evict()
 
 
-def test_ragged_batches_with_empty_slots():
-    t = Pair(S=5, Hkv=2, G=4, P=32, D=64, SW=96, num_pages=300, M=40, seed=3)
+@pytest.mark.parametrize('M', [40, 1000])
+def test_ragged_batches_with_empty_slots(M):
+    t = Pair(S=5, Hkv=2, G=4, P=32, D=64, SW=96, num_pages=300, M=M, seed=3)
     for n_new in ([70, 0, 1, 33, 200], [0, 0, 0, 0, 0], [1, 0, 31, 64, 9], [1, 1, 1, 1, 1], [200, 5, 0, 0, 17]):
         N = max(max(n_new), 1)
         t.append(N, n_new=n_new)
@@ -144,8 +147,9 @@ def test_ragged_batches_with_empty_slots():
         t.evict()
 
 
-def test_padded_rows_are_zero_and_lengths_out_of_range_are_clamped():
-    t = Pair(S=2, Hkv=1, G=4, P=16, D=64, SW=32, num_pages=60, M=20)
+@pytest.mark.parametrize('M', [20, 2000])
+def test_padded_rows_are_zero_and_lengths_out_of_range_are_clamped(M):
+    t = Pair(S=2, Hkv=1, G=4, P=16, D=64, SW=32, num_pages=60, M=M)
     t.append(40, n_new=[40, 3])
     o = t.attend(200, n_new=[40, 3])
     assert not o[0, :, 40:].any() and not o[1, :, 3:].any()
@@ -155,8 +159,9 @@ def test_padded_rows_are_zero_and_lengths_out_of_range_are_clamped():
     assert torch.equal(a, b) and not a[1].any()
 
 
-def test_an_empty_cache_gives_zeros():
-    t = Pair(S=2, Hkv=2, G=2, P=64, D=128, SW=64, num_pages=10, M=4)
+@pytest.mark.parametrize('M', [4, 2000])
+def test_an_empty_cache_gives_zeros(M):
+    t = Pair(S=2, Hkv=2, G=2, P=64, D=128, SW=64, num_pages=10, M=M)
     for n in (1, 50):
         q = t.randn(2, 4, n, 128)
         assert not t.F.paged_attention(t.kv, q).any()
@@ -166,8 +171,9 @@ def test_an_empty_cache_gives_zeros():
     assert t.F.paged_attention(t.kv, t.randn(2, 4, 0, 128)).shape == (2, 4, 0, 128)
 
 
-def test_rows_whose_pages_are_all_hidden():
-    t = Pair(S=1, Hkv=1, G=2, P=16, D=64, SW=16, num_pages=30, M=20)
+@pytest.mark.parametrize('M,G', [(20, 2), (9000, 4)])
+def test_rows_whose_pages_are_all_hidden(M, G):
+    t = Pair(S=1, Hkv=1, G=G, P=16, D=64, SW=16, num_pages=30, M=M)
     t.append(48, roles=np.full((1, 1, 3), SLIDING, np.uint8))
     # limits 31, 47, 63: the next query (position 48) sees the last chunk only; with that one hidden too, nothing
     t.kv.entries[0, 0, :3, 2] = torch.tensor([31, 40, 40], dtype=torch.int32, device=DEV)
@@ -177,10 +183,11 @@ def test_rows_whose_pages_are_all_hidden():
     assert o[:, :, :3].abs().amax() > 0 and not o[:, :, 3:].any()
 
 
+@pytest.mark.parametrize('M', [60, 2000])
 @pytest.mark.parametrize('G,N', [(2, 1), (2, 5), (4, 12), (4, 90)])
-def test_what_nobody_sees_is_never_used(G, N):
+def test_what_nobody_sees_is_never_used(G, N, M):
     """Expired pages that are still in the rows, pages of other slots and the rest of unfinished pages hold NaN and infinities"""
-    t = Pair(S=2, Hkv=2, G=G, P=16, D=64, SW=32, num_pages=200, M=60, seed=N)
+    t = Pair(S=2, Hkv=2, G=G, P=16, D=64, SW=32, num_pages=200, M=M, seed=N)
     t.append(300, n_new=[300, 211], mix=(0.1, 0.2, 0.7))
     t.append(N)
     first = [n - N for n in t.model.length]
@@ -192,8 +199,9 @@ def test_what_nobody_sees_is_never_used(G, N):
     t.attend(N)
 
 
-def test_a_call_without_new_tokens():
-    t = Pair(S=2, Hkv=2, G=4, P=16, D=128, SW=32, num_pages=60, M=20, seed=1)
+@pytest.mark.parametrize('M', [20, 2000])
+def test_a_call_without_new_tokens(M):
+    t = Pair(S=2, Hkv=2, G=4, P=16, D=128, SW=32, num_pages=60, M=M, seed=1)
     t.append(70, n_new=[70, 9])
     for n in (3, 100):
         o = t.attend(n, n_new=[0, 0])
@@ -232,8 +240,9 @@ def test_roles_that_are_not_given_count_as_global():
 
 
 @pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
-def test_types_and_strides(dtype):
-    t = Pair(S=2, Hkv=3, G=2, P=32, D=64, SW=64, num_pages=100, M=30)
+@pytest.mark.parametrize('M', [30, 1000])
+def test_types_and_strides(dtype, M):
+    t = Pair(S=2, Hkv=3, G=2, P=32, D=64, SW=64, num_pages=100, M=M)
     t.append(77, dtype=dtype, token_major=True)
     q = t.randn(2, 77, 6, 64, dtype=dtype).transpose(1, 2)
     t.attend(77, dtype=dtype, q=q)
@@ -284,8 +293,9 @@ def test_out_of_pages_and_out_of_entries():
         t.F.status_word(torch.device(DEV, 0)).zero_()
 
 
-def test_bad_page_numbers_are_pages_that_are_not_there():
-    t = Pair(S=1, Hkv=1, G=2, P=16, D=64, SW=64, num_pages=40, M=12)
+@pytest.mark.parametrize('few', [True, False])
+def test_bad_page_numbers_are_pages_that_are_not_there(few):
+    t = Pair(S=1, Hkv=1, G=2, P=16, D=64, SW=64, num_pages=40, M=12 if few else 9000)
     t.append(160, roles=None)
     keep = t.kv.entries.clone()
     for n in (2, 100):
@@ -351,7 +361,7 @@ def test_other_streams_and_a_recorded_step():
 
 
 def test_a_recorded_call_of_many_tokens():
-    t = Pair(S=2, Hkv=2, G=4, P=32, D=64, SW=64, num_pages=300, M=60, seed=7)
+    t = Pair(S=2, Hkv=2, G=4, P=32, D=64, SW=64, num_pages=300, M=1500, seed=7)
     t.append(500, n_new=[500, 230])
     k, v, q = t.randn(2, 2, 70, 64), t.randn(2, 2, 70, 64), t.randn(2, 8, 70, 64)
     n_new = torch.tensor([70, 3], dtype=torch.int32, device=DEV)
@@ -463,7 +473,7 @@ def test_long_rows_against_dense_attention():
 @pytest.mark.parametrize('G', [40, 64, 128, 130])
 @pytest.mark.parametrize('N', [1, 3])
 def test_many_heads_per_kv_head(G, N):
-    t = Pair(S=2, Hkv=1, G=G, P=16, D=128, SW=32, num_pages=60, M=20, seed=G)
+    t = Pair(S=2, Hkv=1, G=G, P=16, D=128, SW=32, num_pages=60, M=3000, seed=G)
     t.append(70, n_new=[70, 20])
     t.append(N)
     t.attend(N)
