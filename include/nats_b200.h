@@ -342,7 +342,8 @@ int nats_b200_decode_step(const void* d_q, const void* d_k_new, const void* d_v_
  *   d_refs                int32 [num_pages]: rows that hold a page (0: free)
  *   d_free_bits           uint32 [ceil(num_pages / 32)]: bit p is set where page p is free (bits behind the last page: 0)
  *   d_entries             int32 [slots, n_kv_heads, max_entries, 4], the first d_n_pages of a row in use, in the order of positions:
- *                         page, position of its first token, last query position that may see it, 0
+ *                         page, position of its first token, last query position that may see it, mark: 1 where V of the page holds
+ *                         a value that is not finite (the append sets it; who writes pages by other ways sets it too), else 0
  *                         (limit 2^31 - 1: for good; 2^31 - 2: a local chunk that no completed global chunk has closed yet)
  *   d_n_pages             int32 [slots, n_kv_heads]
  *   d_length              int32 [slots]: tokens so far.  Where it is no multiple of the page size, the last page of each of the slot's
@@ -385,8 +386,8 @@ int nats_b200_paged_append_count(const NatsPagedKV* kv, const uint8_t* d_roles, 
 /* Attention of the last d_n_new[slot] (NULL: N) tokens of every slot, whose K and V are in the pages.  q bf16 and o (bf16, or fp32 with
  * o_f32 != 0) are [slots, n_heads, N, head_dim] with the strides given, the last axis dense.  Row i of a slot is the token at position
  * length - n_new + i; rows behind the slot's new tokens, and rows that see no key, are written as zero.  What lies in pages
- * behind a slot's last token, and in pages that no query of the call sees, is never used, whatever it holds; a V value of a visible token that is
- * not finite reaches, besides the queries that see it, others of the same call.
+ * behind a slot's last token, and in pages that no query of the call sees, is never used, whatever it holds; a K or V that is
+ * not finite reaches the queries that see its token and no others (for V by the page's mark).
  */
 typedef struct NatsPagedAttention {
     const void* d_q; void* d_o;

@@ -1,7 +1,8 @@
 // What the operators of the paged cache share.
 //
 // K and V lie in pages of P consecutive tokens of one (sequence, kv-head); a page is one chunk of the role rule.  A slot (a sequence) has a
-// row of entries per kv-head: int4 (page, position of its first token, last query position that may see it, 0) in the order of positions.
+// row of entries per kv-head: int4 (page, position of its first token, last query position that may see it, mark) in the order of positions.
+// The mark is 1 where a V that is not finite has been written to the page, else 0.
 // Only the last page of a row may be part filled, and nobody else holds that page.  refs counts the rows that hold a page; a page that
 // nobody holds has its bit set in free_bits.
 #pragma once
@@ -34,6 +35,15 @@ __device__ __forceinline__ void wait_for_launch_before() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
+
+// Nonzero: one of the bf16 is not finite, in the bits of their signs: one added to an exponent of ones carries into them, and nothing else does.
+__device__ __forceinline__ uint32_t not_finite_bits(uint32_t w) { return ((w & 0x7f807f80u) + 0x00800080u) & 0x80008000u; }
+__device__ __forceinline__ uint32_t not_finite_bits(const uint4& w) {
+    return not_finite_bits(w.x) | not_finite_bits(w.y) | not_finite_bits(w.z) | not_finite_bits(w.w);
+}
+// those of a pair that are not finite, or that are, and zero for the others
+__device__ __forceinline__ uint32_t not_finite_part(uint32_t w) { return w & ((not_finite_bits(w) >> 15) * 0xffffu); }
+__device__ __forceinline__ uint32_t finite_part(uint32_t w) { return w & ~((not_finite_bits(w) >> 15) * 0xffffu); }
 
 // Position of the n-th set bit of a word (n = 0: the lowest), some position below 32 if there are not so many
 __device__ __forceinline__ int nth_set(uint32_t word, int n) {

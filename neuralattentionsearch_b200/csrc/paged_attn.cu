@@ -16,6 +16,7 @@ namespace nats {
 constexpr int kRowThreads = 128, kRowWarps = kRowThreads / 32;
 constexpr int kRowTile = 16;                     // keys per warp tile
 constexpr int kRowStages = 3;
+constexpr int kMarked = (int)0x80000000u;        // added to a position: the page is marked
 constexpr int kRows = 16;                        // query rows of an A fragment
 constexpr int kMaxTickets = 640;                 // blocks of a launch; the workspace begins with as many words, which are zero between calls
 constexpr int kMinStretch = 64;                  // keys of a block's stretch at least
@@ -124,6 +125,32 @@ __device__ __forceinline__ void join_parts(const PagedAttnParams& p, int s, int 
     }
 }
 
+// Sets what is not finite in a tile of V to zero; the whole warp calls it.
+__device__ __forceinline__ void zero_not_finite(uint8_t* v, int bytes) {
+#pragma unroll 1
+    for (int i = (threadIdx.x & 31) * 4; i < bytes; i += 128) {
+        uint32_t* w = reinterpret_cast<uint32_t*>(v + i);
+        *w = finite_part(*w);
+    }
+}
+// Adds what is not finite in four columns of V, of the keys in entries [first, end) that a query at qpos sees.
+template <int D>
+__device__ __forceinline__ void add_not_finite(float4& a, const PagedKv& kv, const int4* entries, int first, int end, int qpos, int d) {
+#pragma unroll 1
+    for (int i = first; i < end; ++i) {
+        const int4 e = entries[i];
+        if (e.w == 0 || (unsigned)e.x >= (unsigned)kv.num_pages || qpos > e.z) continue;
+        const uint2* v = reinterpret_cast<const uint2*>(kv.v + ((size_t)e.x * kv.P * D + d) * 2);
+#pragma unroll 1
+        for (int k = 0; k < kv.P && e.y + k <= qpos; ++k) {
+            const uint2 w = v[k * (D / 4)];
+            const uint32_t lo = not_finite_part(w.x), hi = not_finite_part(w.y);
+            a.x += __uint_as_float(lo << 16); a.y += __uint_as_float(lo & 0xffff0000u);
+            a.z += __uint_as_float(hi << 16); a.w += __uint_as_float(hi & 0xffff0000u);
+        }
+    }
+}
+
 // Work is dealt in pages: the row tiles ("units": sixteen or thirty-two query rows of a (slot, kv-head)) with their pages form one line, of which
 // every block takes a stretch of the same length.  A stretch covers parts of one or more units; a unit within one stretch is written out
 // at once, of the others every part goes to the workspace, and the block that finishes the last of them joins them in order.
@@ -132,6 +159,7 @@ struct RowShared {
     int warp_sum[kRowWarps];
     int row, at, pages, last;
     int2 meta[kRowWarps][kRowStages];              // position of the first key, limit of a stage's tile
+    int marked[kRowWarps];                         // where the last unit began for which a warp had marked pages
 };
 
 __device__ __forceinline__ int row_tokens(const PagedAttnParams& p, int s) { return p.n_new == nullptr ? p.N : min(max(p.n_new[s], 0), p.N); }
@@ -167,7 +195,7 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 && D == 64 ? 3 : 2) paged
         if (row < n_rows_all) sum += row_pages(row);
     }
     const int incl = warp_incl_scan(sum, lane);
-    if (lane == 31) sh.warp_sum[warp] = incl;
+    if (lane == 31) { sh.warp_sum[warp] = incl; sh.marked[warp] = -1; }
     __syncthreads();
     int before = incl - sum, total = 0;
 #pragma unroll
@@ -246,8 +274,9 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 && D == 64 ? 3 : 2) paged
                 const int tile = warp + kRowWarps * (w0 + lane);
                 if (w0 + lane < my_tiles) {
                     e = entries[e_first + tile / tpp];
-                    e.w = tile % tpp * kRowTile;                                    // the tile's first row in the page
-                    e.y += e.w;                                                     // ... and its position
+                    const int at = tile % tpp * kRowTile;                           // the tile's first row in the page
+                    e.y += at;                                                      // ... and its position
+                    e.w = e.w != 0 ? at | kMarked : at;
                     if ((unsigned)e.x >= (unsigned)kv.num_pages) e.z = -1;
                 }
                 return e;
@@ -269,7 +298,7 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 && D == 64 ? 3 : 2) paged
                 seen &= seen - 1u;
                 const int page = __shfl_sync(FULL, e.x, from), pos = __shfl_sync(FULL, e.y, from), at = __shfl_sync(FULL, e.w, from);
                 const int limit = __shfl_sync(FULL, e.z, from);
-                const size_t off = ((size_t)page * P + at) * ROWB + (lane % CHUNKS) * 16;
+                const size_t off = ((size_t)page * P + (at & ~kMarked)) * ROWB + (lane % CHUNKS) * 16;
                 const uint32_t dst = ring + stage_in * STAGE_BYTES;
 #pragma unroll
                 for (int x = 0; x < CP_PER_LANE; ++x) {
@@ -279,7 +308,7 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 && D == 64 ? 3 : 2) paged
                     cp16(to, kv.k + off + (size_t)r * ROWB, ok);
                     cp16(to + TILE_BYTES, kv.v + off + (size_t)r * ROWB, ok);
                 }
-                if (lane == 0) sh.meta[warp][stage_in] = make_int2(pos, limit);
+                if (lane == 0) sh.meta[warp][stage_in] = make_int2(pos | (at & kMarked), limit);
                 stage_in = stage_in + 1 == kRowStages ? 0 : stage_in + 1;
                 return true;
             };
@@ -299,7 +328,7 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 && D == 64 ? 3 : 2) paged
                 cp_wait<kRowStages - 1>();
                 __syncwarp();
                 const int2 meta = sh.meta[warp][stage];
-                const int pos = meta.x, limit = meta.y;
+                const int pos = meta.x & ~kMarked, limit = meta.y;
                 const uint32_t sk = ring + stage * STAGE_BYTES, sv = sk + TILE_BYTES;
                 float sc[MT][2][4];
 #pragma unroll
@@ -353,6 +382,11 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 && D == 64 ? 3 : 2) paged
                         }
                     }
                 }
+                if (__builtin_expect(meta.x < 0, 0)) {
+                    if (lane == 0) sh.marked[warp] = unit_begin;                    // what is not finite is added when the warps are joined
+                    zero_not_finite(dsm + (warp * kRowStages + stage) * STAGE_BYTES + TILE_BYTES, TILE_BYTES);
+                    __syncwarp();
+                }
 #pragma unroll
                 for (int np = 0; np < D / 16; ++np) {
                     uint32_t vb[4];
@@ -386,6 +420,9 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 && D == 64 ? 3 : 2) paged
                 }
             __syncthreads();
             const bool alone = first_block == last_block;
+            bool marked = false;
+#pragma unroll
+            for (int w = 0; w < kRowWarps; ++w) marked |= sh.marked[w] == unit_begin;
             // a block has at most two units that it shares: the one that began before its stretch, and the one that ends behind it
             float* part = p.partials + ((size_t)blockIdx.x * 2 + (unit_begin < begin ? 0 : 1)) * R * PSTRIDE;
             for (int i = tid; i < n_rows * (D / 4); i += kRowThreads) {
@@ -403,6 +440,7 @@ __global__ void __launch_bounds__(kRowThreads, MT == 1 && D == 64 ? 3 : 2) paged
                         l = fmaf(s_l[w][r], f, l);
                     }
                 }
+                if (__builtin_expect(marked, 0) && r < live) add_not_finite<D>(a, kv, entries, e_first, e_end, q0 + (r0 + r) / p.G, d);
                 if (alone) {
                     store_o(p, s, h, r0 + r, d, divided(a, l));
                 } else if (r < live) {

@@ -232,7 +232,13 @@ __device__ __forceinline__ TokenVecs load_tokens(const AppendParams& p, int s, i
     }
     return x;
 }
-__device__ __forceinline__ void store_tokens(const AppendParams& p, const TokenVecs& x, int old, int t0, int t1, const int32_t* map) {
+// the mark of the entry that holds a page, one of [from, to)
+__device__ __forceinline__ void mark_page(int4* entries, int from, int to, int page) {
+    for (int e = from; e < to; ++e)
+        if (entries[e].x == page) { entries[e].w = 1; return; }
+}
+// entries: those of the row, the ones that the call writes to lie in [first, end)
+__device__ __forceinline__ void store_tokens(const AppendParams& p, const TokenVecs& x, int old, int t0, int t1, const int32_t* map, int4* entries, int first, int end) {
     const int vecs = p.kv.D / 8, P = p.kv.P, c0 = old / P;
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
@@ -243,6 +249,7 @@ __device__ __forceinline__ void store_tokens(const AppendParams& p, const TokenV
         const size_t to = (((size_t)page * P + pos % P) * p.kv.D + c * 8) * 2;
         st16(p.kv.k + to, x.k[j]);
         st16(p.kv.v + to, x.v[j]);
+        if (__builtin_expect(not_finite_bits(x.v[j]) != 0u, 0)) mark_page(entries, first, end, page);
     }
 }
 
@@ -313,7 +320,7 @@ __global__ void __launch_bounds__(kTabThreads, 4) paged_append_kernel(const Appe
         if (room < take) paged_status(p.status, kErrNoEntry);
         if (placed > 0) kv.n_pages[row] = n0 + placed;
     }
-    if (p.copy_here) store_tokens(p, vecs, r.old, 0, r.n, s_map);
+    if (p.copy_here) store_tokens(p, vecs, r.old, 0, r.n, s_map, entries, max(n0 - 1, 0), n0 + room);
     if (!last_block(p.ticket, rows)) return;
     take_lowest(kv, total, s_a);
     for (int s = tid; s < kv.S; s += kTabThreads) kv.length[s] += new_tokens(p, s);
@@ -324,8 +331,10 @@ __global__ void __launch_bounds__(kTabThreads) paged_copy_kernel(const AppendPar
     wait_for_launch_before();
     const int n = new_tokens(p, s), t1 = min((int)(blockIdx.x + 1) * kCopyTokens, n);
     const int old = p.kv.length[s] - n;          // the table kernel has moved the lengths on
+    const int n_pages = min(max(p.kv.n_pages[blockIdx.y], 0), p.kv.M);
     for (int t0 = blockIdx.x * kCopyTokens; t0 < t1; t0 += per_pass)
-        store_tokens(p, load_tokens(p, s, h, t0, t1), old, t0, t1, p.map + (size_t)blockIdx.y * p.n_chunks);
+        store_tokens(p, load_tokens(p, s, h, t0, t1), old, t0, t1, p.map + (size_t)blockIdx.y * p.n_chunks, p.kv.entries + (size_t)blockIdx.y * p.kv.M,
+                     max(n_pages - p.n_chunks, 0), n_pages);
 }
 
 // =================================================================================================

@@ -18,7 +18,7 @@
 //
 // Scores lie apart from P and are handed back as soon as they are in registers, so that the next tile's Q.K^T runs beside the softmax.
 // Keys behind a sequence's last one: the rows of an unfinished page may hold anything, and 0 * NaN is NaN, so the issuer of P.V writes zeros over
-// them in shared memory; pages that a part filled tile lacks are read as zero from behind the pool.
+// what is not finite in them; pages that a part filled tile lacks are read as zero from behind the pool.
 #include "paged_attn.cuh"
 #include "sm100.cuh"
 
@@ -39,12 +39,13 @@ struct PtHeader {
     int q0, n;                                   // position of the slot's first new token, number of new tokens
     int part;                                    // -1: the whole unit; else where its partial result goes, see PtPart
     int n_pages;                                 // of the row
-    int pad[2];
+    int marked;                                  // the unit sees marked pages
+    int pad;
 };
 
 // A CTA shares at most two units with others: one that began before its stretch (part 0), one that goes on behind it (part 1).
 // In the workspace: [CTA][2] results of 256 rows, then what the join has to know about the unit that a CTA is the first to share.
-struct PtPart { int split, row, tile, last; int begin, chunk, pad[2]; };
+struct PtPart { int split, row, tile, last; int begin, chunk, marked_from, marked_to; };
 constexpr int kPtRows = 256;
 template <int D>
 struct PtResult { float4 o[D / 4][kPtRows]; float2 ml[kPtRows]; };
@@ -109,14 +110,18 @@ __device__ __forceinline__ bool pt_sees(const PagedKv& kv, const int4& e, int q_
     return (unsigned)e.x < (unsigned)kv.num_pages && e.z >= q_lo && e.y <= q_hi;
 }
 
-// K / V tiles of every unit, in the order (row, pair of query tiles); -1 where all its tokens are padding.  `warps` warps per unit: eight while that
+// What the workspace holds of a unit: its K / V tiles, whether it sees marked pages, and whether one CTA has all of it (set for marked ones); -1 where
+// all its tokens are padding
+constexpr int kUnitTiles = (1 << 28) - 1, kUnitMarked = 1 << 28, kUnitWhole = 1 << 29;
+
+// The above for every unit, in the order (row, pair of query tiles).  `warps` warps per unit: eight while that
 // does not make more blocks than run at once, since a warp waits for its entries most of the time.
 __global__ void __launch_bounds__(256) paged_plan_kernel(const PagedAttnParams p, int warps) {
-    __shared__ int s_seen[8];
+    __shared__ int s_seen[8], s_marked[8];
     const int pairs = (p.row_tiles + 1) / 2, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
     const int unit = blockIdx.x * (8 / warps) + warp / warps, part = warp % warps;
     wait_for_launch_before();
-    int n_vis = 0;
+    int n_vis = 0, marked = 0;
     bool live = false;
     if (unit < p.kv.S * p.kv.H * pairs) {
         const int row = unit / pairs;
@@ -126,15 +131,21 @@ __global__ void __launch_bounds__(256) paged_plan_kernel(const PagedAttnParams p
             const int q_lo = u.q0 + u.t0, q_hi = u.q0 + u.t1 - 1, n = min(max(p.kv.n_pages[row], 0), p.kv.M);
             const int4* entries = p.kv.entries + (size_t)row * p.kv.M;
 #pragma unroll 4
-            for (int i = part * 32 + lane; i < n; i += warps * 32) n_vis += pt_sees(p.kv, entries[i], q_lo, q_hi);
+            for (int i = part * 32 + lane; i < n; i += warps * 32) {
+                const int4 e = entries[i];
+                const bool sees = pt_sees(p.kv, e, q_lo, q_hi);
+                n_vis += sees;
+                marked |= sees && e.w != 0;
+            }
         }
     }
     n_vis = __reduce_add_sync(0xffffffffu, n_vis);
-    if (lane == 0) s_seen[warp] = n_vis;
+    marked = __any_sync(0xffffffffu, marked);
+    if (lane == 0) { s_seen[warp] = n_vis; s_marked[warp] = marked; }
     __syncthreads();
     if (part == 0 && lane == 0 && unit < p.kv.S * p.kv.H * pairs) {
-        for (int w = 1; w < warps; ++w) n_vis += s_seen[warp + w];
-        p.counts[unit] = live ? (n_vis * p.kv.P + kTile - 1) / kTile : -1;
+        for (int w = 1; w < warps; ++w) { n_vis += s_seen[warp + w]; marked |= s_marked[warp + w]; }
+        p.counts[unit] = live ? (int)(((long long)n_vis * p.kv.P + kTile - 1) / kTile) | (marked ? kUnitMarked : 0) : -1;
     }
 }
 
@@ -205,7 +216,7 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
         // a unit that sees nothing has zeros to write, one of padding has no length
         auto length_of = [&](int u) {
             const int c = u < units ? p.counts[u] : -1;
-            return c < 0 ? 0 : c + kPtUnitTiles;
+            return c < 0 ? 0 : (c & kUnitTiles) + kPtUnitTiles;
         };
         // every lane sums up its share of the units; the one whose share holds the beginning of the stretch looks for the unit there
         const int per = (units + 31) / 32;
@@ -254,6 +265,12 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                 hd.skip = t0 * (kTile / kv.P);
                 hd.part = first == last ? -1 : unit_begin < begin ? 0 : 1;
                 if (hd.part == 1) { shared.split = 1; shared.row = hd.row; shared.tile = hd.tile; shared.last = last; shared.begin = unit_begin; shared.chunk = chunk; }
+                hd.marked = p.counts[unit] & kUnitMarked;
+                if (hd.marked && first == last) {
+                    if (lane == 0) p.counts[unit] |= kUnitWhole;
+                    if (shared.marked_to == 0) shared.marked_from = unit;
+                    shared.marked_to = unit + 1;
+                }
                 line = to;
                 unit_begin = unit_end;
                 ++unit;
@@ -452,15 +469,17 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
                         ok = util_wait(smem_u32(&sm.bar_full[gv % NS]), (gv / NS) & 1, abort_flag, p.status, kPtErr + kErrKvFull);
                         if (!ok) break;
                         const uint32_t vl = r_lo0 + (gv % NS) * T16;
-                        const int tail = sm.meta[meta].tail;
+                        const int tail = hd.marked ? kTile << 16 : sm.meta[meta].tail;
                         meta = meta + 1 == Smem::kMetas ? 0 : meta + 1;
                         if (tail != 0) {
-                            // rows without a token: zeros (the swizzle moves 16-byte pieces inside a row of 128 bytes)
+                            // rows without a token, or all that marked pages may have: finite (the swizzle moves 16-byte pieces inside a row of 128 bytes)
                             uint8_t* base = &sm.ring[gv % NS][0];
                             const int r0 = tail & 0xffff, rows = (tail >> 16) - r0;
                             for (int i = lane; i < rows * NBOX * 8; i += 32) {
                                 const int r = r0 + i / (NBOX * 8), c = i % (NBOX * 8);
-                                *reinterpret_cast<uint4*>(base + (c / 8) * kBoxBytes + r * 128 + (c % 8) * 16) = make_uint4(0, 0, 0, 0);
+                                uint4* at = reinterpret_cast<uint4*>(base + (c / 8) * kBoxBytes + r * 128 + (c % 8) * 16);
+                                const uint4 x = *at;
+                                *at = make_uint4(finite_part(x.x), finite_part(x.y), finite_part(x.z), finite_part(x.w));
                             }
                             asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                             __syncwarp();
@@ -688,65 +707,113 @@ paged_tile_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_consta
     }
 }
 
+// Adds what is not finite in V to eight columns (`vec`) of a unit's rows, a lane per row: at its output, if it has one.  The whole warp calls it.
+template <int D>
+__device__ __forceinline__ void add_not_finite(const PagedAttnParams& p, int row, int tile, int vec, int r) {
+    const int lane = threadIdx.x & 31;
+    const PtUnit u = pt_unit(p, row, tile);
+    const int TT = kTile / p.G, rr = r & (kTile - 1), tok = rr / p.G, head = rr - tok * p.G, t = (tile + r / kTile) * TT + tok;
+    const bool real = tok < TT && t < u.n;
+    const int qpos = real ? u.q0 + t : -1, q_lo = u.q0 + u.t0, q_hi = u.q0 + u.t1 - 1, n = min(max(p.kv.n_pages[row], 0), p.kv.M);
+    const int4* entries = p.kv.entries + (size_t)row * p.kv.M;
+    float add[8] = {};
+#pragma unroll 1
+    for (int i = 0; i < n; ++i) {
+        const int4 e = entries[i];
+        if (e.w == 0 || !pt_sees(p.kv, e, q_lo, q_hi)) continue;
+        const uint4* v = reinterpret_cast<const uint4*>(p.kv.v + (size_t)e.x * p.kv.P * (D * 2));
+#pragma unroll 1
+        for (int k0 = 0; k0 < p.kv.P; k0 += 32) {
+            const uint4 mine = k0 + lane < p.kv.P ? v[(k0 + lane) * (D / 8) + vec] : make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll 1
+            for (unsigned who = __ballot_sync(0xffffffffu, not_finite_bits(mine) != 0u); who != 0u; who &= who - 1u) {
+                const int from = __ffs(who) - 1, pos = e.y + k0 + from;
+                const uint32_t w[4] = {__shfl_sync(0xffffffffu, mine.x, from), __shfl_sync(0xffffffffu, mine.y, from), __shfl_sync(0xffffffffu, mine.z, from),
+                                       __shfl_sync(0xffffffffu, mine.w, from)};
+                if (pos > qpos || qpos > e.z) continue;
+#pragma unroll
+                for (int x = 0; x < 4; ++x) {
+                    const uint32_t bad = not_finite_part(w[x]);
+                    add[2 * x] += __uint_as_float(bad << 16);
+                    add[2 * x + 1] += __uint_as_float(bad & 0xffff0000u);
+                }
+            }
+        }
+    }
+    if (!real) return;
+    const long long at = u.s * p.o_slot + ((row - u.s * p.kv.H) * p.G + head) * p.o_head + t * p.o_token + vec * 8;
+#pragma unroll
+    for (int x = 0; x < 8; ++x) {
+        if (add[x] == 0.f) continue;             // the sum of none
+        if (p.o_f32) ((float*)p.o)[at + x] += add[x];
+        else ((__nv_bfloat16*)p.o)[at + x] = __float2bfloat16(__bfloat162float(((const __nv_bfloat16*)p.o)[at + x]) + add[x]);
+    }
+}
+
 // Joins the parts of the units that lie in several stretches: blockIdx.x is the first CTA of such a unit, blockIdx.y 32 of its rows.  A lane
-// per row, eight columns per warp and pass.
+// per row, eight columns per warp.  The blocks of a CTA also look after the marked units that it alone has had.
 template <int D>
 __global__ void __launch_bounds__(256) paged_join_kernel(const PagedAttnParams p, int n_ctas) {
     wait_for_launch_before();
     if (*p.status != 0) return;                  // the CTAs may have left nothing
     const PtResult<D>* results = reinterpret_cast<const PtResult<D>*>(p.partials);
     const PtPart part = reinterpret_cast<const PtPart*>(results + 2 * (size_t)n_ctas)[blockIdx.x];
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.y * 32 + lane, vec = blockIdx.z * 8 + warp;
+    const int pairs = (p.row_tiles + 1) / 2;
+#pragma unroll 1
+    for (int unit = part.marked_from; unit < part.marked_to; ++unit) {
+        const int c = p.counts[unit];
+        if (c > 0 && (c & kUnitWhole)) add_not_finite<D>(p, unit / pairs, unit % pairs * 2, vec, r);
+    }
     if (!part.split) return;
-    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, r = blockIdx.y * 32 + lane;
     const int TT = kTile / p.G, row = r & (kTile - 1), tok = row / p.G, head = row - tok * p.G;
     const int s = part.row / p.kv.H, n = p.n_new == nullptr ? p.N : min(max(p.n_new[s], 0), p.N);
     const int t = (part.tile + r / kTile) * TT + tok, first = blockIdx.x;
-    if (tok >= TT || t >= p.N) return;
-    const bool real = t < n;
+    const bool there = tok < TT && t < p.N, real = there && t < n;
     auto result_of = [&](int x) -> const PtResult<D>& { return results[2 * (size_t)x + (part.begin < x * part.chunk ? 0 : 1)]; };
     const int hq = (part.row - s * p.kv.H) * p.G + head;
     const long long at = s * p.o_slot + hq * p.o_head + t * p.o_token;
-    for (int c = (blockIdx.z * 8 + warp) * 2; c < D / 4; c += 16 * gridDim.z) {     // two groups of four columns
-        float4 a[2] = {};
-        float m = -INFINITY, l = 0.f;
-        constexpr int AT_ONCE = 8;                         // parts on their way at a time
-        for (int x0 = real ? first : part.last + 1; x0 <= part.last; x0 += AT_ONCE) {
-            float2 ml[AT_ONCE];
-            float4 o[AT_ONCE][2];
+    const int c = vec * 2;                             // two groups of four columns
+    float4 a[2] = {};
+    float m = -INFINITY, l = 0.f;
+    constexpr int AT_ONCE = 8;                         // parts on their way at a time
+    for (int x0 = real ? first : part.last + 1; x0 <= part.last; x0 += AT_ONCE) {
+        float2 ml[AT_ONCE];
+        float4 o[AT_ONCE][2];
 #pragma unroll
-            for (int k = 0; k < AT_ONCE; ++k) {
-                const PtResult<D>& res = result_of(min(x0 + k, part.last));
-                ml[k] = __ldcg(&res.ml[r]);
+        for (int k = 0; k < AT_ONCE; ++k) {
+            const PtResult<D>& res = result_of(min(x0 + k, part.last));
+            ml[k] = __ldcg(&res.ml[r]);
 #pragma unroll
-                for (int i = 0; i < 2; ++i) o[k][i] = __ldcg(&res.o[c + i][r]);
-            }
-            float m_new = m;
-#pragma unroll
-            for (int k = 0; k < AT_ONCE; ++k) m_new = fmaxf(m_new, ml[k].x);
-            const float mu = m_new == -INFINITY ? 0.f : m_new, old = ex2(m - mu);
-            l *= old;
-#pragma unroll
-            for (int i = 0; i < 2; ++i) { a[i].x *= old; a[i].y *= old; a[i].z *= old; a[i].w *= old; }
-#pragma unroll
-            for (int k = 0; k < AT_ONCE; ++k) {
-                if (x0 + k > part.last) break;
-                const float f = ex2(ml[k].x - mu);
-                l = fmaf(ml[k].y, f, l);
-#pragma unroll
-                for (int i = 0; i < 2; ++i) {
-                    a[i].x = fmaf(o[k][i].x, f, a[i].x); a[i].y = fmaf(o[k][i].y, f, a[i].y);
-                    a[i].z = fmaf(o[k][i].z, f, a[i].z); a[i].w = fmaf(o[k][i].w, f, a[i].w);
-                }
-            }
-            m = m_new;
+            for (int i = 0; i < 2; ++i) o[k][i] = __ldcg(&res.o[c + i][r]);
         }
-        const float inv = l != 0.f ? 1.f / l : 0.f;
+        float m_new = m;
 #pragma unroll
-        for (int i = 0; i < 2; ++i) {
-            if (p.o_f32) *reinterpret_cast<float4*>((float*)p.o + at + (c + i) * 4) = make_float4(a[i].x * inv, a[i].y * inv, a[i].z * inv, a[i].w * inv);
-            else *reinterpret_cast<uint2*>((__nv_bfloat16*)p.o + at + (c + i) * 4) = make_uint2(pack_bf16(a[i].x * inv, a[i].y * inv), pack_bf16(a[i].z * inv, a[i].w * inv));
+        for (int k = 0; k < AT_ONCE; ++k) m_new = fmaxf(m_new, ml[k].x);
+        const float mu = m_new == -INFINITY ? 0.f : m_new, old = ex2(m - mu);
+        l *= old;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) { a[i].x *= old; a[i].y *= old; a[i].z *= old; a[i].w *= old; }
+#pragma unroll
+        for (int k = 0; k < AT_ONCE; ++k) {
+            if (x0 + k > part.last) break;
+            const float f = ex2(ml[k].x - mu);
+            l = fmaf(ml[k].y, f, l);
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                a[i].x = fmaf(o[k][i].x, f, a[i].x); a[i].y = fmaf(o[k][i].y, f, a[i].y);
+                a[i].z = fmaf(o[k][i].z, f, a[i].z); a[i].w = fmaf(o[k][i].w, f, a[i].w);
+            }
         }
+        m = m_new;
     }
+    const float inv = l != 0.f ? 1.f / l : 0.f;
+#pragma unroll
+    for (int i = 0; i < 2 && there; ++i) {
+        if (p.o_f32) *reinterpret_cast<float4*>((float*)p.o + at + (c + i) * 4) = make_float4(a[i].x * inv, a[i].y * inv, a[i].z * inv, a[i].w * inv);
+        else *reinterpret_cast<uint2*>((__nv_bfloat16*)p.o + at + (c + i) * 4) = make_uint2(pack_bf16(a[i].x * inv, a[i].y * inv), pack_bf16(a[i].z * inv, a[i].w * inv));
+    }
+    if (p.counts[part.row * pairs + part.tile / 2] & kUnitMarked) add_not_finite<D>(p, part.row, part.tile, vec, r);
 }
 
 size_t paged_tile_count_bytes(int S, int H, int row_tiles) { return align_up((size_t)S * H * ((row_tiles + 1) / 2) * 4, 256); }

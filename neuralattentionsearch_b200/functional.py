@@ -657,7 +657,8 @@ class PagedKV:
 
     ``pages_k`` / ``pages_v`` bf16 [n,P,D]; ``refs`` int32 [n]: rows that hold a page; ``free_bits`` int32 [ceil(n/32)]: bit p % 32 of word
     p // 32 is set where page p is free; ``entries`` int32 [S,Hkv,M,4]: (page, position of its first token, last query position that
-    may see it, 0), the first ``n_pages`` int32 [S,Hkv] of a row in use, in the order of positions; ``length`` int32 [S]: tokens so far.
+    may see it, mark: 1 where V of the page holds a value that is not finite, else 0), the first ``n_pages`` int32 [S,Hkv] of a row in use, in the
+    order of positions; ``length`` int32 [S]: tokens so far.
     All contiguous.  ``scratch``: None, or a dict in which the calls on this cache keep their workspaces; its owner then sees to it that no two calls
     run at the same time, recorded ones among them.  ``paged_append``, ``paged_attention``, ``paged_evict`` and ``paged_reorder`` work on it; nothing is copied."""
 

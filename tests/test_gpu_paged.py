@@ -199,6 +199,104 @@ def test_what_nobody_sees_is_never_used(G, N, M):
     t.attend(N)
 
 
+def marks_wanted(t):
+    """[slot][head]: 1 for entries whose page holds a V that is not finite in a row that has been written"""
+    out = []
+    for s in range(t.S):
+        for h in range(t.H):
+            written = [min(t.P, t.model.length[s] - e[1]) for e in t.model.rows[s][h]]
+            out.append([int(not np.isfinite(t.model.v[e[0], :n]).all()) for e, n in zip(t.model.rows[s][h], written)])
+    return out
+
+
+def marks(t):
+    n, entries = t.kv.n_pages.cpu(), t.kv.entries.cpu()
+    return [entries[s, h, :n[s, h], 3].tolist() for s in range(t.S) for h in range(t.H)]
+
+
+def append_with(t, N, poison, n_new=None, dtype=torch.bfloat16, skip_hidden=False):
+    """Like Pair.append, with values (slot, head, token, channel, value) of V given; the model holds them as bf16"""
+    k, v = t.randn(t.S, t.H, N, t.D, dtype=dtype), t.randn(t.S, t.H, N, t.D, dtype=dtype)
+    for *at, value in poison:
+        v[tuple(at)] = value
+    roles = t.roles((N + 2 * t.P - 2) // t.P)
+    dev_n = None if n_new is None else torch.tensor(n_new, dtype=torch.int32, device=DEV)
+    t.F.paged_append(t.kv, k, v, torch.from_numpy(roles).to(DEV), t.SW, n_new=dev_n, skip_hidden=skip_hidden)
+    t.F.check_status()
+    t.model.append(bf16(k).double().cpu().numpy(), bf16(v).double().cpu().numpy(), roles, n_new or [N] * t.S, skip_hidden)
+
+
+@pytest.mark.parametrize('N', [1, 5, 40, 700])          # few tokens are copied by the kernel of the tables, many by one of their own
+@pytest.mark.parametrize('skip', [False, True])
+def test_pages_with_values_that_are_not_finite_are_marked(N, skip):
+    t = Pair(S=3, Hkv=2, G=1, P=16, D=64, SW=48, num_pages=600, M=150, seed=N)
+    nan, inf = float('nan'), float('inf')
+    n_new = [N, 0, N // 2 + 1]
+    poison = [(0, 0, N - 1, 63, nan), (0, 1, 0, 0, -inf), (1, 0, 0, 0, nan), (2, 0, N // 2, 8, inf), (2, 1, N // 3, 7, nan)]
+    poison += [(2, 0, N // 2 + 1, 3, nan)] if N > 2 else []           # behind the slot's tokens
+    append_with(t, 30, [(1, 1, 20, 5, inf)])
+    assert marks(t) == marks_wanted(t) == [[0, 0]] * 3 + [[0, 1]] + [[0, 0]] * 2
+    append_with(t, N, poison, n_new=n_new, skip_hidden=skip)
+    assert marks(t) == marks_wanted(t)
+    assert sum(map(sum, marks(t))) >= (4 if not skip else 2)
+    append_with(t, N, [], n_new=n_new)
+    assert marks(t) == marks_wanted(t)
+    before = marks(t)
+    src = [2, 0, 2]                                     # the copies of unfinished pages stay marked
+    t.F.paged_reorder(t.kv, torch.tensor(src, dtype=torch.int32, device=DEV))
+    t.model.reorder(src)
+    assert marks(t) == [before[2 * s + h] for s in src for h in range(2)] == marks_wanted(t)
+    t.F.paged_evict(t.kv)
+    t.model.evict()
+    assert marks(t) == marks_wanted(t)
+
+
+def test_fp32_values_that_bf16_cannot_hold_are_marked():
+    t = Pair(S=1, Hkv=1, G=1, P=16, D=64, SW=48, num_pages=20, M=20)
+    append_with(t, 40, [(0, 0, 3, 1, 3.4e38), (0, 0, 20, 1, 3.38e38)], dtype=torch.float32)       # the first one rounds to infinity
+    assert marks(t) == marks_wanted(t) == [[1, 0, 0]]
+
+
+@pytest.mark.parametrize('dtype', [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize('D', [64, 128])
+@pytest.mark.parametrize('M', [60, 2000])
+@pytest.mark.parametrize('G,N', [(1, 2), (2, 5), (4, 7), (4, 30), (4, 90), (3, 260)])
+def test_what_is_not_finite_stays_with_the_queries_that_see_it(G, N, M, D, dtype):
+    """NaN and infinities in V, and NaN in K, of tokens that some queries of the call see and others do not"""
+    P, nan, inf = 16, float('nan'), float('inf')
+    t = Pair(S=2, Hkv=2, G=G, P=P, D=D, SW=32, num_pages=300, M=M, seed=N)
+    t.append(200, n_new=[200, 191])
+    poison = [(s, h, N - 1, c, value) for s in range(2) for h in range(2) for c, value in ((2, nan), (3, -inf))]
+    poison += [(s, h, N // 2, D - 1, nan) for s in range(2) for h in range(2)]
+    append_with(t, N, poison)
+    for s in range(2):
+        first, last = t.model.length[s] - N, t.model.length[s] - 1
+        for h in range(2):
+            row = t.model.rows[s][h]
+            old = [i for i, e in enumerate(row) if e[1] + P <= first and e[2] >= first]
+            for i in old[1::2][-4:]:                    # pages that the call stops seeing on its way
+                row[i][2] = int(t.rng.integers(first, last + 1))
+                t.kv.entries[s, h, i, 2:] = torch.tensor([row[i][2], 1])
+                t.model.v[row[i][0], 3, 1] = inf
+                t.kv.pages_v[row[i][0], 3, 1] = inf
+    page, start, _ = t.model.rows[1][1][-1]             # the newest key of one head
+    t.model.k[page, last - start] = nan
+    t.kv.pages_k[page, last - start, 7:9] = nan
+    q = t.randn(2, 2 * G, N, D, dtype=dtype)
+    o = t.F.paged_attention(t.kv, q)
+    t.F.check_status()
+    with np.errstate(invalid='ignore'):
+        want, mag = t.model.attention(bf16(q).double().cpu().numpy(), [N, N], D ** -0.5)
+    got = o.double().cpu().numpy()
+    there = np.isfinite(want)
+    assert np.array_equal(np.isfinite(got), there)
+    assert np.array_equal(got[~there], want[~there], equal_nan=True)
+    assert 0.6 < there.mean() < 1 and there[..., 0].any(-1).all()
+    got, want, mag = got[there], want[there], mag[there]
+    worst = np.max(np.abs(got - want) - (2.0 ** -8 + 2e-4) * mag - (2.0 ** -8 * np.abs(want) if dtype == torch.bfloat16 else 0))
+    assert worst <= 1e-30, worst
+
+
 @pytest.mark.parametrize('M', [20, 2000])
 def test_a_call_without_new_tokens(M):
     t = Pair(S=2, Hkv=2, G=4, P=16, D=128, SW=32, num_pages=60, M=M, seed=1)
