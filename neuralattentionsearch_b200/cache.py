@@ -455,17 +455,20 @@ class NAtSCache:
     def reorder_cache(self, beam_idx: torch.Tensor):
         """Sequence b of every layer becomes a copy of what sequence ``beam_idx[b]`` was.  Only with ``pages``."""
         self._need_pages()
+        self.pages.take(sum(layer.reorder_pages() for layer in self.cache_model))      # for all layers, so that none is moved if one cannot be
         self.moves += 1
         for layer in self.cache_model:
-            layer.reorder(beam_idx)
-        self.cached_x = [None if x is None else x.index_select(0, beam_idx.to(x.device)) for x in self.cached_x]
+            layer.reorder(beam_idx, taken=True)
+        # a number out of range has raised the status word; it must not end the process here
+        self.cached_x = [None if x is None else x.index_select(0, beam_idx.to(x.device).clamp(0, x.shape[0] - 1)) for x in self.cached_x]
 
     def batch_repeat_interleave(self, repeats: int):
         """Every sequence ``repeats`` times, one after the other.  Only with ``pages``."""
         self._need_pages()
+        self.pages.take(sum(layer.reorder_pages(repeats) for layer in self.cache_model))
         self.moves += 1
         for layer in self.cache_model:
-            layer.repeat_interleave(repeats)
+            layer.repeat_interleave(repeats, taken=True)
         self.cached_x = [None if x is None else x.repeat_interleave(repeats, 0) for x in self.cached_x]
 
     def _need_pages(self):

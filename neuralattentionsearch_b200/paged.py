@@ -20,7 +20,8 @@ from . import functional as F_
 
 
 class KVPagePool:
-    """Pages for the K and V of any number of layer caches on one device: ``num_pages`` pages of ``page_size`` tokens of one kv-head."""
+    """Pages for the K and V of any number of layer caches on one device: ``num_pages`` pages of ``page_size`` tokens of one kv-head.
+    A cache gives its pages back in ``reset_cache``; one that is dropped without it keeps them."""
 
     def __init__(self, num_pages: int, page_size: int, head_dim: int, device: torch.device = torch.device('cuda')):
         if page_size not in F_.PAGE_SIZES:
@@ -208,21 +209,32 @@ class NAtSPagedLayerCache:
         self.chunk_fill_size = self._seen_tokens % self.chunk_size
 
     # ------------------------------------------------------------------ sequences
-    def reorder(self, src: torch.Tensor) -> None:
+    def reorder_pages(self, repeats: int = 1) -> int:
+        """Pages that ``reorder``, or ``repeat_interleave``, takes from the pool at most."""
+        if repeats < 1:
+            raise ValueError('repeats must be positive')
+        return self.bsz * repeats * self.n_msks if self.chunk_fill_size else 0
+
+    def reorder(self, src: torch.Tensor, taken: bool = False) -> None:
         """Sequence b becomes a copy of what sequence ``src[b]`` was (int [B]); whole pages are shared, the unfinished one is copied where
-        several sequences go on from it."""
+        several sequences go on from it.  ``taken``: the caller has asked the pool for ``reorder_pages()`` already."""
         if src.shape != (self.bsz,):
             raise ValueError(f'src must have shape [{self.bsz}]')
         if self._pending is not None:
             raise RuntimeError('post_update() has not been called for the first call yet')
-        if self.chunk_fill_size:
-            self.pool.take(self.bsz * self.n_msks)
+        if not taken:
+            self.pool.take(self.reorder_pages())
         F_.paged_reorder(self.kv, src.to(device=self.device, dtype=torch.int32).contiguous())
 
-    def repeat_interleave(self, repeats: int) -> None:
-        """Every sequence ``repeats`` times, one after the other: several replies to each prompt."""
-        if repeats < 1:
-            raise ValueError('repeats must be positive')
-        old = self.bsz
-        self._make_tables(old * repeats, self.kv.max_entries)
-        self.reorder(torch.arange(old, device=self.device).repeat_interleave(repeats))
+    def repeat_interleave(self, repeats: int, taken: bool = False) -> None:
+        """Every sequence ``repeats`` times, one after the other: several replies to each prompt.  ``taken``: as in ``reorder``."""
+        pages = self.reorder_pages(repeats)
+        if not taken:
+            self.pool.take(pages)
+        old, kv = self.bsz, self.kv
+        self._make_tables(old * repeats, kv.max_entries)
+        try:
+            self.reorder(torch.arange(old, device=self.device).repeat_interleave(repeats), taken=True)
+        except Exception:                             # refused, nothing has been launched: as it was
+            self.kv, self.bsz = kv, old
+            raise

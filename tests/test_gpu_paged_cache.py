@@ -119,6 +119,54 @@ def test_tables_grow_and_the_pool_runs_out():
     assert torch.isfinite(o).all() and lc.kv.length.item() == 977
 
 
+def _two_layers(num_pages, n=21):
+    """A cache of two layers with two sequences of ``n`` tokens (n % 16 of them in unfinished pages) and pooled states of the unfinished chunk"""
+    from neuralattentionsearch_b200 import KVPagePool, NAtSCache
+    g = torch.Generator(device=DEV).manual_seed(3)
+    cache = NAtSCache(32, 16, pages=KVPagePool(num_pages, 16, 64))
+    for layer in range(2):
+        k = randn(g, 2, 1, n, 64)
+        cache.update(k, k, layer, dict(token_states_info=torch.zeros(2, 1, -(-n // 16), dtype=torch.uint8, device=DEV)))
+        cache.cache_model[layer].post_update(n)
+        cache._set_cached_x(randn(g, 2, 1, 8), layer)
+    return cache
+
+
+def _tables(cache):
+    return [[t.tolist() for t in (c.kv.n_pages, c.kv.length, c.kv.entries[..., :2, :])] for c in cache.cache_model] + [cache.pages.refs.tolist()]
+
+
+def test_a_move_that_one_layer_has_no_pages_for_moves_none():
+    from neuralattentionsearch_b200 import _lib, check_status
+    cache = _two_layers(11)                             # eight pages held; a move may take two per layer, a second reply four
+    before, states = _tables(cache), [x.clone() for x in cache.cached_x]
+    with pytest.raises(_lib.NatsB200Error, match='4 pages'):
+        cache.reorder_cache(torch.tensor([1, 1], device=DEV))
+    with pytest.raises(_lib.NatsB200Error, match='8 pages'):
+        cache.batch_repeat_interleave(2)
+    with pytest.raises(ValueError, match='positive'):
+        cache.batch_repeat_interleave(0)
+    assert _tables(cache) == before and [c.bsz for c in cache.cache_model] == [2, 2]
+    assert all(torch.equal(a, b) for a, b in zip(states, cache.cached_x))
+    cache = _two_layers(50, n=32)                       # no unfinished pages; more slots than a table can have
+    before = _tables(cache)
+    with pytest.raises(_lib.NatsB200Error, match='slots'):
+        cache.batch_repeat_interleave(4000)
+    assert _tables(cache) == before and [c.bsz for c in cache.cache_model] == [2, 2]
+    cache.reorder_cache(torch.tensor([1, 0], device=DEV))
+    check_status()
+
+
+def test_a_beam_out_of_range_raises_the_status_word():
+    from neuralattentionsearch_b200 import _lib, check_status
+    cache = _two_layers(50)
+    cache.reorder_cache(torch.tensor([1, 7], device=DEV))
+    with pytest.raises(_lib.NatsB200Error, match='slot'):
+        check_status()
+    assert torch.equal(*[x[:1] for x in (cache.cached_x[0], cache.cached_x[0][1:])])
+    check_status()
+
+
 def _model():
     from neuralattentionsearch_b200.hf import TransformerArgs, enable_llama_nats_chunk_eval
     model = tiny_llama()
